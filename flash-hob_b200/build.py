@@ -21,8 +21,9 @@ CSRC = HERE / "csrc"
 OBJ = HERE / "build"
 OUT = HERE / "fhob" / "libfhob.so"
 NATIVE = HERE / "fhob" / "_native.so"          # host path of the Python package, against torch's C++ API
-NATIVE_SOURCE = "host_binding.cpp"
-SOURCES = ["fhob_api.cu", "simt_kernels.cu", "tc_kernels.cu", "tc_forward.cu", "tc_backward.cu", "static_scratch.cu"]
+NATIVE_SOURCES = ["host_binding.cpp", "host_layer.cpp"]
+SOURCES = ["fhob_api.cu", "simt_kernels.cu", "tc_kernels.cu", "tc_forward.cu", "tc_backward.cu", "static_scratch.cu",
+           "rotary.cu", "layer_norm.cu"]
 HEADERS = ["fhob_common.cuh", "sm100_ptx.cuh", "tc_common.cuh", "../../include/fhob.h"]
 FLAGS = ["-Xcompiler", "-fPIC", "-O3", "-std=c++17", "-lineinfo", "-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -38,27 +39,25 @@ def _newest_header() -> float:
 
 
 def _native_stale() -> bool:
-    deps = [CSRC / NATIVE_SOURCE, (CSRC / "../../include/fhob.h").resolve(), Path(__file__)]
+    deps = [*(CSRC / s for s in NATIVE_SOURCES), CSRC / "host_layer.h", (CSRC / "../../include/fhob.h").resolve(), Path(__file__)]
     return not NATIVE.exists() or NATIVE.stat().st_mtime < max(p.stat().st_mtime for p in deps)
 
 
-def _native_object(force: bool):
-    """Compiles the binding (no link yet: it needs libfhob.so); None when it is up to date."""
-    if not force and not _native_stale():
-        return None
+def _native_object(source: str) -> Path:
+    """Compiles a part of the binding (no link yet: it needs libfhob.so)."""
     import torch
     inc = Path(torch.__file__).parent / "include"
     cuda = Path(nvcc_path()).parent.parent / "include"
-    obj = OBJ / "host_binding.o"
+    obj = OBJ / (Path(source).stem + ".o")
     subprocess.run(["g++", "-c", "-O2", "-std=c++17", "-fPIC", "-Wno-interference-size", f"-I{inc}",
                     f"-I{inc}/torch/csrc/api/include", f"-I{cuda}", f"-I{sysconfig.get_paths()['include']}",
-                    str(CSRC / NATIVE_SOURCE), "-o", str(obj)], check=True)
+                    str(CSRC / source), "-o", str(obj)], check=True)
     return obj
 
 
-def _link_native(obj: Path) -> None:
+def _link_native(objs) -> None:
     import torch
-    subprocess.run(["g++", "-shared", str(obj), "-o", str(NATIVE), f"-L{Path(torch.__file__).parent / 'lib'}", "-lc10",
+    subprocess.run(["g++", "-shared", *(str(o) for o in objs), "-o", str(NATIVE), f"-L{Path(torch.__file__).parent / 'lib'}", "-lc10",
                     "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", f"-L{OUT.parent}", f"-l:{OUT.name}",
                     "-Wl,-rpath,$ORIGIN"], check=True)
 
@@ -84,13 +83,13 @@ def build(force: bool = False, verbose: bool = False) -> Path:
             subprocess.run([nvcc, "-c", *FLAGS, *extra, "-o", str(obj), str(CSRC / src)], check=True)
         return obj
 
-    with ThreadPoolExecutor(max_workers=len(SOURCES) + 1) as pool:
-        native = pool.submit(_native_object, force)
+    with ThreadPoolExecutor(max_workers=len(SOURCES) + len(NATIVE_SOURCES)) as pool:
+        native = [pool.submit(_native_object, s) for s in NATIVE_SOURCES] if force or _native_stale() else []
         objs = list(pool.map(compile_one, SOURCES))
-        native_obj = native.result()
+        native_objs = [n.result() for n in native]
     subprocess.run([nvcc, "-shared", *FLAGS, "-o", str(OUT)] + [str(o) for o in objs], check=True)
-    if native_obj is not None:
-        _link_native(native_obj)
+    if native_objs:
+        _link_native(native_objs)
     return OUT
 
 

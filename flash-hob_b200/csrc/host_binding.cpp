@@ -18,6 +18,7 @@
 #include <torch/extension.h>
 
 #include "../../include/fhob.h"
+#include "host_layer.h"
 
 namespace {
 
@@ -400,6 +401,11 @@ PyMethodDef g_methods[] = {
     {"backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_backward)), METH_FASTCALL, nullptr},
     {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_attention)), METH_FASTCALL, nullptr},
     {"use_workspaces", py_use_workspaces, METH_O, nullptr},
+    {"rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fhob_py_rotary)), METH_FASTCALL, nullptr},
+    {"layer_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fhob_py_layer_norm)), METH_FASTCALL, nullptr},
+    {"layer_norm_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fhob_py_layer_norm_forward)), METH_FASTCALL, nullptr},
+    {"layer_norm_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fhob_py_layer_norm_backward)), METH_FASTCALL, nullptr},
+    {"layer_norm_bwdbwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fhob_py_layer_norm_bwdbwd)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", "Native host path of fhob", -1, g_methods};
 

@@ -18,6 +18,8 @@ SYMBOLS = (
     "fhob_read_status", "fhob_forward", "fhob_backward", "fhob_bwdbwd_static_scratch",
     "fhob_selftest_expired_wait", "fhob_visible_tiles", "fhob_static_scratch_status",
     "fhob_workspace_bytes_problem", "fhob_cta_work",
+    "fhob_rotary", "fhob_layer_norm", "fhob_layer_norm_backward", "fhob_layer_norm_bwdbwd",
+    "fhob_layer_norm_workspace_bytes",
 )
 STATIC_SCRATCH_MAX_ROWS = 262144
 
@@ -41,6 +43,29 @@ class FhobProblem(C.Structure):
         ("dq2", C.c_void_p), ("dk2", C.c_void_p), ("dv2", C.c_void_p), ("ddo", C.c_void_p),
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
         ("layout", C.POINTER(FhobLayout)),
+    ]
+
+
+class FhobRotaryTensor(C.Structure):
+    _fields_ = [("in", C.c_void_p), ("out", C.c_void_p), ("heads", C.c_int32), ("reserved", C.c_int32),
+                ("row", C.c_int64), ("head", C.c_int64), ("batch", C.c_int64)]
+
+
+class FhobRotary(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("tensors", C.c_int32), ("tensor", FhobRotaryTensor * 2), ("batch", C.c_int64), ("n", C.c_int64),
+        ("d", C.c_int32), ("pairs", C.c_int32), ("axes", C.c_int32), ("interleaved", C.c_int32), ("inverse", C.c_int32),
+        ("positions_are_64_bit", C.c_int32), ("frequencies_are_64_bit", C.c_int32), ("reserved", C.c_int32),
+        ("positions", C.c_void_p), ("pos_axis", C.c_int64), ("pos_batch", C.c_int64), ("pos_n", C.c_int64),
+        ("frequencies", C.c_void_p), ("axis_of_pair", C.POINTER(C.c_uint8)),
+    ]
+
+
+class FhobLayerNorm(C.Structure):
+    _fields_ = [
+        ("rows", C.c_int64), ("cols", C.c_int32), ("dtype", C.c_int32), ("w_dtype", C.c_int32), ("eps", C.c_float),
+        ("x", C.c_void_p), ("x_row", C.c_int64), ("w", C.c_void_p), ("b", C.c_void_p), ("mean", C.c_void_p), ("rstd", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
     ]
 
 
@@ -85,6 +110,17 @@ def load() -> C.CDLL:
     lib.fhob_static_scratch_status.argtypes = [C.c_void_p]
     lib.fhob_forward.restype = C.c_int
     lib.fhob_forward.argtypes = [P, C.c_void_p, C.c_void_p, C.c_void_p]
+    lib.fhob_rotary.restype = C.c_int
+    lib.fhob_rotary.argtypes = [C.POINTER(FhobRotary), C.c_void_p]
+    N = C.POINTER(FhobLayerNorm)
+    lib.fhob_layer_norm_workspace_bytes.restype = C.c_size_t
+    lib.fhob_layer_norm_workspace_bytes.argtypes = [C.c_int32]
+    lib.fhob_layer_norm.restype = C.c_int
+    lib.fhob_layer_norm.argtypes = [N, C.c_void_p, C.c_void_p]
+    lib.fhob_layer_norm_backward.restype = C.c_int
+    lib.fhob_layer_norm_backward.argtypes = [N, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
+    lib.fhob_layer_norm_bwdbwd.restype = C.c_int
+    lib.fhob_layer_norm_bwdbwd.argtypes = [N, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64] + [C.c_void_p] * 6
     _lib = lib
     return lib
 

@@ -320,6 +320,86 @@ int fhob_bwdbwd_static_scratch(const FhobProblem* p, void* stream);
  */
 int fhob_static_scratch_status(void* stream);
 
+/* ---------------------------------------------------------------------------
+ * What such a layer runs around its attention.  The reference has none of it.
+ */
+
+/*
+ * Rotary positions with several axes (time, height, width).  The first 2 *
+ * pairs elements of every row of d are pairs - (j, pairs + j), or with
+ * `interleaved` the neighbours (2j, 2j + 1) - and pair j turns by the angle
+ * positions[axis_of_pair[j]] * frequencies[j] (`inverse`: by its negative,
+ * which is also the backward pass).  The other elements are copied.  One call
+ * takes up to two tensors of the same tokens (queries and keys, with heads of
+ * their own).  Positions may be any integers of their type; the angle is
+ * exact to position * frequency * 2^-52 radians.  Frequencies are finite.
+ * in: rows contiguous, other strides in elements, any alignment of whole
+ * elements.  out: contiguous (batch, heads, n, d), not overlapping in.
+ */
+#define FHOB_ROTARY_MAX_PAIRS 512
+#define FHOB_ROTARY_MAX_DIM 1024
+typedef struct FhobRotaryTensor {
+  const void* in;
+  void* out;
+  int32_t heads;
+  int32_t reserved;            /* must be 0 */
+  int64_t row, head, batch;    /* strides of in */
+} FhobRotaryTensor;
+typedef struct FhobRotary {
+  int32_t dtype;               /* FHOB_BF16, FHOB_F16 or FHOB_F32 */
+  int32_t tensors;             /* 1 or 2 */
+  FhobRotaryTensor tensor[2];
+  int64_t batch, n;
+  int32_t d, pairs;            /* 2 * pairs <= d */
+  int32_t axes;
+  int32_t interleaved, inverse;
+  int32_t positions_are_64_bit;
+  int32_t frequencies_are_64_bit;
+  int32_t reserved;            /* must be 0 */
+  const void* positions;       /* device, int32 or int64; strides of axes, batch entries and tokens: */
+  int64_t pos_axis, pos_batch, pos_n;
+  const void* frequencies;     /* device, `pairs` floats or doubles: radians per position */
+  const uint8_t* axis_of_pair; /* host, `pairs` numbers below `axes` */
+} FhobRotary;
+int fhob_rotary(const FhobRotary* r, void* stream);
+
+/*
+ * Layer norm over rows of `cols` elements, and its first and second
+ * derivatives: with mean and rstd = 1 / sqrt(var + eps) of a row and
+ * h = (x - mean) rstd, y = h w + b.  w and b may be NULL (ones, zeros); they and
+ * their gradients and cotangents are of type w_dtype, FHOB_F32 or dtype.
+ * Rows are contiguous, at any stride; results are contiguous.
+ *
+ * fhob_layer_norm           writes y, mean, rstd.
+ * fhob_layer_norm_backward  from the cotangent dy of y: dx, and dw = sum dy h,
+ *                           db = sum dy over the rows where they are not NULL.
+ * fhob_layer_norm_bwdbwd    from the cotangents ddx, ddw, ddb of dx, dw, db (any
+ *                           may be NULL: zero): the gradients ddy, dx2 and (unless
+ *                           NULL) dw2 of dy, x, w; mean and rstd are
+ *                           regarded as functions of x.
+ *
+ * The sums over rows need a workspace of fhob_layer_norm_workspace_bytes(cols)
+ * bytes, 256-byte aligned; they are added up in a fixed order.
+ */
+#define FHOB_LAYER_NORM_MAX_COLS 16384
+typedef struct FhobLayerNorm {
+  int64_t rows;
+  int32_t cols;
+  int32_t dtype, w_dtype;
+  float eps;                   /* fhob_layer_norm only; >= 0 */
+  const void* x;
+  int64_t x_row;               /* element stride between rows */
+  const void *w, *b;
+  float *mean, *rstd;          /* (rows): written by fhob_layer_norm, read by the others */
+  void* workspace;
+  size_t workspace_bytes;
+} FhobLayerNorm;
+size_t fhob_layer_norm_workspace_bytes(int32_t cols);
+int fhob_layer_norm(const FhobLayerNorm* n, void* y, void* stream);
+int fhob_layer_norm_backward(const FhobLayerNorm* n, const void* dy, int64_t dy_row, void* dx, void* dw, void* db, void* stream);
+int fhob_layer_norm_bwdbwd(const FhobLayerNorm* n, const void* dy, int64_t dy_row, const void* ddx, int64_t ddx_row, const void* ddw,
+                           const void* ddb, void* ddy, void* dx2, void* dw2, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
