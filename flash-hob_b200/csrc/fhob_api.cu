@@ -191,11 +191,28 @@ bool use_tc(const FhobProblem& p) {
   return tc_supported(p);
 }
 
+// The problem of a call with first tokens that stay visible: FHOB_ERR_ARG for sinks without a window.  Where that
+// leaves no key in front of a diagonal hidden, the mask is the window's (it hides none) or plainly causal.
+int attention_problem(const FhobProblem* p, int32_t sink_tokens, Problem* q) {
+  if (!p || sink_tokens < 0 || (sink_tokens > 0 && p->window <= 0)) return FHOB_ERR_ARG;
+  static_cast<FhobProblem&>(*q) = *p;
+  q->sinks = 0;
+  if (sink_tokens == 0 || p->window >= p->n_k) return FHOB_OK;
+  if (static_cast<long long>(sink_tokens) + p->window >= p->n_k) q->window = 0;
+  else q->sinks = sink_tokens;
+  return FHOB_OK;
+}
+Problem plain_problem(const FhobProblem& p) {
+  Problem q;
+  static_cast<FhobProblem&>(q) = p;
+  return q;
+}
+
 int run_pass(int pass, const FhobProblem* p, void* stream) {
   int st = validate(p, pass >= 3);
   if (st != FHOB_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return use_tc(*p) ? tc_pass(pass, *p, s) : simt_pass(pass, *p, s);
+  return use_tc(*p) ? tc_pass(pass, plain_problem(*p), s) : simt_pass(pass, plain_problem(*p), s);
 }
 
 }  // namespace
@@ -288,15 +305,21 @@ int fhob_pass12(const FhobProblem* p, void* stream) {
   int st = validate(p, false, true, true);
   if (st != FHOB_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (use_tc(*p)) return tc_pass(12, *p, s);
-  return simt_pass(12, *p, s);
+  if (use_tc(*p)) return tc_pass(12, plain_problem(*p), s);
+  return simt_pass(12, plain_problem(*p), s);
 }
 int fhob_pass3(const FhobProblem* p, void* stream) { return run_pass(3, p, stream); }
 int fhob_pass4(const FhobProblem* p, void* stream) { return run_pass(4, p, stream); }
 
-int fhob_bwdbwd(const FhobProblem* p, void* stream) {
-  int st = validate(p, true, true, true);
+int fhob_bwdbwd(const FhobProblem* p, void* stream) { return fhob_bwdbwd_sinks(p, 0, stream); }
+
+int fhob_bwdbwd_sinks(const FhobProblem* given, int32_t sink_tokens, void* stream) {
+  int st = validate(given, true, true, true);
   if (st != FHOB_OK) return st;
+  Problem problem;
+  st = attention_problem(given, sink_tokens, &problem);
+  if (st != FHOB_OK) return st;
+  const Problem* p = &problem;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   std::lock_guard<std::mutex> together(workspace_lock(p->workspace));
   // tensor cores: dd and b come out of one sweep (sum_j P dP = D makes b linear in sums that need no
@@ -345,10 +368,21 @@ int fhob_visible_tiles(int q_stationary, int m0, int rows, int tile, int n_q, in
   return FHOB_OK;
 }
 
+int fhob_visible_tiles_sinks(int q_stationary, int m0, int rows, int tile, int n_q, int n_k, int window, int sink_tokens,
+                             int* first, int* t_begin, int* t_end) {
+  if (!first || !t_begin || !t_end || rows <= 0 || tile <= 0 || n_q <= 0 || n_k <= 0 || m0 < 0 || window <= 0 || sink_tokens < 0)
+    return FHOB_ERR_ARG;
+  const TileList t = streamed_tiles(q_stationary != 0, m0, rows, tile, q_stationary ? n_k : n_q, n_k - n_q, 1, window, sink_tokens);
+  *first = t.first;
+  *t_begin = t.begin;
+  *t_end = t.begin + t.count - t.first;
+  return FHOB_OK;
+}
+
 int fhob_cta_work(const FhobProblem* p, int64_t block, int32_t* pass, int32_t* item, int32_t* part, int32_t* parts) {
   if (!p || !pass || !item || !part || !parts || block < 0 || p->bh <= 0 || p->n_q <= 0 || p->n_k <= 0) return FHOB_ERR_ARG;
   PairGrid g;
-  const int st = use_tc(*p) ? tc_grid(*p, &g) : simt_grid(*p, &g);
+  const int st = use_tc(*p) ? tc_grid(plain_problem(*p), &g) : simt_grid(plain_problem(*p), &g);
   if (st != FHOB_OK) return st;
   if (block >= g.blocks) return FHOB_ERR_ARG;
   const bool q_side = block < g.q_blocks;
@@ -367,7 +401,15 @@ int fhob_selftest_expired_wait(void* workspace, size_t workspace_bytes, void* st
 }
 
 int fhob_forward(const FhobProblem* p, void* o_out, float* lse_out, void* stream) {
-  if (!p || !p->q || !p->k || !p->v || !lse_out) return FHOB_ERR_ARG;
+  return fhob_forward_sinks(p, 0, o_out, lse_out, stream);
+}
+
+int fhob_forward_sinks(const FhobProblem* given, int32_t sink_tokens, void* o_out, float* lse_out, void* stream) {
+  Problem problem;
+  const int known = attention_problem(given, sink_tokens, &problem);
+  if (known != FHOB_OK) return known;
+  const Problem* p = &problem;
+  if (!p->q || !p->k || !p->v || !lse_out) return FHOB_ERR_ARG;
   if (p->bh <= 0 || p->n_q <= 0 || p->n_k <= 0 || p->d <= 0 || p->d > 128 || p->d_v < 0 || p->d_v > 128)
     return FHOB_ERR_SHAPE;
   if (p->dtype != FHOB_BF16 && p->dtype != FHOB_F32 && p->dtype != FHOB_F16) return FHOB_ERR_ARG;
@@ -399,9 +441,17 @@ int fhob_forward(const FhobProblem* p, void* o_out, float* lse_out, void* stream
 }
 
 int fhob_backward(const FhobProblem* p, void* dq, void* dk, void* dv, void* stream) {
+  return fhob_backward_sinks(p, 0, dq, dk, dv, stream);
+}
+
+int fhob_backward_sinks(const FhobProblem* given, int32_t sink_tokens, void* dq, void* dk, void* dv, void* stream) {
   if (!dq || !dk || !dv) return FHOB_ERR_ARG;
-  int st = validate(p, false, false);
+  int st = validate(given, false, false);
   if (st != FHOB_OK) return st;
+  Problem problem;
+  st = attention_problem(given, sink_tokens, &problem);
+  if (st != FHOB_OK) return st;
+  const Problem* p = &problem;
   if (!aligned16(dq) || !aligned16(dk) || !aligned16(dv)) return FHOB_ERR_ALIGN;
   std::lock_guard<std::mutex> together(workspace_lock(p->workspace));
   st = run_prepass(p, stream, false);  // stores -L*log2(e) and -D in the workspace

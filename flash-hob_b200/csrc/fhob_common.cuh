@@ -38,6 +38,12 @@ struct RowVectors {
   float* k23;   // -D*dd - b
 };
 
+// What the kernels' host side works on: the caller's problem and the first tokens that a sliding window leaves visible.
+// sinks > 0 only with a window that hides some key, and then sinks < n_k (see attention_problem in fhob_api.cu).
+struct Problem : FhobProblem {
+  int32_t sinks = 0;
+};
+
 // Head dim of V, ddV, dO, O and of the results ddO, dV2 (0 in the struct = same as d).
 inline int head_dim_v(const FhobProblem& p) { return p.d_v > 0 ? p.d_v : p.d; }
 
@@ -120,11 +126,12 @@ inline SplitBuffers split_buffers(const FhobProblem& p) {
 }
 
 // Mask of the reference (jax_refs/flash_impl.py:86-91): with off = n_k - n_q, key j is visible to
-// query i iff 0 <= i + off - j, and i + off - j < window when a sliding window is set.
-__host__ __device__ inline bool pair_visible(int qi, int kj, int off, int causal, int window) {
+// query i iff 0 <= i + off - j, and i + off - j < window when a sliding window is set.  The first `sinks` keys
+// stay visible behind the window.
+__host__ __device__ inline bool pair_visible(int qi, int kj, int off, int causal, int window, int sinks) {
   if (!causal) return true;
   const int dist = qi + off - kj;
-  return dist >= 0 && (window <= 0 || dist < window);
+  return dist >= 0 && (window <= 0 || dist < window || kj < sinks);
 }
 
 // Range [t_begin, t_end) of streamed tiles (tn rows each, n_strm rows in all) that can hold a
@@ -152,6 +159,32 @@ __host__ __device__ inline void visible_tiles(bool q_stationary, int m0, int tm,
   if (t_begin > t_end) t_begin = t_end;
 }
 
+// The streamed tiles of a stationary tile when the first keys stay visible behind the window.
+//  Queries stationary: first the tiles of those keys, then the window's from there on.  A tile that holds both is
+//  streamed twice, once for either kind of key, so that a row's visible keys are one interval in every tile: [0, sinks)
+//  or [max(window's first, sinks), diagonal].  (Only the queries near the start have such tiles.)
+//  Keys stationary: one range, up to the last query if one of the keys is a first one.
+struct TileList {
+  int first;   // the first keys' tiles are 0 .. first - 1 ...
+  int begin;   // ... and then come begin, begin + 1, ...
+  int count;   // in all
+  __host__ __device__ int tile(int i) const { return i < first ? i : begin + i - first; }
+};
+__host__ __device__ inline TileList streamed_tiles(bool q_stationary, int m0, int tm, int tn, int n_strm, int off, int causal, int window, int sinks) {
+  TileList t;
+  int end;
+  t.first = 0;
+  visible_tiles(q_stationary, m0, tm, tn, n_strm, off, causal, !q_stationary && m0 < sinks ? 0 : window, t.begin, end);
+  if (q_stationary && sinks > 0) {
+    const long seen = static_cast<long>(m0) + tm + off;   // keys the last query sees, were it not for the window
+    t.first = seen <= 0 ? 0 : static_cast<int>(((seen < sinks ? seen : sinks) + tn - 1) / tn);
+    if (t.begin < sinks / tn) t.begin = sinks / tn;
+    if (seen <= sinks || t.begin > end) t.begin = end;
+  }
+  t.count = t.first + end - t.begin;
+  return t;
+}
+
 // Per-thread record of the last CUDA error (read through fhob_last_cuda_error).
 void set_cuda_error(cudaError_t e, const char* where);
 void set_cuda_error_text(const char* text);
@@ -174,13 +207,13 @@ struct PairGrid {
   long long blocks;
 };
 // Grid of passes 3 and 4 of a whole problem; FHOB_ERR_SHAPE if it has too many CTAs
-int simt_grid(const FhobProblem& p, PairGrid* g);
-int tc_grid(const FhobProblem& p, PairGrid* g);
+int simt_grid(const Problem& p, PairGrid* g);
+int tc_grid(const Problem& p, PairGrid* g);
 
 // CUDA-core kernels (fp32 accumulate, any sizes): simt_kernels.cu
-int simt_pass(int pass, const FhobProblem& p, cudaStream_t s);
-int simt_forward(const FhobProblem& p, void* o_out, float* lse_out, int* status, cudaStream_t s);
-int simt_backward(const FhobProblem& p, void* dq, void* dk, void* dv, cudaStream_t s);
+int simt_pass(int pass, const Problem& p, cudaStream_t s);
+int simt_forward(const Problem& p, void* o_out, float* lse_out, int* status, cudaStream_t s);
+int simt_backward(const Problem& p, void* dq, void* dk, void* dv, cudaStream_t s);
 
 // tcgen05 / TMEM / TMA kernels (bf16, d in {64,128}): tc_kernels.cu
 bool tc_supported(const FhobProblem& p);
@@ -188,13 +221,13 @@ bool tc_split_supported(const FhobProblem& p);            // fp32 on the tensor 
 // which inputs tc_split_inputs copies (the operator needs all seven, the forward q, k, v, ...)
 enum { kSplitQ = 1, kSplitDDQ = 2, kSplitDO = 4, kSplitK = 8, kSplitDDK = 16, kSplitV = 32, kSplitDDV = 64, kSplitAll = 127 };
 int tc_split_inputs(const FhobProblem& p, cudaStream_t s, int which = kSplitAll);  // writes hi/lo copies into the workspace
-int tc_pass(int pass, const FhobProblem& p, cudaStream_t s);
-int tc_operator(const FhobProblem& p, cudaStream_t s);   // the whole double backward
+int tc_pass(int pass, const Problem& p, cudaStream_t s);
+int tc_operator(const Problem& p, cudaStream_t s);   // the whole double backward
 
 // tensor-core forward (O, L): tc_forward.cu, and first backward (dQ, dK, dV): tc_backward.cu
 bool tc_first_order_supported(const FhobProblem& p);
-int tc_forward(const FhobProblem& p, void* o_out, float* lse_out, int* status, cudaStream_t s);
-int tc_backward(const FhobProblem& p, void* dq, void* dk, void* dv, cudaStream_t s);
+int tc_forward(const Problem& p, void* o_out, float* lse_out, int* status, cudaStream_t s);
+int tc_backward(const Problem& p, void* dq, void* dk, void* dv, cudaStream_t s);
 int tc_selftest_expired_wait(int* status, cudaStream_t s);
 
 }  // namespace fhob

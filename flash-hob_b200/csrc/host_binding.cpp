@@ -28,7 +28,8 @@ PyObject* g_workspaces = nullptr;   // the package's dict (device, stream) -> wo
 
 struct Mask {
   bool causal;
-  int64_t window;   // 0 = none
+  int64_t window;      // 0 = none
+  int64_t sinks = 0;   // first tokens that stay visible behind it
 };
 
 // Index order of FhobLayout.
@@ -168,7 +169,7 @@ bool run_bwdbwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor*
   const Tensor* like[4] = {&q, &k, &v, &d_o};
   for (int i = 0; i < 4; ++i) out[i] = empty_like_shape(*like[i]);
   c.p.dq2 = out[0].data_ptr(); c.p.dk2 = out[1].data_ptr(); c.p.dv2 = out[2].data_ptr(); c.p.ddo = out[3].data_ptr();
-  return launched(c, [&] { return fhob_bwdbwd(&c.p, c.stream); });
+  return launched(c, [&] { return fhob_bwdbwd_sinks(&c.p, static_cast<int32_t>(m.sinks), c.stream); });
 }
 
 bool run_forward(const Tensor& q, const Tensor& k, const Tensor& v, double scale, const Mask& m, int impl, bool need_o,
@@ -184,7 +185,7 @@ bool run_forward(const Tensor& q, const Tensor& k, const Tensor& v, double scale
   }
   shape.pop_back();
   lse = at::detail::empty_cuda(shape, at::kFloat, q.device(), std::nullopt);
-  return launched(c, [&] { return fhob_forward(&c.p, need_o ? o.data_ptr() : nullptr, static_cast<float*>(lse.data_ptr()), c.stream); });
+  return launched(c, [&] { return fhob_forward_sinks(&c.p, static_cast<int32_t>(m.sinks), need_o ? o.data_ptr() : nullptr, static_cast<float*>(lse.data_ptr()), c.stream); });
 }
 
 bool run_backward(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& o, const Tensor& d_o, const Tensor& lse,
@@ -195,7 +196,7 @@ bool run_backward(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
   if (!take_workspace(c, ws)) return false;
   const Tensor* like[3] = {&q, &k, &v};
   for (int i = 0; i < 3; ++i) out[i] = empty_like_shape(*like[i]);
-  return launched(c, [&] { return fhob_backward(&c.p, out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), c.stream); });
+  return launched(c, [&] { return fhob_backward_sinks(&c.p, static_cast<int32_t>(m.sinks), out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), c.stream); });
 }
 
 // ---- fhob.attention: twice differentiable.  The derivative of the first backward is taken with O
@@ -207,6 +208,7 @@ py::dict mask_kwargs(const Mask& m) {
   py::dict kw;
   kw["is_causal"] = m.causal;
   kw["sliding_window"] = m.window ? py::cast(m.window) : py::object(py::none());
+  kw["sink_tokens"] = py::cast(m.sinks);
   return kw;
 }
 
@@ -215,12 +217,13 @@ using torch::autograd::variable_list;
 
 struct AttentionBackward : torch::autograd::Function<AttentionBackward> {
   static variable_list forward(AutogradContext* ctx, Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, Tensor d_o,
-                               double scale, bool causal, int64_t window) {
+                               double scale, bool causal, int64_t window, int64_t sinks) {
     ctx->save_for_backward({q, k, v, o, lse, d_o});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["window"] = window;
-    const Mask m{causal, window};
+    ctx->saved_data["sinks"] = sinks;
+    const Mask m{causal, window, sinks};
     py::gil_scoped_acquire gil;
     Tensor g[3];
     if (run_backward(q, k, v, o, d_o, lse, scale, m, FHOB_IMPL_AUTO, g)) return {g[0], g[1], g[2]};
@@ -229,7 +232,7 @@ struct AttentionBackward : torch::autograd::Function<AttentionBackward> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto s = ctx->get_saved_variables();
     const double scale = ctx->saved_data["scale"].toDouble();
-    const Mask m{ctx->saved_data["causal"].toBool(), ctx->saved_data["window"].toInt()};
+    const Mask m{ctx->saved_data["causal"].toBool(), ctx->saved_data["window"].toInt(), ctx->saved_data["sinks"].toInt()};
     py::gil_scoped_acquire gil;
     Tensor r[4];
     if (!run_bwdbwd(s[0], s[1], s[2], &s[3], s[5], g[0], g[1], g[2], s[4], scale, m, FHOB_IMPL_AUTO, r)) {
@@ -237,13 +240,13 @@ struct AttentionBackward : torch::autograd::Function<AttentionBackward> {
           s[0], s[1], s[2], s[3], s[5], g[0].contiguous(), g[1].contiguous(), g[2].contiguous(), s[4], scale, **mask_kwargs(m)));
       for (int i = 0; i < 4; ++i) r[i] = got[i];
     }
-    return {r[0], r[1], r[2], Tensor(), Tensor(), r[3], Tensor(), Tensor(), Tensor()};
+    return {r[0], r[1], r[2], Tensor(), Tensor(), r[3], Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 
 struct Attention : torch::autograd::Function<Attention> {
-  static Tensor forward(AutogradContext* ctx, Tensor q, Tensor k, Tensor v, double scale, bool causal, int64_t window) {
-    const Mask m{causal, window};
+  static Tensor forward(AutogradContext* ctx, Tensor q, Tensor k, Tensor v, double scale, bool causal, int64_t window, int64_t sinks) {
+    const Mask m{causal, window, sinks};
     Tensor o, lse;
     {
       py::gil_scoped_acquire gil;
@@ -257,13 +260,14 @@ struct Attention : torch::autograd::Function<Attention> {
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["window"] = window;
+    ctx->saved_data["sinks"] = sinks;
     return o;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto s = ctx->get_saved_variables();
     const auto r = AttentionBackward::apply(s[0], s[1], s[2], s[3].detach(), s[4], g[0], ctx->saved_data["scale"].toDouble(),
-                                            ctx->saved_data["causal"].toBool(), ctx->saved_data["window"].toInt());
-    return {r[0], r[1], r[2], Tensor(), Tensor(), Tensor()};
+                                            ctx->saved_data["causal"].toBool(), ctx->saved_data["window"].toInt(), ctx->saved_data["sinks"].toInt());
+    return {r[0], r[1], r[2], Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 
@@ -271,15 +275,19 @@ struct Attention : torch::autograd::Function<Attention> {
 
 const Tensor* tensor_arg(PyObject* o) { return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr; }
 
-// sliding_window: None, or a positive int together with a causal mask
-bool mask_args(PyObject* causal, PyObject* window, Mask& m) {
+// sliding_window: None, or a positive int together with a causal mask; sink_tokens: 0, or a positive int together with a window
+bool mask_args(PyObject* causal, PyObject* window, PyObject* sinks, Mask& m) {
   const int c = PyObject_IsTrue(causal);
   if (c < 0) { PyErr_Clear(); return false; }
   m.causal = c == 1;
   m.window = 0;
-  if (window == Py_None) return true;
-  if (!PyLong_CheckExact(window)) return false;
+  if (!PyLong_CheckExact(sinks)) return false;
   int overflow = 0;
+  const long long first = PyLong_AsLongLongAndOverflow(sinks, &overflow);
+  if (overflow || first < 0 || first > INT32_MAX) return false;
+  m.sinks = first;
+  if (window == Py_None) return first == 0;
+  if (!PyLong_CheckExact(window)) return false;
   const long long w = PyLong_AsLongLongAndOverflow(window, &overflow);
   if (overflow || w < 1 || w > INT32_MAX || !m.causal) return false;
   m.window = w;
@@ -306,12 +314,12 @@ PyObject* wrapped(const Tensor* t, int n) {
   return r;
 }
 
-// bwdbwd(Q, K, V, O, dO, ddQ, ddK, ddV, L, scale, is_causal, sliding_window, impl)
+// bwdbwd(Q, K, V, O, dO, ddQ, ddK, ddV, L, scale, is_causal, sliding_window, impl, sink_tokens)
 PyObject* py_bwdbwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Mask m;
   double scale;
-  if (n != 13 || !mask_args(a[10], a[11], m) || !scale_arg(a[9], scale)) Py_RETURN_NONE;
+  if (n != 14 || !mask_args(a[10], a[11], a[13], m) || !scale_arg(a[9], scale)) Py_RETURN_NONE;
   const Tensor* t[9];
   for (int i = 0; i < 9; ++i) {
     t[i] = tensor_arg(a[i]);
@@ -323,11 +331,11 @@ PyObject* py_bwdbwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// forward(Q, K, V, scale, is_causal, sliding_window, impl, need_o) -> (O, L) | (None, L)
+// forward(Q, K, V, scale, is_causal, sliding_window, impl, need_o, sink_tokens) -> (O, L) | (None, L)
 PyObject* py_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Mask m;
-  if (n != 8 || !mask_args(a[4], a[5], m)) Py_RETURN_NONE;
+  if (n != 9 || !mask_args(a[4], a[5], a[8], m)) Py_RETURN_NONE;
   const Tensor *q = tensor_arg(a[0]), *k = tensor_arg(a[1]), *v = tensor_arg(a[2]);
   if (!q || !k || !v || q->dim() < 1) Py_RETURN_NONE;
   double scale = 1.0 / std::sqrt(static_cast<double>(q->size(-1)));
@@ -344,12 +352,12 @@ PyObject* py_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// backward(Q, K, V, O, dO, L, scale, is_causal, sliding_window, impl) -> (dQ, dK, dV)
+// backward(Q, K, V, O, dO, L, scale, is_causal, sliding_window, impl, sink_tokens) -> (dQ, dK, dV)
 PyObject* py_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Mask m;
   double scale;
-  if (n != 10 || !mask_args(a[7], a[8], m) || !scale_arg(a[6], scale)) Py_RETURN_NONE;
+  if (n != 11 || !mask_args(a[7], a[8], a[10], m) || !scale_arg(a[6], scale)) Py_RETURN_NONE;
   const Tensor* t[6];
   for (int i = 0; i < 6; ++i)
     if (!(t[i] = tensor_arg(a[i]))) Py_RETURN_NONE;
@@ -359,10 +367,10 @@ PyObject* py_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// attention(q, k, v, scale, is_causal, window): window 0 = none (validated by the caller)
+// attention(q, k, v, scale, is_causal, window, sinks): window 0 = none (validated by the caller)
 PyObject* py_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  TORCH_CHECK_TYPE(n == 6, "attention takes 6 arguments");
+  TORCH_CHECK_TYPE(n == 7, "attention takes 7 arguments");
   const Tensor* t[3];
   for (int i = 0; i < 3; ++i) {
     t[i] = tensor_arg(a[i]);
@@ -370,12 +378,12 @@ PyObject* py_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   const double scale = PyFloat_AsDouble(a[3]);
   const int causal = PyObject_IsTrue(a[4]);
-  const long long window = PyLong_AsLongLong(a[5]);
+  const long long window = PyLong_AsLongLong(a[5]), sinks = PyLong_AsLongLong(a[6]);
   if (PyErr_Occurred()) return nullptr;
   Tensor o;
   try {
     pybind11::gil_scoped_release nogil;
-    o = Attention::apply(*t[0], *t[1], *t[2], scale, causal == 1, static_cast<int64_t>(window));
+    o = Attention::apply(*t[0], *t[1], *t[2], scale, causal == 1, static_cast<int64_t>(window), static_cast<int64_t>(sinks));
   } catch (py::error_already_set& e) {   // from the Python path: keep its type
     e.restore();
     return nullptr;

@@ -25,7 +25,7 @@ struct SimtParams {
   void *dq2, *dk2, *dv2, *ddo;
   const float *nlc, *k1;
   float *ndd, *k23;
-  int bh, n_q, n_k, d, dv, causal, window;
+  int bh, n_q, n_k, d, dv, causal, window, sinks;
   float scale;
   int q_blocks;           // the first q_blocks CTAs are query-tiled, the others key-tiled
   int items_q, items_k;   // (head, tile) pairs of either kind
@@ -192,6 +192,18 @@ __device__ __forceinline__ void store4(void* base, size_t at, const float2& a, c
   }
 }
 
+// Streamed tiles of an item.  Elements are masked pair by pair here, so a tile that holds both first keys and keys of
+// the window comes once.
+__device__ __forceinline__ TileList simt_tiles(bool q_stationary, int m0, int tile, int n_strm, const SimtParams& p) {
+  TileList list = streamed_tiles(q_stationary, m0, OM, tile, n_strm, p.n_k - p.n_q, p.causal, p.window, p.sinks);
+  if (list.begin < list.first) {
+    const int twice = min(list.first - list.begin, list.count - list.first);
+    list.begin += twice;
+    list.count -= twice;
+  }
+  return list;
+}
+
 template <typename T, int MODE>
 __device__ __forceinline__ void simt_body(const SimtParams& p, int block) {
   using C = Tiles<MODE>;
@@ -255,14 +267,14 @@ __device__ __forceinline__ void simt_body(const SimtParams& p, int block) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) out[i][j] = make_float2(0.f, 0.f);
 
-  int t_begin, t_end;
-  visible_tiles(kQStat, m0, OM, ON, n_strm, off, p.causal, p.window, t_begin, t_end);
+  const TileList list = simt_tiles(kQStat, m0, ON, n_strm, p);
+  int t_begin = 0, t_end = list.count;
   if (split > 1) split_range(begin_part, split, t_begin, t_end);
   if (padding) t_end = t_begin;
   const float sl2 = p.scale * kLog2e;
 
   for (int t = t_begin; t < t_end; ++t) {
-    const int n0 = t * ON;
+    const int n0 = list.tile(t) * ON;
     __syncthreads();   // the previous step has read its tiles
     load_side(strm, !kQStat, n0, ON);
     if (!kQStat && threadIdx.x < ON) {
@@ -287,7 +299,7 @@ __device__ __forceinline__ void simt_body(const SimtParams& p, int block) {
     auto allowed = [&](int i, int j) {
       if (!masked) return true;
       const int r = m0 + 4 * ty + i, c = n0 + tx + 8 * j;
-      return c < n_strm && pair_visible(kQStat ? r : c, kQStat ? c : r, off, p.causal, p.window);
+      return c < n_strm && pair_visible(kQStat ? r : c, kQStat ? c : r, off, p.causal, p.window, p.sinks);
     };
 
     float2 u0[4][4], u1[4][4];   // group 0: S, A2; group 1: dP, X
@@ -544,8 +556,8 @@ __global__ void __launch_bounds__(NT, 1) simt_forward_kernel(const __grid_consta
   const size_t qoff = static_cast<size_t>(bh) * p.n_q * d, ooff = static_cast<size_t>(bh) * p.n_q * dv;
   const size_t koff = static_cast<size_t>(bh) * p.n_k * d, voff = static_cast<size_t>(bh) * p.n_k * dv;
   const int off = p.n_k - p.n_q;
-  int t_begin, t_end;
-  visible_tiles(true, m0, OM, FN, p.n_k, off, p.causal, p.window, t_begin, t_end);
+  const TileList list = simt_tiles(true, m0, FN, p.n_k, p);
+  int t_begin = 0, t_end = list.count;
   if (split > 1) split_range(part, split, t_begin, t_end);
   if (!live) t_end = t_begin;
   const float sl2 = p.scale * kLog2e;
@@ -559,11 +571,11 @@ __global__ void __launch_bounds__(NT, 1) simt_forward_kernel(const __grid_consta
     acc[i][0] = acc[i][1] = make_float2(0.f, 0.f);
   }
   load_rows_any<T>(qs, p.q, qoff, m0, OM, p.n_q, d, vec);
-  if (t_begin < t_end) load_rows_any<T>(ks, p.k, koff, t_begin * FN, FN, p.n_k, d, vec);
+  if (t_begin < t_end) load_rows_any<T>(ks, p.k, koff, list.tile(t_begin) * FN, FN, p.n_k, d, vec);
   loads_commit();
 
   for (int t = t_begin; t < t_end; ++t) {
-    const int n0 = t * FN;
+    const int n0 = list.tile(t) * FN;
     if (o_out) load_rows_any<T>(vs, p.v, voff, n0, FN, p.n_k, dv, vec);
     loads_commit();
     loads_landed_but_last();
@@ -588,7 +600,7 @@ __global__ void __launch_bounds__(NT, 1) simt_forward_kernel(const __grid_consta
       }
     }
     __syncthreads();   // K has been read
-    if (t + 1 < t_end) load_rows_any<T>(ks, p.k, koff, n0 + FN, FN, p.n_k, d, vec);
+    if (t + 1 < t_end) load_rows_any<T>(ks, p.k, koff, list.tile(t + 1) * FN, FN, p.n_k, d, vec);
     loads_commit();
 
     const bool masked = n0 + FN > p.n_k || (p.causal && (n0 + FN - 1 > m0 + off || (p.window > 0 && m0 + OM - 1 + off - n0 >= p.window)));
@@ -599,7 +611,7 @@ __global__ void __launch_bounds__(NT, 1) simt_forward_kernel(const __grid_consta
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int c = n0 + lane + 32 * j;
-        const bool ok = !masked || (c < p.n_k && pair_visible(row0 + i, c, off, p.causal, p.window));
+        const bool ok = !masked || (c < p.n_k && pair_visible(row0 + i, c, off, p.causal, p.window, p.sinks));
         sv[j] = ok ? (s[i][j].x + s[i][j].y) * sl2 : -INFINITY;
         mx = fmaxf(mx, sv[j]);
       }
@@ -703,13 +715,13 @@ __global__ void __launch_bounds__(NT, 1) simt_forward_kernel(const __grid_consta
 }
 
 
-SimtParams make_params(const FhobProblem& p) {
+SimtParams make_params(const Problem& p) {
   RowVectors rv = row_vectors(p);
   SimtParams s;
   s.q = p.q; s.k = p.k; s.v = p.v; s.d_o = p.d_o; s.ddq = p.ddq; s.ddk = p.ddk; s.ddv = p.ddv;
   s.dq2 = p.dq2; s.dk2 = p.dk2; s.dv2 = p.dv2; s.ddo = p.ddo;
   s.nlc = rv.nlc; s.k1 = rv.k1; s.ndd = rv.ndd; s.k23 = rv.k23;
-  s.bh = p.bh; s.n_q = p.n_q; s.n_k = p.n_k; s.d = p.d; s.dv = head_dim_v(p); s.causal = p.causal; s.window = p.window; s.scale = p.scale;
+  s.bh = p.bh; s.n_q = p.n_q; s.n_k = p.n_k; s.d = p.d; s.dv = head_dim_v(p); s.causal = p.causal; s.window = p.window; s.sinks = p.sinks; s.scale = p.scale;
   return s;
 }
 
@@ -720,14 +732,14 @@ SimtParams make_params(const FhobProblem& p) {
 // 8 heads N = 1024 1326 -> 1337, 64 heads 9333 -> 9596, causal 5174 -> 5371.
 constexpr SplitCost kSimtCost = {1.f, 0.5f, 1.f / 16};
 
-PairGrid modes_grid(const FhobProblem& p, bool q_side, bool k_side) {
+PairGrid modes_grid(const Problem& p, bool q_side, bool k_side) {
   const int tiles_q = (p.n_q + OM - 1) / OM, tiles_k = (p.n_k + OM - 1) / OM;
-  return pair_grid(q_side ? static_cast<long long>(tiles_q) * p.bh : 0, split_parts(tiles_q, longest(p.n_k, ON, OM, p.window), kSimtCost),
-                   k_side ? static_cast<long long>(tiles_k) * p.bh : 0, split_parts(tiles_k, longest(p.n_q, ON, OM, p.window), kSimtCost));
+  return pair_grid(q_side ? static_cast<long long>(tiles_q) * p.bh : 0, split_parts(tiles_q, longest(true, p.n_k, ON, OM, p.window, p.sinks), kSimtCost),
+                   k_side ? static_cast<long long>(tiles_k) * p.bh : 0, split_parts(tiles_k, longest(false, p.n_q, ON, OM, p.window, p.sinks), kSimtCost));
 }
 
 template <typename T, int MODE_Q, int MODE_K>
-int launch_modes(const FhobProblem& problem, SimtParams& p, bool q_side, bool k_side, cudaStream_t st) {
+int launch_modes(const Problem& problem, SimtParams& p, bool q_side, bool k_side, cudaStream_t st) {
   constexpr auto kernel = simt_pass_kernel<T, MODE_Q, MODE_K>;
   constexpr int kQ = Tiles<MODE_Q>::SMEM_BYTES, kK = Tiles<MODE_K ? MODE_K : MODE_Q>::SMEM_BYTES, kSmem = kQ > kK ? kQ : kK;
   const int ok = allow_smem(kernel, kSmem);
@@ -744,7 +756,7 @@ int launch_modes(const FhobProblem& problem, SimtParams& p, bool q_side, bool k_
 
 // `pass` as in the entry points; passes 1 and 2 are one sweep, whichever is asked for
 template <typename T>
-int dispatch_pass(int pass, const FhobProblem& p, cudaStream_t st) {
+int dispatch_pass(int pass, const Problem& p, cudaStream_t st) {
   SimtParams s = make_params(p);
   switch (pass) {
     case 1:
@@ -758,7 +770,7 @@ int dispatch_pass(int pass, const FhobProblem& p, cudaStream_t st) {
 }
 
 template <typename T>
-int launch_backward(const FhobProblem& p, void* dq, void* dk, void* dv, cudaStream_t st) {
+int launch_backward(const Problem& p, void* dq, void* dk, void* dv, cudaStream_t st) {
   SimtParams s = make_params(p);
   s.dq2 = dq; s.dk2 = dk; s.dv2 = dv;
   return launch_modes<T, 5, 6>(p, s, true, true, st);
@@ -766,7 +778,7 @@ int launch_backward(const FhobProblem& p, void* dq, void* dk, void* dv, cudaStre
 
 // The forward reads rows element by element if they are not whole, aligned 16-byte pieces.
 template <typename T>
-int launch_forward(const FhobProblem& p, void* o_out, float* lse_out, int* status, cudaStream_t st) {
+int launch_forward(const Problem& p, void* o_out, float* lse_out, int* status, cudaStream_t st) {
   constexpr auto kernel = simt_forward_kernel<T>;
   const int ok = allow_smem(kernel, kForwardSmem);
   if (ok != FHOB_OK) return ok;
@@ -776,7 +788,7 @@ int launch_forward(const FhobProblem& p, void* o_out, float* lse_out, int* statu
   const long long items = static_cast<long long>((p.n_q + OM - 1) / OM) * p.bh;
   if (items > 0x7fffffffLL) return FHOB_ERR_SHAPE;
   s.items_q = static_cast<int>(items);
-  s.split_q = s.cluster = split_parts((p.n_q + OM - 1) / OM, longest(p.n_k, FN, OM, p.window), kSimtCost);
+  s.split_q = s.cluster = split_parts((p.n_q + OM - 1) / OM, longest(true, p.n_k, FN, OM, p.window, p.sinks), kSimtCost);
   if (items * s.split_q > 0x7fffffffLL) return FHOB_ERR_SHAPE;
   FHOB_CUDA_OK(launch_pdl(kernel, static_cast<unsigned>(items * s.split_q), NT, kForwardSmem, s.cluster, st, s, o_out, lse_out, status, vec));
   return FHOB_OK;
@@ -784,26 +796,26 @@ int launch_forward(const FhobProblem& p, void* o_out, float* lse_out, int* statu
 
 }  // namespace
 
-int simt_grid(const FhobProblem& p, PairGrid* g) {
+int simt_grid(const Problem& p, PairGrid* g) {
   *g = modes_grid(p, true, true);
   return g->blocks > 0x7fffffffLL ? FHOB_ERR_SHAPE : FHOB_OK;
 }
 
-int simt_backward(const FhobProblem& p, void* dq, void* dk, void* dv, cudaStream_t st) {
+int simt_backward(const Problem& p, void* dq, void* dk, void* dv, cudaStream_t st) {
   if (p.d > 128 || head_dim_v(p) > 128) return FHOB_ERR_SHAPE;
   if (p.dtype == FHOB_F32) return launch_backward<float>(p, dq, dk, dv, st);
   if (p.dtype == FHOB_F16) return launch_backward<__half>(p, dq, dk, dv, st);
   return launch_backward<__nv_bfloat16>(p, dq, dk, dv, st);
 }
 
-int simt_pass(int pass, const FhobProblem& p, cudaStream_t st) {
+int simt_pass(int pass, const Problem& p, cudaStream_t st) {
   if (p.d > 128 || head_dim_v(p) > 128) return FHOB_ERR_SHAPE;
   if (p.dtype == FHOB_F32) return dispatch_pass<float>(pass, p, st);
   if (p.dtype == FHOB_F16) return dispatch_pass<__half>(pass, p, st);
   return dispatch_pass<__nv_bfloat16>(pass, p, st);
 }
 
-int simt_forward(const FhobProblem& p, void* o_out, float* lse_out, int* status, cudaStream_t st) {
+int simt_forward(const Problem& p, void* o_out, float* lse_out, int* status, cudaStream_t st) {
   if (p.d > 128 || head_dim_v(p) > 128) return FHOB_ERR_SHAPE;
   if (p.dtype == FHOB_F32) return launch_forward<float>(p, o_out, lse_out, status, st);
   if (p.dtype == FHOB_F16) return launch_forward<__half>(p, o_out, lse_out, status, st);

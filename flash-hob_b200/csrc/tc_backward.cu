@@ -71,7 +71,7 @@ struct BwParams {
   const float* k1;    // -D per query
   void *dq, *dk, *dv;
   int* status;
-  int n_q, n_k, causal, window;
+  int n_q, n_k, causal, window, sinks;
   int tiles_q, tiles_k;   // 128-row tiles of a head
   int items_q, items_k;   // (head, tile) pairs of the two halves
   int q_blocks;           // the first q_blocks CTAs are BQ
@@ -125,8 +125,8 @@ __device__ __forceinline__ void bw_body(const BwParams& p, int block) {
   const int m0 = tile * BM;
   const int n_stat = KSIDE ? p.n_k : p.n_q, n_strm = KSIDE ? p.n_q : p.n_k;
   const int off = p.n_k - p.n_q;
-  int t_begin, t_end;
-  visible_tiles(!KSIDE, m0, BM, BN, n_strm, off, p.causal, p.window, t_begin, t_end);
+  const TileList list = streamed_tiles(!KSIDE, m0, BM, BN, n_strm, off, p.causal, p.window, p.sinks);
+  int t_begin = 0, t_end = list.count;
   if (split > 1) split_range(part, split, t_begin, t_end);
   const int n_iter = live ? t_end - t_begin : 0;
   auto stat_map = [&](int i) { return &p.map[KSIDE ? kBwK + i : kBwQ + i]; };   // Q, dO | K, V
@@ -178,7 +178,7 @@ __device__ __forceinline__ void bw_body(const BwParams& p, int block) {
       load_tile<BM, DV, BM * 128>(smem + C::STAT0, stat_map(1), &bars->stat_full, m0, head_h, head_b);
       int issued0 = 0, issued1 = 0;
       for (int it = 0; it < n_iter; ++it) {
-        const int n0 = (t_begin + it) * BN, s1 = it % C::N1, s0 = it % C::N0;
+        const int n0 = list.tile(t_begin + it) * BN, s1 = it % C::N1, s0 = it % C::N0;
         if (!wait_bar(&bars->free1[s1], ((it / C::N1) & 1) ^ 1, bars, status)) break;
         mbar_arrive_expect_tx(&bars->full1[s1], C::TILE1);
         load_tile<BN, DV, BN * 128>(ring1 + s1 * C::SLOT1, strm_map(1), &bars->full1[s1], n0, head_h, head_b);
@@ -314,17 +314,18 @@ __device__ __forceinline__ void bw_body(const BwParams& p, int block) {
       hi = p.n_k - 1;
       if (p.causal && g_row + off < hi) hi = g_row + off;
       if (p.window > 0 && g_row + off - p.window + 1 > 0) lo = g_row + off - p.window + 1;
+      if (lo < p.sinks) lo = p.sinks;
     } else {
       lo = p.causal ? g_row - off : 0;
       if (lo < 0) lo = 0;
       hi = p.n_q - 1;
-      if (p.window > 0 && g_row - off + p.window - 1 < hi) hi = g_row - off + p.window - 1;
+      if (p.window > 0 && g_row >= p.sinks && g_row - off + p.window - 1 < hi) hi = g_row - off + p.window - 1;
     }
     bool ok = true;
     constexpr int NC = CPT / 32;
 
     // One streamed tile; tiles that need masking take a copy of the code of their own.
-    auto step = [&](auto masked_tile, int it, int col_base) {
+    auto step = [&](auto masked_tile, int it, int col_base, int lo, int hi) {
       constexpr bool kMasked = decltype(masked_tile)::value;
       const int ns = it % C::NS, nd = it % C::ND;
       uint32_t sv = 0;
@@ -405,18 +406,20 @@ __device__ __forceinline__ void bw_body(const BwParams& p, int block) {
     };
 
     for (int it = 0; it < n_iter; ++it) {
-      const int n0 = (t_begin + it) * BN;
+      const int n0 = list.tile(t_begin + it) * BN;
+      const bool first = !KSIDE && t_begin + it < list.first;   // a tile of the first keys: [0, sinks) of it
       bool masked = n0 + BN > n_strm;
       if (p.causal) {
         if (!KSIDE) masked = masked || (n0 + BN - 1 > m0 + off);
         else masked = masked || (n0 + off < m0 + BM - 1);
         if (p.window > 0) {
-          if (!KSIDE) masked = masked || (m0 + BM - 1 + off - n0 >= p.window);
+          if (!KSIDE) masked = masked || (first ? n0 + BN > p.sinks : m0 + BM - 1 + off - n0 >= p.window || n0 < p.sinks);
           else masked = masked || (n0 + BN - 1 + off - m0 >= p.window);
         }
       }
-      if (masked) step(std::true_type{}, it, n0 + half * CPT);
-      else step(std::false_type{}, it, n0 + half * CPT);
+      const int lo_t = first ? 0 : lo, hi_t = first && p.sinks <= hi ? p.sinks - 1 : hi;
+      if (masked) step(std::true_type{}, it, n0 + half * CPT, lo_t, hi_t);
+      else step(std::false_type{}, it, n0 + half * CPT, lo_t, hi_t);
       if (!ok) break;
     }
 
@@ -492,7 +495,7 @@ __global__ void __launch_bounds__(NTHREADS, 1) bw_kernel(const __grid_constant__
 
 // ------------------------------------------------------------------ host side
 template <int DQK, int DV, bool F16, bool SPLIT = false>
-int bw_launch(const FhobProblem& p, void* dq, void* dk, void* dv, cudaStream_t s) {
+int bw_launch(const Problem& p, void* dq, void* dk, void* dv, cudaStream_t s) {
   constexpr auto kernel = bw_kernel<DQK, DV, F16, SPLIT>;
   using CQ = BwCfg<false, DQK, DV, SPLIT>;
   using CK = BwCfg<true, DQK, DV, SPLIT>;
@@ -522,7 +525,7 @@ int bw_launch(const FhobProblem& p, void* dq, void* dk, void* dv, cudaStream_t s
   tp.heads = (!SPLIT && p.layout) ? p.layout->heads : p.bh;
   tp.d = p.d;
   tp.d_v = head_dim_v(p);
-  tp.n_q = p.n_q; tp.n_k = p.n_k; tp.causal = p.causal; tp.window = p.window; tp.scale = p.scale;
+  tp.n_q = p.n_q; tp.n_k = p.n_k; tp.causal = p.causal; tp.window = p.window; tp.sinks = p.sinks; tp.scale = p.scale;
   tp.tiles_q = (p.n_q + BM - 1) / BM;
   tp.tiles_k = (p.n_k + BM - 1) / BM;
   if (static_cast<long long>(tp.tiles_q > tp.tiles_k ? tp.tiles_q : tp.tiles_k) * p.bh > 0x3fffffffLL) return FHOB_ERR_SHAPE;
@@ -531,7 +534,7 @@ int bw_launch(const FhobProblem& p, void* dq, void* dk, void* dv, cudaStream_t s
   const int st = allow_smem(kernel, kSmem);
   if (st != FHOB_OK) return st;
   auto go = [&](bool q_side, bool k_side) -> int {
-    const PairGrid g = pair_grid(q_side ? tp.items_q : 0, tc_parts(p.n_q, p.n_k, p.window), k_side ? tp.items_k : 0, tc_parts(p.n_k, p.n_q, p.window));
+    const PairGrid g = pair_grid(q_side ? tp.items_q : 0, tc_parts(true, p), k_side ? tp.items_k : 0, tc_parts(false, p));
     if (g.blocks > 0x7fffffffLL) return FHOB_ERR_SHAPE;
     tp.split_q = g.split_q; tp.split_k = g.split_k;
     tp.cluster = g.cluster;
@@ -539,13 +542,13 @@ int bw_launch(const FhobProblem& p, void* dq, void* dk, void* dv, cudaStream_t s
     FHOB_CUDA_OK(launch_pdl(kernel, static_cast<unsigned>(g.blocks), NTHREADS, kSmem, g.cluster, s, tp));
     return FHOB_OK;
   };
-  if (!launch_apart(pair_grid(tp.items_q, tc_parts(p.n_q, p.n_k, p.window), tp.items_k, tc_parts(p.n_k, p.n_q, p.window)))) return go(true, true);
+  if (!launch_apart(pair_grid(tp.items_q, tc_parts(true, p), tp.items_k, tc_parts(false, p)))) return go(true, true);
   const int first = go(true, false);
   return first != FHOB_OK ? first : go(false, true);
 }
 
 template <bool F16>
-int bw_dims(const FhobProblem& p, void* dq, void* dk, void* dv, cudaStream_t s) {
+int bw_dims(const Problem& p, void* dq, void* dk, void* dv, cudaStream_t s) {
   // tile widths: the head dims rounded up to 64 or 128
   const int d_v = head_dim_v(p);
   if (p.d <= 64) return d_v <= 64 ? bw_launch<64, 64, F16>(p, dq, dk, dv, s) : bw_launch<64, 128, F16>(p, dq, dk, dv, s);
@@ -580,7 +583,7 @@ int tc_selftest_expired_wait(int* status, cudaStream_t s) {
 // holds the bf16 hi/lo copies (see tc_split_supported)
 bool tc_first_order_supported(const FhobProblem& p) { return tc_supported(p); }
 
-int tc_backward(const FhobProblem& p, void* dq, void* dk, void* dv, cudaStream_t s) {
+int tc_backward(const Problem& p, void* dq, void* dk, void* dv, cudaStream_t s) {
   if (!tc_first_order_supported(p)) return FHOB_ERR_SHAPE;
   int st = check_device();
   if (st != FHOB_OK) return st;

@@ -416,15 +416,19 @@ inline int split_parts(int stationary_tiles, int streamed_tiles, const SplitCost
   }
   return parts;
 }
-// Streamed tiles of `tile` rows that the longest item of `rows` stationary rows sees.
-inline int longest(int n, int tile, int rows, int window) {
+// Streamed tiles of `tile` rows that the longest item of `rows` stationary rows sees (`sinks`: first keys that stay
+// visible behind the window; every query streams their tiles, and they stream every query).
+inline int longest(bool q_stationary, int n, int tile, int rows, int window, int sinks) {
   const int all = (n + tile - 1) / tile;
-  const long long seen = window > 0 ? (static_cast<long long>(rows) + window - 2) / tile + 2 : all;
+  if (!q_stationary && sinks > 0) return all;
+  const long long seen = window > 0 ? (static_cast<long long>(rows) + window - 2) / tile + 2 + (sinks + tile - 1) / tile : all;
   return seen < all ? static_cast<int>(seen) : all;
 }
 
 // The tensor-core kernels: 128-row stationary tiles, streamed rows in units of 64.
-inline int tc_parts(int n_stat, int n_strm, int window) { return split_parts((n_stat + BM - 1) / BM, longest(n_strm, 64, BM, window)); }
+inline int tc_parts(bool q_stationary, const Problem& p) {
+  return split_parts(((q_stationary ? p.n_q : p.n_k) + BM - 1) / BM, longest(q_stationary, q_stationary ? p.n_k : p.n_q, 64, BM, p.window, p.sinks));
+}
 
 }  // namespace
 

@@ -63,7 +63,7 @@ struct FwParams {
   float* lse_out;
   void* o;
   int* status;
-  int n_q, n_k, causal, window;
+  int n_q, n_k, causal, window, sinks;
   int groups;     // CTAs per head: groups of `q_tiles` 128-query tiles
   int q_tiles;    // 1 or 2
   int items;      // heads * groups
@@ -127,19 +127,35 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
   // key tiles of the two query tiles (a tile beyond the last query has none and is left alone)
   auto m_of = [&](int x) { return (group * p.q_tiles + x) * BM; };
   auto live = [&](int x) { return x < p.q_tiles && m_of(x) < p.n_q; };
-  int begin[2], end[2];
+  // Tiles of the first keys (n_first, if any stay visible behind the window; both query tiles take those of the later
+  // one) and then of the window: query tile x has begin[x] .. end[x] - 1 of those.  Steps t count through the list:
+  // step t < n_first is key tile t, a later one is key tile w_begin + t - n_first.
+  int begin[2], end[2], n_first = 0;
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     begin[x] = end[x] = 0;
     if (live(x)) {
-      visible_tiles(true, m_of(x), BM, BN, p.n_k, off, p.causal, p.window, begin[x], end[x]);
-      if (p.split > 1) split_range(part, p.split, begin[x], end[x]);
+      const TileList list = streamed_tiles(true, m_of(x), BM, BN, p.n_k, off, p.causal, p.window, p.sinks);
+      n_first = max(n_first, list.first);
+      begin[x] = list.begin;
+      end[x] = list.begin + list.count - list.first;
     }
   }
   const bool any0 = end[0] > begin[0], any1 = end[1] > begin[1];
-  const int t_begin = any0 && any1 ? min(begin[0], begin[1]) : (any0 ? begin[0] : begin[1]);
-  const int t_end = any0 && any1 ? max(end[0], end[1]) : (any0 ? end[0] : end[1]);
-  const int n_tiles = t_end > t_begin ? t_end - t_begin : 0;
+  const int w_begin = any0 && any1 ? min(begin[0], begin[1]) : (any0 ? begin[0] : begin[1]);
+  const int w_end = any0 && any1 ? max(end[0], end[1]) : (any0 ? end[0] : end[1]);
+  int t_begin = 0, t_end = n_first + (w_end > w_begin ? w_end - w_begin : 0);
+  if (p.split > 1) split_range(part, p.split, t_begin, t_end);   // (query tile A only: it has every step)
+  const int n_tiles = t_end - t_begin;
+  auto key_tile = [&](int t) { return t < n_first ? t : w_begin + t - n_first; };
+  auto active = [&](int x, int t) {
+    if (t < n_first) return live(x) && t < t_end;
+    const int tile = w_begin + t - n_first;
+    return t < t_end && tile >= begin[x] && tile < end[x];
+  };
+  auto skipped = [&](int x) { return end[x] > begin[x] ? begin[x] - w_begin : 0; };   // steps between the first keys and x's window
+  auto step_no = [&](int x, int t) { return t - t_begin - (t < n_first ? 0 : skipped(x)); };   // how many steps of x come before t
+  auto steps = [&](int x) { return p.split > 1 ? (x == 0 ? n_tiles : 0) : (live(x) ? n_first : 0) + end[x] - begin[x]; };
 
   int fault = 0;   // thread 0: what to report at the end
   if (threadIdx.x == 0) {
@@ -197,7 +213,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
       const int head_b = head / p.heads, head_h = head - head_b * p.heads;   // batch entry and head within it
 #pragma unroll
       for (int x = 0; x < 2; ++x)
-        if (end[x] > begin[x]) {
+        if (steps(x) > 0) {
           mbar_arrive_expect_tx(&bars->q_full[x], C::Q_BYTES);
           load_tile<BM, DQK, BM * 128>(smem + x * C::Q_BYTES, &p.q, &bars->q_full[x], m_of(x), head_h, head_b);
         }
@@ -207,7 +223,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
         const int slot = i % C::NSLOT;
         if (!wait_bar(&bars->kv_free[slot], ((i / C::NSLOT) & 1) ^ 1, bars, p.status)) break;
         const bool is_v = OUT && (kStages == 1 ? (i & 1) != 0 : i > 0 && (i % 2 == 0 || i == n_loads - 1));
-        const int j = !OUT ? i : (kStages == 1 ? i >> 1 : (is_v ? (i - 1) >> 1 : (i + 1) >> 1)), n0 = (t_begin + j) * BN;
+        const int j = !OUT ? i : (kStages == 1 ? i >> 1 : (is_v ? (i - 1) >> 1 : (i + 1) >> 1)), n0 = key_tile(t_begin + j) * BN;
         uint8_t* dst = ring + slot * C::SLOT_BYTES;
         if (is_v) {
           mbar_arrive_expect_tx(&bars->kv_full[slot], BN * DV * 2);
@@ -221,7 +237,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
       // drain: every load issued above must have landed before the CTA may exit
 #pragma unroll
       for (int x = 0; x < 2; ++x)
-        if (end[x] > begin[x]) wait_landed(&bars->q_full[x], 0, p.status);
+        if (steps(x) > 0) wait_landed(&bars->q_full[x], 0, p.status);
       for (int i = issued > C::NSLOT ? issued - C::NSLOT : 0; i < issued; ++i)
         wait_landed(&bars->kv_full[i % C::NSLOT], (i / C::NSLOT) & 1, p.status);
     }
@@ -239,10 +255,9 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
         ok = ok && wait_bar(bar, parity, bars, p.status);
         return ok;
       };
-      auto active = [&](int x, int t) { return t >= begin[x] && t < end[x]; };
       // S_x(t) = Q_x . K(t)^T; the slot is handed back after its last product
       auto scores = [&](int x, int t) {
-        const int i = k_load(t - t_begin), slot = i % C::NSLOT, it = t - begin[x], stage = it % kStages;
+        const int i = k_load(t - t_begin), slot = i % C::NSLOT, it = step_no(x, t), stage = it % kStages;
         if (it == 0 && !wait(&bars->q_full[x], 0)) return;
         if (!OUT && !wait(&bars->s_free[x][stage], ((it / kStages) & 1) ^ 1)) return;
         if (!wait(&bars->kv_full[slot], (i / C::NSLOT) & 1)) return;
@@ -263,7 +278,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
       };
       // O_x += P_x . V(t)
       auto output = [&](int x, int t) {
-        const int i = v_load(t - t_begin), slot = i % C::NSLOT, it = t - begin[x], stage = it % kStages;
+        const int i = v_load(t - t_begin), slot = i % C::NSLOT, it = step_no(x, t), stage = it % kStages;
         if (!wait(kHalves ? &bars->p_half[x] : &bars->p_full[x][stage], (it / kStages) & 1)) return;
         if (!wait(&bars->kv_full[slot], (i / C::NSLOT) & 1)) return;
         tc_fence_after();
@@ -287,7 +302,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
             umma_ts_split(o_cols(x) + 64, s_cols(x, stage) + BN / 2 + 8 * ks, b + ((ks * 2048) >> 4), kDescHi, idesc_o64, 1u);
         }
         umma_commit(&bars->o_done[x]);
-        if (t + 1 == end[x]) umma_commit(&bars->out_full[x]);
+        if (it + 1 == steps(x)) umma_commit(&bars->out_full[x]);
         if (x == 1 || !active(1, t)) umma_commit(&bars->kv_free[slot]);
       };
       if (OUT) {
@@ -316,18 +331,19 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const int m0 = m_of(x), g_row = m0 + row;
-    const int n_iter = end[x] - begin[x], t0 = begin[x];
+    const int n_iter = steps(x);
     const float sl2 = p.scale * kLog2e, abs_sl2 = fabsf(sl2);
     // visible keys of this row
     int lo = 0, hi = p.n_k - 1;
     if (p.causal && g_row + off < hi) hi = g_row + off;
     if (p.window > 0 && g_row + off - p.window + 1 > 0) lo = g_row + off - p.window + 1;
+    if (lo < p.sinks) lo = p.sinks;
     float run_m = -INFINITY, run_l = 0.f;   // reference maximum (log2 domain) and sum of exponentials
     bool ok = true;
     const uint32_t o_addr = lane_base + o_cols(x);
 
     // One key tile; tiles that need masking take a copy of the code of their own.
-    auto step = [&](auto masked_tile, int it, int n0, int stage) {
+    auto step = [&](auto masked_tile, int it, int n0, int stage, int lo, int hi) {
       ok = __all_sync(0xffffffffu, wait_bar(&bars->s_full[x][stage], (it / kStages) & 1, bars, p.status));
       if (!ok) return;
       tc_fence_after();
@@ -430,15 +446,19 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
       }
     };
     for (int it = 0; it < n_iter; ++it) {
-      const int n0 = (t0 + it) * BN, stage = it % kStages;
+      int t = t_begin + it;
+      const bool first = t < n_first;   // a tile of the first keys: [0, sinks) of it
+      if (!first) t += skipped(x);
+      const int n0 = key_tile(t) * BN, stage = it % kStages;
       // does any score of this tile need masking?  (uniform over the tile's warps)
       bool masked = n0 + BN > p.n_k;
       if (p.causal) {
         masked = masked || (n0 + BN - 1 > m0 + off);
-        if (p.window > 0) masked = masked || (m0 + BM - 1 + off - n0 >= p.window);
+        if (p.window > 0) masked = masked || (first ? n0 + BN > p.sinks : m0 + BM - 1 + off - n0 >= p.window || n0 < p.sinks);
       }
-      if (masked) step(std::true_type{}, it, n0, stage);
-      else step(std::false_type{}, it, n0, stage);
+      const int lo_t = first ? 0 : lo, hi_t = first && p.sinks <= hi ? p.sinks - 1 : hi;
+      if (masked) step(std::true_type{}, it, n0, stage, lo_t, hi_t);
+      else step(std::false_type{}, it, n0, stage, lo_t, hi_t);
       if (!ok) break;
     }
 
@@ -548,7 +568,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
 
 // ------------------------------------------------------------------ host side
 template <int DQK, int DV, bool F16, bool SPLIT, bool OUT>
-int fw_launch(const FhobProblem& p, void* o_out, float* lse_out, int* status, cudaStream_t s) {
+int fw_launch(const Problem& p, void* o_out, float* lse_out, int* status, cudaStream_t s) {
   using C = FwCfg<DQK, DV, OUT>;
   constexpr auto kernel = fw_kernel<DQK, DV, F16, SPLIT, OUT>;
   FwParams tp;
@@ -570,14 +590,14 @@ int fw_launch(const FhobProblem& p, void* o_out, float* lse_out, int* status, cu
   tp.lse_out = lse_out;
   tp.o = o_out;
   tp.status = status;
-  tp.n_q = p.n_q; tp.n_k = p.n_k; tp.causal = p.causal; tp.window = p.window;
+  tp.n_q = p.n_q; tp.n_k = p.n_k; tp.causal = p.causal; tp.window = p.window; tp.sinks = p.sinks;
   tp.heads = (!SPLIT && p.layout) ? p.layout->heads : p.bh;
   tp.d_v = dv;
   tp.scale = p.scale;
   const int tiles = (p.n_q + BM - 1) / BM;
   if (static_cast<long long>(tiles) * p.bh > 0x7fffffffLL) return FHOB_ERR_SHAPE;
   // A head of one query tile may split its keys (a second tile would cost the parts more than they save).
-  tp.split = tiles == 1 ? tc_parts(p.n_q, p.n_k, p.window) : 1;
+  tp.split = tiles == 1 ? tc_parts(true, p) : 1;
   // Two query tiles a CTA hide each other's latency and share K and V; a tile takes as long alone, so
   // when single tiles fit the GPU at once, a CTA has one.  (The bits are the same.)
   tp.q_tiles = tiles == 1 || static_cast<long long>(tiles) * p.bh <= sm_count() ? 1 : 2;
@@ -590,14 +610,14 @@ int fw_launch(const FhobProblem& p, void* o_out, float* lse_out, int* status, cu
 }
 
 template <int DQK, int DV, bool F16, bool SPLIT = false>
-int fw_dispatch(const FhobProblem& p, void* o_out, float* lse_out, int* status, cudaStream_t s) {
+int fw_dispatch(const Problem& p, void* o_out, float* lse_out, int* status, cudaStream_t s) {
   // no O wanted: the scores alone (no tile of the second head dim is touched)
   return o_out ? fw_launch<DQK, DV, F16, SPLIT, true>(p, o_out, lse_out, status, s)
                : fw_launch<DQK, DQK, F16, SPLIT, false>(p, o_out, lse_out, status, s);
 }
 
 template <bool F16>
-int fw_dims(const FhobProblem& p, void* o_out, float* lse_out, int* status, cudaStream_t s) {
+int fw_dims(const Problem& p, void* o_out, float* lse_out, int* status, cudaStream_t s) {
   // tile widths: the head dims rounded up to 64 or 128
   const int dv = head_dim_v(p);
   if (p.d <= 64)
@@ -607,7 +627,7 @@ int fw_dims(const FhobProblem& p, void* o_out, float* lse_out, int* status, cuda
 
 }  // namespace
 
-int tc_forward(const FhobProblem& p, void* o_out, float* lse_out, int* status, cudaStream_t s) {
+int tc_forward(const Problem& p, void* o_out, float* lse_out, int* status, cudaStream_t s) {
   if (!tc_first_order_supported(p)) return FHOB_ERR_SHAPE;
   int st = check_device();
   if (st != FHOB_OK) return st;

@@ -120,7 +120,7 @@ struct TcParams {
   long long lse_head, lse_batch;
   void *dq2, *ddo, *dk2, *dv2;
   int* status;
-  int n_q, n_k, causal, window;
+  int n_q, n_k, causal, window, sinks;
   int tiles_q, tiles_k;   // 128-row tiles of a head
   int q_blocks;           // passes 3 and 4 in one launch: the first q_blocks CTAs are pass 3
   int items_q, items_k;   // (head, tile) pairs of the query-tiled and key-tiled passes
@@ -453,8 +453,8 @@ __device__ __forceinline__ void tc_pass_body(const TcParams& p, int block) {
   const int n_strm = kQStat ? p.n_k : p.n_q;
   const int off = p.n_k - p.n_q;
 
-  int t_begin, t_end;
-  visible_tiles(kQStat, m0, BM, BN, n_strm, off, p.causal, p.window, t_begin, t_end);
+  const TileList list = streamed_tiles(kQStat, m0, BM, BN, n_strm, off, p.causal, p.window, p.sinks);
+  int t_begin = 0, t_end = list.count;
   if (split > 1) split_range(part, split, t_begin, t_end);
   const int n_iter = live ? t_end - t_begin : 0;
 
@@ -526,7 +526,7 @@ __device__ __forceinline__ void tc_pass_body(const TcParams& p, int block) {
         if (!wait_bar(&bars->strm_free[slot], ((it / C::NSLOT) & 1) ^ 1, bars, p.status)) break;
         mbar_arrive_expect_tx(&bars->strm_full[slot], C::SLOT_BYTES);
         uint8_t* dst = strm_tiles + slot * C::SLOT_BYTES;
-        const int n0 = (t_begin + it) * BN;
+        const int n0 = list.tile(t_begin + it) * BN;
 #pragma unroll
         for (int i = 0; i < C::NSTRM; ++i) {
           uint8_t* at = dst + C::strm_base(i);
@@ -754,18 +754,25 @@ __device__ __forceinline__ void tc_pass_body(const TcParams& p, int block) {
       c.hi = p.n_k - 1;
       if (p.causal && g_row + off < c.hi) c.hi = g_row + off;
       if (p.window > 0 && g_row + off - p.window + 1 > 0) c.lo = g_row + off - p.window + 1;
+      if (c.lo < p.sinks) c.lo = p.sinks;
     } else {
       c.lo = p.causal ? g_row - off : 0;
       if (c.lo < 0) c.lo = 0;
       c.hi = p.n_q - 1;
-      if (p.window > 0 && g_row - off + p.window - 1 < c.hi) c.hi = g_row - off + p.window - 1;
+      if (p.window > 0 && g_row >= p.sinks && g_row - off + p.window - 1 < c.hi) c.hi = g_row - off + p.window - 1;
     }
+    [[maybe_unused]] const int row_lo = c.lo, row_hi = c.hi;
     float2 racc[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
     float2& rowacc = racc[0];
     bool ok = true;
 
     for (int it = 0; it < n_iter; ++it) {
-      const int n0 = (t_begin + it) * BN;
+      const int n0 = list.tile(t_begin + it) * BN;
+      const bool first = kQStat && t_begin + it < list.first;   // a tile of the first keys: [0, sinks) of it
+      if (kQStat && list.first > 0) {
+        c.lo = first ? 0 : row_lo;
+        c.hi = first && p.sinks <= row_hi ? p.sinks - 1 : row_hi;
+      }
       // does any element of this tile need masking?  (CTA-uniform: depends on tile coordinates only)
       bool masked = n0 + BN > n_strm;
       if (p.causal) {
@@ -773,7 +780,7 @@ __device__ __forceinline__ void tc_pass_body(const TcParams& p, int block) {
         else masked = masked || (n0 + off < m0 + BM - 1);
         if (p.window > 0) {
           // the pair of the tile that is furthest apart: last query row against first key row
-          if (kQStat) masked = masked || (m0 + BM - 1 + off - n0 >= p.window);
+          if (kQStat) masked = masked || (first ? n0 + BN > p.sinks : m0 + BM - 1 + off - n0 >= p.window || n0 < p.sinks);
           else masked = masked || (n0 + BN - 1 + off - m0 >= p.window);
         }
       }
@@ -1052,17 +1059,17 @@ __global__ void split_rows_kernel(const __grid_constant__ SplitJobs jobs) {
   dst[row * 64 + 32 + c2] = lo;
 }
 
-int first_live_query(const FhobProblem& p) {
+int first_live_query(const Problem& p) {
   // bottom-right aligned causal mask: query i sees key 0 only if i + n_k - n_q >= 0
   return (p.causal && p.n_q > p.n_k) ? p.n_q - p.n_k : 0;
 }
 
-bool tc_items_fit(const FhobProblem& p) {   // both passes together stay below 2^31 items
+bool tc_items_fit(const Problem& p) {   // both passes together stay below 2^31 items
   return (static_cast<long long>(p.n_q > p.n_k ? p.n_q : p.n_k) + BM - 1) / BM * p.bh <= 0x3fffffffLL;
 }
 
 template <bool F16, bool SPLIT>
-int fill_params(const FhobProblem& p, TcParams& tp) {
+int fill_params(const Problem& p, TcParams& tp) {
   if (!tc_items_fit(p)) return FHOB_ERR_SHAPE;
   RowVectors rv = row_vectors(p);
   const void* mats[kMaps] = {p.q, p.ddq, p.d_o, p.k, p.ddk, p.v, p.ddv};
@@ -1092,7 +1099,7 @@ int fill_params(const FhobProblem& p, TcParams& tp) {
   tp.lse_batch = p.layout ? p.layout->lse_batch : static_cast<long long>(p.bh) * p.n_q;
   tp.dq2 = p.dq2; tp.ddo = p.ddo; tp.dk2 = p.dk2; tp.dv2 = p.dv2;
   tp.status = rv.status;
-  tp.n_q = p.n_q; tp.n_k = p.n_k; tp.causal = p.causal; tp.window = p.window; tp.scale = p.scale;
+  tp.n_q = p.n_q; tp.n_k = p.n_k; tp.causal = p.causal; tp.window = p.window; tp.sinks = p.sinks; tp.scale = p.scale;
   tp.tiles_q = (p.n_q + BM - 1) / BM;
   tp.tiles_k = (p.n_k + BM - 1) / BM;
   tp.q_blocks = 0;
@@ -1116,23 +1123,23 @@ int launch(K kernel, const TcParams& tp, long long blocks, int smem, cudaStream_
 }
 
 template <int PASS, int DQK, int DV, int BN, int FUSED, bool F16, bool SPLIT>
-int launch_pass(TcParams& tp, cudaStream_t s) {
+int launch_pass(const Problem& p, TcParams& tp, cudaStream_t s) {
   constexpr auto kernel = tc_pass_kernel<PASS, DQK, DV, BN, FUSED, F16, SPLIT>;
   constexpr int kSmem = Cfg<PASS, DQK, DV, BN>::SMEM_BYTES;
-  if (FUSED) tp.split_q = tp.cluster = tc_parts(tp.n_q, tp.n_k, tp.window);
+  if (FUSED) tp.split_q = tp.cluster = tc_parts(true, p);
   return launch(kernel, tp, static_cast<long long>(tp.items_q) * tp.split_q, kSmem, s);
 }
 
 // Passes 3 and 4, or one of them.
 template <int DQK, int DV, bool F16, bool SPLIT>
-int launch_34(TcParams& tp, bool pass3, bool pass4, cudaStream_t s) {
+int launch_34(const Problem& p, TcParams& tp, bool pass3, bool pass4, cudaStream_t s) {
   constexpr auto kernel = tc_pass34_kernel<DQK, DV, F16, SPLIT>;
   constexpr int kSmem3 = Cfg<3, DQK, DV, 64>::SMEM_BYTES, kSmem4 = Cfg<4, DQK, DV, 64>::SMEM_BYTES;
   constexpr int kSmem = kSmem3 > kSmem4 ? kSmem3 : kSmem4;
-  const PairGrid g = pair_grid(pass3 ? tp.items_q : 0, tc_parts(tp.n_q, tp.n_k, tp.window), pass4 ? tp.items_k : 0, tc_parts(tp.n_k, tp.n_q, tp.window));
+  const PairGrid g = pair_grid(pass3 ? tp.items_q : 0, tc_parts(true, p), pass4 ? tp.items_k : 0, tc_parts(false, p));
   if (pass3 && pass4 && launch_apart(g)) {
-    const int st = launch_34<DQK, DV, F16, SPLIT>(tp, true, false, s);
-    return st != FHOB_OK ? st : launch_34<DQK, DV, F16, SPLIT>(tp, false, true, s);
+    const int st = launch_34<DQK, DV, F16, SPLIT>(p, tp, true, false, s);
+    return st != FHOB_OK ? st : launch_34<DQK, DV, F16, SPLIT>(p, tp, false, true, s);
   }
   tp.split_q = g.split_q; tp.split_k = g.split_k;
   tp.cluster = g.cluster;
@@ -1143,29 +1150,29 @@ int launch_34(TcParams& tp, bool pass3, bool pass4, cudaStream_t s) {
 // `pass`: 1, 2, 3, 4 alone, 12 = passes 1 and 2 in one sweep, kWholeOperator = the sweep, then passes 3 and 4
 constexpr int kWholeOperator = 1234;
 template <int DQK, int DV, bool F16, bool SPLIT = false>
-int dispatch(int pass, const FhobProblem& p, cudaStream_t s) {
+int dispatch(int pass, const Problem& p, cudaStream_t s) {
   TcParams tp;
   int st = fill_params<F16, SPLIT>(p, tp);
   if (st != FHOB_OK) return st;
   switch (pass) {
     // pass 1 streams 128-row tiles (the stacked [K ; ddK] operand reaches N = 256), the others 64;
     // it touches no tile of the second head dim
-    case 1: return launch_pass<1, DQK, DQK, 128, 0, F16, SPLIT>(tp, s);
-    case 2: return launch_pass<2, DQK, DV, 64, 0, F16, SPLIT>(tp, s);
-    case 3: return launch_34<DQK, DV, F16, SPLIT>(tp, true, false, s);
-    case 4: return launch_34<DQK, DV, F16, SPLIT>(tp, false, true, s);
+    case 1: return launch_pass<1, DQK, DQK, 128, 0, F16, SPLIT>(p, tp, s);
+    case 2: return launch_pass<2, DQK, DV, 64, 0, F16, SPLIT>(p, tp, s);
+    case 3: return launch_34<DQK, DV, F16, SPLIT>(p, tp, true, false, s);
+    case 4: return launch_34<DQK, DV, F16, SPLIT>(p, tp, false, true, s);
     case 12:
     case kWholeOperator:
       // without O the sweep also produces D = sum P dP
-      st = p.o ? launch_pass<2, DQK, DV, 64, 1, F16, SPLIT>(tp, s) : launch_pass<2, DQK, DV, 64, 2, F16, SPLIT>(tp, s);
+      st = p.o ? launch_pass<2, DQK, DV, 64, 1, F16, SPLIT>(p, tp, s) : launch_pass<2, DQK, DV, 64, 2, F16, SPLIT>(p, tp, s);
       if (st != FHOB_OK || pass == 12) return st;
-      return launch_34<DQK, DV, F16, SPLIT>(tp, true, true, s);
+      return launch_34<DQK, DV, F16, SPLIT>(p, tp, true, true, s);
   }
   return FHOB_ERR_ARG;
 }
 
 template <bool F16>
-int dispatch_dims(int pass, const FhobProblem& p, cudaStream_t s) {
+int dispatch_dims(int pass, const Problem& p, cudaStream_t s) {
   // tile widths: the head dims rounded up to 64 or 128
   const int dv = head_dim_v(p);
   if (p.d <= 64) return dv <= 64 ? dispatch<64, 64, F16>(pass, p, s) : dispatch<64, 128, F16>(pass, p, s);
@@ -1224,14 +1231,14 @@ int tc_split_inputs(const FhobProblem& p, cudaStream_t s, int which) {
   return FHOB_OK;
 }
 
-int tc_grid(const FhobProblem& p, PairGrid* g) {
+int tc_grid(const Problem& p, PairGrid* g) {
   if (!tc_items_fit(p)) return FHOB_ERR_SHAPE;
   const int tq = (p.n_q + BM - 1) / BM, tk = (p.n_k + BM - 1) / BM;
-  *g = pair_grid(tq * p.bh, tc_parts(p.n_q, p.n_k, p.window), tk * p.bh, tc_parts(p.n_k, p.n_q, p.window));
+  *g = pair_grid(tq * p.bh, tc_parts(true, p), tk * p.bh, tc_parts(false, p));
   return g->blocks > 0x7fffffffLL ? FHOB_ERR_SHAPE : FHOB_OK;
 }
 
-int tc_pass(int pass, const FhobProblem& p, cudaStream_t s) {
+int tc_pass(int pass, const Problem& p, cudaStream_t s) {
   if (!tc_supported(p)) return FHOB_ERR_SHAPE;
   int st = check_device();
   if (st != FHOB_OK) return st;
@@ -1239,7 +1246,7 @@ int tc_pass(int pass, const FhobProblem& p, cudaStream_t s) {
   return p.dtype == FHOB_F16 ? dispatch_dims<true>(pass, p, s) : dispatch_dims<false>(pass, p, s);
 }
 
-int tc_operator(const FhobProblem& p, cudaStream_t s) {
+int tc_operator(const Problem& p, cudaStream_t s) {
   if (p.dtype == FHOB_F32) {
     const int st = tc_split_inputs(p, s);
     if (st != FHOB_OK) return st;

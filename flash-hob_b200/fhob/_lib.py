@@ -18,6 +18,7 @@ SYMBOLS = (
     "fhob_read_status", "fhob_forward", "fhob_backward", "fhob_bwdbwd_static_scratch",
     "fhob_selftest_expired_wait", "fhob_visible_tiles", "fhob_static_scratch_status",
     "fhob_workspace_bytes_problem", "fhob_cta_work",
+    "fhob_visible_tiles_sinks", "fhob_bwdbwd_sinks", "fhob_forward_sinks", "fhob_backward_sinks",
     "fhob_rotary", "fhob_layer_norm", "fhob_layer_norm_backward", "fhob_layer_norm_bwdbwd",
     "fhob_layer_norm_workspace_bytes",
 )
@@ -110,6 +111,14 @@ def load() -> C.CDLL:
     lib.fhob_static_scratch_status.argtypes = [C.c_void_p]
     lib.fhob_forward.restype = C.c_int
     lib.fhob_forward.argtypes = [P, C.c_void_p, C.c_void_p, C.c_void_p]
+    lib.fhob_visible_tiles_sinks.restype = C.c_int
+    lib.fhob_visible_tiles_sinks.argtypes = [C.c_int] * 8 + [C.POINTER(C.c_int)] * 3
+    lib.fhob_bwdbwd_sinks.restype = C.c_int
+    lib.fhob_bwdbwd_sinks.argtypes = [P, C.c_int32, C.c_void_p]
+    lib.fhob_forward_sinks.restype = C.c_int
+    lib.fhob_forward_sinks.argtypes = [P, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p]
+    lib.fhob_backward_sinks.restype = C.c_int
+    lib.fhob_backward_sinks.argtypes = [P, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]
     lib.fhob_rotary.restype = C.c_int
     lib.fhob_rotary.argtypes = [C.POINTER(FhobRotary), C.c_void_p]
     N = C.POINTER(FhobLayerNorm)

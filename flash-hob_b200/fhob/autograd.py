@@ -22,41 +22,46 @@ import ctypes as C
 import torch
 
 from . import _lib
-from .ops import _native, _Problem, _window
+from .ops import _native, _Problem, _sinks, _window
 
 
-def attention_backward(Q, K, V, O, dO, L, scale, *, is_causal: bool = False, sliding_window=None, impl: str = "auto"):
+def attention_backward(Q, K, V, O, dO, L, scale, *, is_causal: bool = False, sliding_window=None, impl: str = "auto",
+                       sink_tokens: int = 0):
     """First backward from the saved forward results: returns ``(dQ, dK, dV)``.
 
     Same maths as ``attn_bwd`` (jax_refs/flash_impl.py:124-173) with
-    ``P = exp(S - L)`` and ``D = rowsum(dO * O)``; O(N) memory.
+    ``P = exp(S - L)`` and ``D = rowsum(dO * O)``; O(N) memory.  The mask arguments are those the forward had.
     """
     if Q.is_cuda:
-        got = _native().backward(Q, K, V, O, dO, L, scale, is_causal, sliding_window, impl)
+        got = _native().backward(Q, K, V, O, dO, L, scale, is_causal, sliding_window, impl, sink_tokens)
         if got is not None:
             return got
     if Q.numel() == 0 or K.numel() == 0 or V.numel() == 0:
+        _sinks(_window(is_causal, sliding_window), sink_tokens)
         return tuple(torch.zeros_like(t) for t in (Q, K, V))   # no queries or no keys: nothing to launch
     # the problem struct wants three cotangent tensors of the right shapes; they are not read
-    prob = _Problem(Q, K, V, O, dO, Q, K, V, L, scale, is_causal, impl, need_outputs=False, window=sliding_window)
+    prob = _Problem(Q, K, V, O, dO, Q, K, V, L, scale, is_causal, impl, need_outputs=False, window=sliding_window,
+                    sinks=sink_tokens)
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (Q, K, V))   # contiguous results
     lib = _lib.load()
     with torch.cuda.device(prob.device):
-        call = lambda pr: lib.fhob_backward(C.byref(pr.p), C.c_void_p(dq.data_ptr()), C.c_void_p(dk.data_ptr()),
-                                            C.c_void_p(dv.data_ptr()), C.c_void_p(pr.stream))
+        call = lambda pr: lib.fhob_backward_sinks(C.byref(pr.p), pr.sinks, C.c_void_p(dq.data_ptr()), C.c_void_p(dk.data_ptr()),
+                                                  C.c_void_p(dv.data_ptr()), C.c_void_p(pr.stream))
         rc = call(prob)
         if rc != 0 and prob.layout is not None:
             # a view the tensor-map encoder does not take: read copies instead
             prob = _Problem(Q, K, V, O, dO, Q, K, V, L, scale, is_causal, impl, need_outputs=False,
-                            window=sliding_window, allow_views=False)
+                            window=sliding_window, allow_views=False, sinks=sink_tokens)
             rc = call(prob)
         _lib.check(rc, "fhob_backward")
     return dq, dk, dv
 
 
-def attention(q, k, v, scale=None, *, is_causal: bool = False, sliding_window=None):
+def attention(q, k, v, scale=None, *, is_causal: bool = False, sliding_window=None, sink_tokens: int = 0):
     """``softmax(q k^T scale) v`` for CUDA bfloat16/float32 tensors ``(BH, N, D)`` or ``(B, H, N, D)``,
-    differentiable twice (``create_graph=True``)."""
+    differentiable twice (``create_graph=True``).  ``sliding_window`` W: a query sees the W keys up to its diagonal;
+    ``sink_tokens`` S: and the first S keys."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
-    return _native().attention(q, k, v, float(scale), bool(is_causal), _window(is_causal, sliding_window))
+    window = _window(is_causal, sliding_window)
+    return _native().attention(q, k, v, float(scale), bool(is_causal), window, _sinks(window, sink_tokens))

@@ -106,11 +106,21 @@ def _window(is_causal, sliding_window) -> int:
     return w
 
 
+def _sinks(window: int, sink_tokens) -> int:
+    """The validated number of first tokens that stay visible behind the window (a number from _window)."""
+    s = int(sink_tokens)
+    if s != sink_tokens or s < 0 or s > 2 ** 31 - 1:
+        raise ValueError(f"sink_tokens must be a non-negative integer, got {sink_tokens!r}")
+    if s and not window:
+        raise ValueError("sink_tokens needs a sliding_window (without one every key up to the diagonal is visible)")
+    return s
+
+
 class _Problem:
     """Validated tensors + the FhobProblem struct that points at them."""
 
     def __init__(self, Q, K, V, O, dO, ddQ, ddK, ddV, L, scale, is_causal, impl, need_outputs=True,
-                 window=None, out=None, workspace=None, allow_views=True):
+                 window=None, out=None, workspace=None, allow_views=True, sinks=0):
         names = ("Q", "K", "V", "O", "dO", "ddQ", "ddK", "ddV")
         no_o = O is None
         if no_o:
@@ -174,6 +184,7 @@ class _Problem:
         p.dtype = _lib.DTYPES[str(dt)]
         p.causal = 1 if is_causal else 0
         p.window = _window(is_causal, window)
+        self.sinks = _sinks(p.window, sinks)
         p.impl = _lib.IMPL[impl]
         p.scale = float(scale)
         if workspace is None:
@@ -231,17 +242,17 @@ class _Problem:
 
 
 def _run_device(Q, K, V, O, dO, ddQ, ddK, ddV, L, scale, is_causal, impl, check, window=None, out=None,
-                workspace=None):
+                workspace=None, sinks=0):
     prob = _Problem(Q, K, V, O, dO, ddQ, ddK, ddV, L, scale, is_causal, impl, window=window, out=out,
-                    workspace=workspace)
+                    workspace=workspace, sinks=sinks)
     lib = _lib.load()
     with torch.cuda.device(prob.device):
-        rc = lib.fhob_bwdbwd(C.byref(prob.p), C.c_void_p(prob.stream))
+        rc = lib.fhob_bwdbwd_sinks(C.byref(prob.p), prob.sinks, C.c_void_p(prob.stream))
         if rc != 0 and prob.layout is not None:
             # a view the driver's tensor-map encoder (or the library) does not take: fall back to copies
             prob = _Problem(Q, K, V, O, dO, ddQ, ddK, ddV, L, scale, is_causal, impl, window=window, out=out,
-                            workspace=workspace, allow_views=False)
-            rc = lib.fhob_bwdbwd(C.byref(prob.p), C.c_void_p(prob.stream))
+                            workspace=workspace, allow_views=False, sinks=sinks)
+            rc = lib.fhob_bwdbwd_sinks(C.byref(prob.p), prob.sinks, C.c_void_p(prob.stream))
         _lib.check(rc, "fhob_bwdbwd")
         if check:
             _lib.check(prob.status(), "fhob_bwdbwd (device status)")
@@ -262,7 +273,8 @@ def _empty_problem(Q, K, V, dO, out):
 
 def flash_bwdbwd(Q, K, V, O, dO, ddQ, ddK, ddV, L, scale, *, is_causal: bool = False,
                  sliding_window: Optional[int] = None, impl: str = "auto", check: Optional[bool] = None,
-                 device: Optional[torch.device] = None, out=None, workspace=None) -> Tuple[torch.Tensor, ...]:
+                 device: Optional[torch.device] = None, out=None, workspace=None,
+                 sink_tokens: int = 0) -> Tuple[torch.Tensor, ...]:
     """Double backward of scaled-dot-product attention.
 
     Same positional signature and return order as the reference
@@ -283,7 +295,9 @@ def flash_bwdbwd(Q, K, V, O, dO, ddQ, ddK, ddV, L, scale, *, is_causal: bool = F
     ``is_causal`` bottom-right aligned causal mask (the reference operator has
     none; its oracle does: jax_refs/flash_impl.py:86-91); ``sliding_window``
     the oracle's ``sliding_window_length`` W (needs ``is_causal``): query i
-    then sees only the W keys that end at its causal diagonal; ``impl`` one of
+    then sees only the W keys that end at its causal diagonal; ``sink_tokens``
+    S (needs ``sliding_window``): the first S keys stay visible to every query
+    from their own on; ``impl`` one of
     "auto", "simt", "tcgen05"; ``check`` read the device status word after
     the kernels and raise if a bounded device wait ran out.  Reading it
     synchronises the stream, so the default is ``False`` for device tensors
@@ -305,16 +319,19 @@ def flash_bwdbwd(Q, K, V, O, dO, ddQ, ddK, ddV, L, scale, *, is_causal: bool = F
     ``out``, four host tensors, preferably pinned) after a stream synchronise.
     """
     if Q.is_cuda and out is None and workspace is None:
-        got = _native().bwdbwd(Q, K, V, O, dO, ddQ, ddK, ddV, L, scale, is_causal, sliding_window, impl)
+        got = _native().bwdbwd(Q, K, V, O, dO, ddQ, ddK, ddV, L, scale, is_causal, sliding_window, impl,
+                               sink_tokens)
         if got is not None:
             if check:
                 _check_status(Q.device, "fhob_bwdbwd")
             return got
     if Q.numel() == 0 or K.numel() == 0 or V.numel() == 0:
+        if sink_tokens:
+            _sinks(_window(is_causal, sliding_window), sink_tokens)
         return _empty_problem(Q, K, V, dO, out)
     if Q.device.type == "cuda":
         return _run_device(Q, K, V, O, dO, ddQ, ddK, ddV, L, scale, is_causal, impl, bool(check), sliding_window,
-                           out, workspace)
+                           out, workspace, sink_tokens)
     if not torch.cuda.is_available():
         raise RuntimeError("flash_bwdbwd needs a CUDA device; there is no CPU implementation")
     if workspace is not None:
@@ -322,7 +339,7 @@ def flash_bwdbwd(Q, K, V, O, dO, ddQ, ddK, ddV, L, scale, *, is_causal: bool = F
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     with _host_locks.setdefault(dev.index, threading.Lock()):   # a call ends synchronised: the next finds the sets idle
         return _run_host((Q, K, V, O, dO, ddQ, ddK, ddV), L, scale, is_causal, impl, check is None or bool(check), dev,
-                         window=sliding_window, out=out)
+                         window=sliding_window, out=out, sinks=sink_tokens)
 
 
 _copy_streams: dict = {}
@@ -347,7 +364,7 @@ def _host_ranges(bh: int, head_bytes: int, range_bytes: int):
     return bounds
 
 
-def _run_host(mats, L, scale, is_causal, impl, check, dev, window=None, out=None, range_bytes=None):
+def _run_host(mats, L, scale, is_causal, impl, check, dev, window=None, out=None, range_bytes=None, sinks=0):
     """Host tensors in, pinned host tensors out.  Heads are independent, so the batch is cut into
     head ranges of about ``HOST_RANGE_BYTES`` of input each (at least four ranges when there are
     that many heads) that flow through three streams: upload of range i+1, the kernels of range i
@@ -422,7 +439,7 @@ def _run_host(mats, L, scale, is_causal, impl, check, dev, window=None, out=None
         if st["drained"] is not None:
             main.wait_event(st["drained"])
         res = _run_device(*(None if t is None else t[:n] for t in st["ins"]), scale, is_causal, impl, False, window,
-                          out=tuple(t[:n] for t in st["res"]), workspace=ws)
+                          out=tuple(t[:n] for t in st["res"]), workspace=ws, sinks=sinks)
         if check:
             status_dev[i:i + 1].copy_(ws[:4].view(torch.int32), non_blocking=True)
         st["read"] = torch.cuda.Event()
@@ -451,7 +468,7 @@ def release_cached_memory() -> None:
 
 
 def attention_forward(Q, K, V, scale=None, *, is_causal: bool = False, sliding_window: Optional[int] = None,
-                      impl: str = "auto", check: bool = False, need_o: bool = True):
+                      impl: str = "auto", check: bool = False, need_o: bool = True, sink_tokens: int = 0):
     """O(N)-memory producer of the saved forward results: returns ``(O, L)``.
 
     ``O = softmax(Q K^T scale) V`` in the input dtype and the fp32 logsumexp
@@ -465,9 +482,10 @@ def attention_forward(Q, K, V, scale=None, *, is_causal: bool = False, sliding_w
     ``need_o=False`` skips the ``P V`` product and returns ``(None, L)``.
     ``check`` synchronises and raises if a bounded device wait ran out.
     Queries that see no key (causal with N_K < N_Q) get ``O = 0``, ``L = -inf``.
+    ``sliding_window`` and ``sink_tokens`` as in ``flash_bwdbwd``.
     """
     if Q.is_cuda:
-        got = _native().forward(Q, K, V, scale, is_causal, sliding_window, impl, need_o)
+        got = _native().forward(Q, K, V, scale, is_causal, sliding_window, impl, need_o, sink_tokens)
         if got is not None:
             if check:
                 _check_status(Q.device, "fhob_forward")
@@ -477,6 +495,7 @@ def attention_forward(Q, K, V, scale=None, *, is_causal: bool = False, sliding_w
         raise ValueError("attention_forward needs CUDA bfloat16/float16/float32 tensors")
     if impl not in _lib.IMPL:
         raise ValueError(f"impl must be one of {sorted(_lib.IMPL)}, got {impl!r}")
+    sinks = _sinks(_window(is_causal, sliding_window), sink_tokens)
     # views are read in place when the tensor-core kernels run (see _Problem); else folded copies
     strides = None
     if (all(t.dim() in (3, 4) for t in (Q, K, V)) and impl != "simt" and _tc_capable(Q.dtype, Q.shape[-1], V.shape[-1])
@@ -526,8 +545,8 @@ def attention_forward(Q, K, V, scale=None, *, is_causal: bool = False, sliding_w
     ws = _workspace(Q.device, stream, max(256, lib.fhob_workspace_bytes_problem(C.byref(p))))
     p.workspace, p.workspace_bytes = ws.data_ptr(), ws.numel()
     with torch.cuda.device(Q.device):
-        call = lambda: lib.fhob_forward(C.byref(p), C.c_void_p(o.data_ptr() if need_o else None),
-                                        C.c_void_p(lse.data_ptr()), C.c_void_p(stream))
+        call = lambda: lib.fhob_forward_sinks(C.byref(p), sinks, C.c_void_p(o.data_ptr() if need_o else None),
+                                              C.c_void_p(lse.data_ptr()), C.c_void_p(stream))
         rc = call()
         if rc != 0 and lay is not None:
             # a view the tensor-map encoder does not take: read copies instead
@@ -540,11 +559,12 @@ def attention_forward(Q, K, V, scale=None, *, is_causal: bool = False, sliding_w
     return (o.reshape(*shape_q[:-1], d_v) if need_o else None), lse.reshape(shape_q[:-1])
 
 
-def produce_L(Q, K, is_causal: bool = False, scale=None, sliding_window: Optional[int] = None):
+def produce_L(Q, K, is_causal: bool = False, scale=None, sliding_window: Optional[int] = None, sink_tokens: int = 0):
     """fp32 logsumexp of the scaled scores, same name and argument order as the
     reference helper (fhog/triton_flash.py:252-258) but O(N) memory, fp32 and
     causal-capable.  Only the scores are computed (no ``P V`` product)."""
-    return attention_forward(Q, K, K, scale, is_causal=is_causal, sliding_window=sliding_window, need_o=False)[1]
+    return attention_forward(Q, K, K, scale, is_causal=is_causal, sliding_window=sliding_window, need_o=False,
+                             sink_tokens=sink_tokens)[1]
 
 
 def run_passes(Q, K, V, O, dO, ddQ, ddK, ddV, L, scale, *, is_causal=False, sliding_window=None, impl="auto",

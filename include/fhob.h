@@ -225,6 +225,15 @@ int fhob_visible_tiles(int q_stationary, int m0, int rows, int tile, int n_q, in
                        int* t_begin, int* t_end);
 
 /*
+ * The same for a causal window with `sink_tokens` first keys that stay
+ * visible: the streamed tiles are 0 .. *first - 1 (keys below sink_tokens;
+ * none if keys are stationary), then *t_begin .. *t_end - 1 (the other keys).  A
+ * tile with keys of both kinds may be in both lists.
+ */
+int fhob_visible_tiles_sinks(int q_stationary, int m0, int rows, int tile, int n_q, int n_k, int window, int sink_tokens,
+                             int* first, int* t_begin, int* t_end);
+
+/*
  * The CTA-to-work rule of passes 3 and 4 in one launch (host evaluation, no GPU
  * needed): CTA `block` works for pass *pass (3 query-tiled, 4 key-tiled, 0 = it only fills up a cluster) on
  * part *part of *parts of item *item; the items of a pass are the (head, stationary tile) pairs, and the
@@ -275,6 +284,18 @@ int fhob_forward(const FhobProblem* p, void* o_out, float* lse_out, void* stream
  * fhob_forward.
  */
 int fhob_backward(const FhobProblem* p, void* dq, void* dk, void* dv, void* stream);
+
+/*
+ * fhob_bwdbwd, fhob_forward and fhob_backward with a sliding window (p->window
+ * > 0) and a few first tokens that stay visible behind it: key j is visible to
+ * query i iff i + n_k - n_q >= j and (i + n_k - n_q - j < window or
+ * j < sink_tokens).  sink_tokens = 0 is the call without it; sink_tokens < 0, or
+ * > 0 without a window, FHOB_ERR_ARG.  A forward's L and O go with a backward of
+ * the same window and sink_tokens.  The reference has no counterpart.
+ */
+int fhob_bwdbwd_sinks(const FhobProblem* p, int32_t sink_tokens, void* stream);
+int fhob_forward_sinks(const FhobProblem* p, int32_t sink_tokens, void* o_out, float* lse_out, void* stream);
+int fhob_backward_sinks(const FhobProblem* p, int32_t sink_tokens, void* dq, void* dk, void* dv, void* stream);
 
 /*
  * The operator for callers that cannot allocate device memory at all.
