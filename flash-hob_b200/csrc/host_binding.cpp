@@ -276,14 +276,14 @@ struct Attention : torch::autograd::Function<Attention> {
 const Tensor* tensor_arg(PyObject* o) { return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr; }
 
 // sliding_window: None, or a positive int together with a causal mask; sink_tokens: 0, or a positive int together with a window
-bool mask_args(PyObject* causal, PyObject* window, PyObject* sinks, Mask& m) {
+bool mask_args(PyObject* causal, PyObject* window, PyObject* sinks, Mask& m) {   // sinks: NULL = 0
   const int c = PyObject_IsTrue(causal);
   if (c < 0) { PyErr_Clear(); return false; }
   m.causal = c == 1;
   m.window = 0;
-  if (!PyLong_CheckExact(sinks)) return false;
   int overflow = 0;
-  const long long first = PyLong_AsLongLongAndOverflow(sinks, &overflow);
+  if (sinks && !PyLong_CheckExact(sinks)) return false;
+  const long long first = sinks ? PyLong_AsLongLongAndOverflow(sinks, &overflow) : 0;
   if (overflow || first < 0 || first > INT32_MAX) return false;
   m.sinks = first;
   if (window == Py_None) return first == 0;
@@ -314,12 +314,12 @@ PyObject* wrapped(const Tensor* t, int n) {
   return r;
 }
 
-// bwdbwd(Q, K, V, O, dO, ddQ, ddK, ddV, L, scale, is_causal, sliding_window, impl, sink_tokens)
+// bwdbwd(Q, K, V, O, dO, ddQ, ddK, ddV, L, scale, is_causal, sliding_window, impl, sink_tokens = 0)
 PyObject* py_bwdbwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Mask m;
   double scale;
-  if (n != 14 || !mask_args(a[10], a[11], a[13], m) || !scale_arg(a[9], scale)) Py_RETURN_NONE;
+  if (n < 13 || n > 14 || !mask_args(a[10], a[11], n > 13 ? a[13] : nullptr, m) || !scale_arg(a[9], scale)) Py_RETURN_NONE;
   const Tensor* t[9];
   for (int i = 0; i < 9; ++i) {
     t[i] = tensor_arg(a[i]);
@@ -331,11 +331,11 @@ PyObject* py_bwdbwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// forward(Q, K, V, scale, is_causal, sliding_window, impl, need_o, sink_tokens) -> (O, L) | (None, L)
+// forward(Q, K, V, scale, is_causal, sliding_window, impl, need_o, sink_tokens = 0) -> (O, L) | (None, L)
 PyObject* py_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Mask m;
-  if (n != 9 || !mask_args(a[4], a[5], a[8], m)) Py_RETURN_NONE;
+  if (n < 8 || n > 9 || !mask_args(a[4], a[5], n > 8 ? a[8] : nullptr, m)) Py_RETURN_NONE;
   const Tensor *q = tensor_arg(a[0]), *k = tensor_arg(a[1]), *v = tensor_arg(a[2]);
   if (!q || !k || !v || q->dim() < 1) Py_RETURN_NONE;
   double scale = 1.0 / std::sqrt(static_cast<double>(q->size(-1)));
@@ -352,12 +352,12 @@ PyObject* py_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// backward(Q, K, V, O, dO, L, scale, is_causal, sliding_window, impl, sink_tokens) -> (dQ, dK, dV)
+// backward(Q, K, V, O, dO, L, scale, is_causal, sliding_window, impl, sink_tokens = 0) -> (dQ, dK, dV)
 PyObject* py_backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Mask m;
   double scale;
-  if (n != 11 || !mask_args(a[7], a[8], a[10], m) || !scale_arg(a[6], scale)) Py_RETURN_NONE;
+  if (n < 10 || n > 11 || !mask_args(a[7], a[8], n > 10 ? a[10] : nullptr, m) || !scale_arg(a[6], scale)) Py_RETURN_NONE;
   const Tensor* t[6];
   for (int i = 0; i < 6; ++i)
     if (!(t[i] = tensor_arg(a[i]))) Py_RETURN_NONE;

@@ -104,7 +104,7 @@ __device__ __forceinline__ void fw_split_pack(float x, float y, uint32_t& hi, ui
 // fp32 problems (SPLIT): every fp32 operand as bf16 hi + lo, rows [hi(64) | lo(64)] = the two boxes of a
 // 128-wide tile; a contraction is hi.hi + hi.lo + lo.hi (see tc_kernels.cu).  Head dims up to 64.  The small
 // terms of P V have an accumulator of their own (see BwCfg in tc_backward.cu).
-template <int DQK, int DV, bool F16, bool SPLIT, bool OUT>
+template <int DQK, int DV, bool F16, bool SPLIT, bool OUT, bool SINKS>
 __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant__ FwParams p) {
   using C = FwCfg<DQK, DV, OUT>;
   static_assert(!SPLIT || (DQK == 128 && DV == 128 && !F16), "split fp32 operands are [hi(64) | lo(64)] bf16 rows");
@@ -127,35 +127,52 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
   // key tiles of the two query tiles (a tile beyond the last query has none and is left alone)
   auto m_of = [&](int x) { return (group * p.q_tiles + x) * BM; };
   auto live = [&](int x) { return x < p.q_tiles && m_of(x) < p.n_q; };
-  // Tiles of the first keys (n_first, if any stay visible behind the window; both query tiles take those of the later
-  // one) and then of the window: query tile x has begin[x] .. end[x] - 1 of those.  Steps t count through the list:
-  // step t < n_first is key tile t, a later one is key tile w_begin + t - n_first.
+  // Steps t of the walk over the key tiles; query tile x takes part in those that are active(x, t).
+  //  Without first keys behind the window (SINKS false): step t is key tile t, query tile x has begin[x] .. end[x] - 1.
+  //  With them: n_first steps for their tiles (both query tiles take those of the later one), then the window's, key tile
+  //  w_begin + t - n_first.
   int begin[2], end[2], n_first = 0;
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     begin[x] = end[x] = 0;
-    if (live(x)) {
+    if (!live(x)) continue;
+    if constexpr (SINKS) {
       const TileList list = streamed_tiles(true, m_of(x), BM, BN, p.n_k, off, p.causal, p.window, p.sinks);
       n_first = max(n_first, list.first);
       begin[x] = list.begin;
       end[x] = list.begin + list.count - list.first;
+    } else {
+      visible_tiles(true, m_of(x), BM, BN, p.n_k, off, p.causal, p.window, begin[x], end[x]);
+      if (p.split > 1) split_range(part, p.split, begin[x], end[x]);
     }
   }
   const bool any0 = end[0] > begin[0], any1 = end[1] > begin[1];
   const int w_begin = any0 && any1 ? min(begin[0], begin[1]) : (any0 ? begin[0] : begin[1]);
   const int w_end = any0 && any1 ? max(end[0], end[1]) : (any0 ? end[0] : end[1]);
-  int t_begin = 0, t_end = n_first + (w_end > w_begin ? w_end - w_begin : 0);
-  if (p.split > 1) split_range(part, p.split, t_begin, t_end);   // (query tile A only: it has every step)
-  const int n_tiles = t_end - t_begin;
-  auto key_tile = [&](int t) { return t < n_first ? t : w_begin + t - n_first; };
+  int t_begin = w_begin, t_end = w_end;
+  if constexpr (SINKS) {
+    t_begin = 0;
+    t_end = n_first + (w_end > w_begin ? w_end - w_begin : 0);
+    if (p.split > 1) split_range(part, p.split, t_begin, t_end);   // (query tile A only: it has every step)
+  }
+  const int n_tiles = t_end > t_begin ? t_end - t_begin : 0;
+  auto key_tile = [&](int t) { return !SINKS || t < n_first ? t : w_begin + t - n_first; };
   auto active = [&](int x, int t) {
-    if (t < n_first) return live(x) && t < t_end;
-    const int tile = w_begin + t - n_first;
-    return t < t_end && tile >= begin[x] && tile < end[x];
+    if constexpr (!SINKS) return t >= begin[x] && t < end[x];
+    if (t >= t_end) return false;
+    return t < n_first ? live(x) : key_tile(t) >= begin[x] && key_tile(t) < end[x];
   };
-  auto skipped = [&](int x) { return end[x] > begin[x] ? begin[x] - w_begin : 0; };   // steps between the first keys and x's window
-  auto step_no = [&](int x, int t) { return t - t_begin - (t < n_first ? 0 : skipped(x)); };   // how many steps of x come before t
-  auto steps = [&](int x) { return p.split > 1 ? (x == 0 ? n_tiles : 0) : (live(x) ? n_first : 0) + end[x] - begin[x]; };
+  // with first keys: the steps between them and x's window
+  auto skipped = [&](int x) { return end[x] > begin[x] ? begin[x] - w_begin : 0; };
+  // how many steps of x there are, and how many of them come before t
+  auto steps = [&](int x) {
+    if constexpr (!SINKS) return end[x] - begin[x];
+    return p.split > 1 ? (x == 0 ? n_tiles : 0) : (live(x) ? n_first : 0) + end[x] - begin[x];
+  };
+  auto step_no = [&](int x, int t) {
+    if constexpr (!SINKS) return t - begin[x];
+    return t - t_begin - (t < n_first ? 0 : skipped(x));
+  };
 
   int fault = 0;   // thread 0: what to report at the end
   if (threadIdx.x == 0) {
@@ -337,7 +354,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
     int lo = 0, hi = p.n_k - 1;
     if (p.causal && g_row + off < hi) hi = g_row + off;
     if (p.window > 0 && g_row + off - p.window + 1 > 0) lo = g_row + off - p.window + 1;
-    if (lo < p.sinks) lo = p.sinks;
+    if (SINKS && lo < p.sinks) lo = p.sinks;
     float run_m = -INFINITY, run_l = 0.f;   // reference maximum (log2 domain) and sum of exponentials
     bool ok = true;
     const uint32_t o_addr = lane_base + o_cols(x);
@@ -446,17 +463,16 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
       }
     };
     for (int it = 0; it < n_iter; ++it) {
-      int t = t_begin + it;
-      const bool first = t < n_first;   // a tile of the first keys: [0, sinks) of it
-      if (!first) t += skipped(x);
+      const bool first = SINKS && t_begin + it < n_first;   // a tile of the first keys: [0, sinks) of it
+      const int t = SINKS ? t_begin + it + (first ? 0 : skipped(x)) : begin[x] + it;
       const int n0 = key_tile(t) * BN, stage = it % kStages;
       // does any score of this tile need masking?  (uniform over the tile's warps)
       bool masked = n0 + BN > p.n_k;
       if (p.causal) {
         masked = masked || (n0 + BN - 1 > m0 + off);
-        if (p.window > 0) masked = masked || (first ? n0 + BN > p.sinks : m0 + BM - 1 + off - n0 >= p.window || n0 < p.sinks);
+        if (p.window > 0) masked = masked || (first ? n0 + BN > p.sinks : m0 + BM - 1 + off - n0 >= p.window || (SINKS && n0 < p.sinks));
       }
-      const int lo_t = first ? 0 : lo, hi_t = first && p.sinks <= hi ? p.sinks - 1 : hi;
+      const int lo_t = first ? 0 : lo, hi_t = first && p.sinks <= hi ? p.sinks - 1 : hi;   // (lo, hi without first keys)
       if (masked) step(std::true_type{}, it, n0, stage, lo_t, hi_t);
       else step(std::false_type{}, it, n0, stage, lo_t, hi_t);
       if (!ok) break;
@@ -567,10 +583,10 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
 }
 
 // ------------------------------------------------------------------ host side
-template <int DQK, int DV, bool F16, bool SPLIT, bool OUT>
+template <int DQK, int DV, bool F16, bool SPLIT, bool OUT, bool SINKS>
 int fw_launch(const Problem& p, void* o_out, float* lse_out, int* status, cudaStream_t s) {
   using C = FwCfg<DQK, DV, OUT>;
-  constexpr auto kernel = fw_kernel<DQK, DV, F16, SPLIT, OUT>;
+  constexpr auto kernel = fw_kernel<DQK, DV, F16, SPLIT, OUT, SINKS>;
   FwParams tp;
   memset(&tp, 0, sizeof(tp));
   const int dv = head_dim_v(p);
@@ -612,8 +628,11 @@ int fw_launch(const Problem& p, void* o_out, float* lse_out, int* status, cudaSt
 template <int DQK, int DV, bool F16, bool SPLIT = false>
 int fw_dispatch(const Problem& p, void* o_out, float* lse_out, int* status, cudaStream_t s) {
   // no O wanted: the scores alone (no tile of the second head dim is touched)
-  return o_out ? fw_launch<DQK, DV, F16, SPLIT, true>(p, o_out, lse_out, status, s)
-               : fw_launch<DQK, DQK, F16, SPLIT, false>(p, o_out, lse_out, status, s);
+  if (p.sinks > 0)
+    return o_out ? fw_launch<DQK, DV, F16, SPLIT, true, true>(p, o_out, lse_out, status, s)
+                 : fw_launch<DQK, DQK, F16, SPLIT, false, true>(p, o_out, lse_out, status, s);
+  return o_out ? fw_launch<DQK, DV, F16, SPLIT, true, false>(p, o_out, lse_out, status, s)
+               : fw_launch<DQK, DQK, F16, SPLIT, false, false>(p, o_out, lse_out, status, s);
 }
 
 template <bool F16>
