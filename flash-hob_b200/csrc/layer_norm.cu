@@ -10,12 +10,21 @@
 //   (sums over rows for dw, db, dw2; means over a row).  mean(p (g - m - h q)) equals mean(v g) - a m - c q, but its
 //   terms do not cancel when v or g have a large common part.
 //
-// What bounds it: each matrix is read once and written once, so the memory.  A row belongs to a group of one to 32 warps, which
-// keep it in registers (as it came, 16 bits an element) from its only load to its results; sums over a row are
-// shuffles, then, if the group has several warps, one exchange through shared memory per round.  Rounds: two in the forward
-// (the variance is a sum of squares around the mean), one in the backward, two in the double backward.
-// A thread owns the same columns of all its rows, so what the sums over rows add up stays in its registers; the groups
-// of a block are added up in shared memory and the blocks' sums in a second launch, always in the same order.
+// What bounds it: each matrix is read once and written once, so the memory.
+//  - A row belongs to a group: 2 to 32 lanes of a warp or 2 to 32 warps, 8 or 16 elements a lane.  It is in registers, in fp32,
+//    from its only load to its results; sums over it are shuffles, then, if the group has several warps, one exchange
+//    through shared memory per round.  Rounds: two in the forward (the variance is a sum of squares around the mean), one
+//    in the backward, two in the double backward.
+//  - Next to the memory comes the number of instructions: elements are converted once, the arithmetic is on packed pairs, and the
+//    vectors over the columns stay in registers.  (Converted where they are used, with scalar arithmetic, an element of the
+//    forward took 34 instructions, of the double backward 93; now 7 and 20.)
+//  - What keeps the memory busy is the number of bytes on their way.  Rows come through a ring in shared memory, up to
+//    three rows ahead of the one in work, by asynchronous copies.  On the 16-byte grid a thread copies its own elements
+//    alone: it is the only one to read them, so nothing waits but for its own copies.
+//  - A thread owns the same columns of all its rows, so what the sums over rows add up stays in its registers; the groups of a
+//    block are added up in shared memory and the blocks' sums in a second launch, always in the same order.
+//  - Rows off the 16-byte grid (an odd number of columns) are copied by their group together, in the 16-byte pieces of memory
+//    that hold them, and read element by element: neighbouring threads own neighbouring columns then.
 #include "fhob_common.cuh"
 #include "tc_common.cuh"
 
@@ -32,305 +41,538 @@ struct LnParams {
   void *y, *dx;                            // y | dx, and of the double backward ddy | dx2; contiguous
   float *mean, *rstd;
   float* partial;                          // [block][0 = dw, 1 = db][cols], NULL when no such sum is wanted
-  long long rows;
-  int cols, warps;                         // warps of a group
+  int rows, cols, warps, lanes;            // of a group: warps, and lanes of a warp (32 if there are several warps)
   int w_f32;                               // type of w, b, vw, vb: fp32, or that of the matrices
   int want_dw, want_db;
   float eps, inv_cols;
 };
 
-// V elements of a row at column c, as they are in memory
+// How a thread's elements lie in a row: in pieces of 16 bytes (V elements each), or, V == 2, one here and one there.
 template <class T, int V>
-struct Piece {
-  alignas(V * sizeof(T) > 16 ? 16 : V * sizeof(T)) T e[V];
-};
-template <class T, int V>
-__device__ __forceinline__ void load_piece(Piece<T, V>& to, const T* from) {
-  if constexpr (V * sizeof(T) == 16) *reinterpret_cast<uint4*>(to.e) = *reinterpret_cast<const uint4*>(from);
-  else if constexpr (V * sizeof(T) == 4) *reinterpret_cast<uint32_t*>(to.e) = *reinterpret_cast<const uint32_t*>(from);
-  else to.e[0] = from[0];
-}
-template <class T, int V>
-__device__ __forceinline__ void store_piece(T* to, const Piece<T, V>& from) {
-  if constexpr (V * sizeof(T) == 16) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(from.e);
-  else if constexpr (V * sizeof(T) == 4) *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(from.e);
-  else to[0] = from.e[0];
-}
+constexpr bool kWide = V * sizeof(T) == 16;
 
-// What a thread needs to know of its place: its columns are (warp_in_group * 32 + lane + i * width) * V, i < NV.
-template <int V>
+// `bytes` of 16 are read, the others zero
+__device__ __forceinline__ void cp_async(uint32_t to, const void* from, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+template <class T>
+__device__ __forceinline__ float2 unpack(uint32_t w) {
+  if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <class T>
+__device__ __forceinline__ uint32_t pack(const float2& x) { return pack16<std::is_same<T, __half>::value>(x.x, x.y); }
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// What a thread needs to know of its place.  Element e of its piece i is at column(i, e).  SUB: several rows share a warp.
+template <class T, int V, bool SUB>
 struct Place {
-  int group, groups, lane, warp, warps, width, first;   // groups of a block; width = threads of a group
-  __device__ __forceinline__ explicit Place(int warps_per_group) {
-    warps = warps_per_group;
-    const int w = threadIdx.x >> 5;
-    group = w / warps;
-    groups = (blockDim.x >> 5) / warps;
-    warp = w - group * warps;
-    lane = threadIdx.x & 31;
-    width = warps * 32;
-    first = warp * 32 + lane;
+  static constexpr bool kSub = SUB;
+  int group, groups;         // of the block
+  int warp, warps;           // of the group
+  int lanes;                 // of a warp
+  int first, width;          // this thread of the group's threads
+  int above;                 // groups of this warp in front of this thread's
+  __device__ __forceinline__ Place(int warps_per_group, int lanes_per_group) {
+    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    warps = SUB ? 1 : warps_per_group;
+    lanes = SUB ? lanes_per_group : 32;
+    const int per_warp = SUB ? 32 / lanes : 1;
+    above = SUB ? lane / lanes : 0;
+    group = w / warps * per_warp + above;
+    groups = (blockDim.x >> 5) / warps * per_warp;
+    warp = w % warps;
+    first = warp * 32 + (SUB ? lane % lanes : lane);
+    width = warps * lanes;
   }
-  __device__ __forceinline__ int column(int i) const { return (first + i * width) * V; }
+  __device__ __forceinline__ int column(int i, int e = 0) const {
+    return kWide<T, V> ? (first + i * width) * V + e : first + (i * V + e) * width;
+  }
+  // x at the columns of a pair of piece i, zero behind the last column.  (Pieces of 16 bytes are whole.)
+  __device__ __forceinline__ float2 inside(float x, int i, int cols) const {
+    const float here = column(i) < cols ? x : 0.f;
+    return make_float2(here, kWide<T, V> ? here : (column(i, 1) < cols ? x : 0.f));
+  }
+  __device__ __forceinline__ void meet() const {   // the group
+    if (SUB || warps == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(width) : "memory");
+  }
+  // Stores piece i of a row.
+  __device__ __forceinline__ void store(T* row, int i, int cols, const float2 (&x)[V / 2]) const {
+    const int c = column(i);
+    if (c >= cols) return;
+    if constexpr (!kWide<T, V>) {
+      row[c] = static_cast<T>(x[0].x);
+      if (column(i, 1) < cols) row[column(i, 1)] = static_cast<T>(x[0].y);
+    } else if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(row + c) = make_float4(x[0].x, x[0].y, x[1].x, x[1].y);
+    } else {
+      *reinterpret_cast<uint4*>(row + c) = make_uint4(pack<T>(x[0]), pack<T>(x[1]), pack<T>(x[2]), pack<T>(x[3]));
+    }
+  }
+  // Piece i of a vector over the columns; `otherwise` where there is no vector or no such column.
+  __device__ __forceinline__ void vector(float2 (&to)[V / 2], const void* from, int f32, int i, int cols, float otherwise) const {
+    auto element = [&](int e) {
+      const int c = column(i, e);
+      if (!from || c >= cols) return otherwise;
+      return f32 ? static_cast<const float*>(from)[c] : static_cast<float>(static_cast<const T*>(from)[c]);
+    };
+    if (kWide<T, V> && from && !f32 && sizeof(T) == 2 && column(i) < cols) {
+      const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const T*>(from) + column(i));
+      const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) to[j] = unpack<T>(ws[j & 3]);
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) to[j] = make_float2(element(2 * j), element(2 * j + 1));
+  }
 };
 
-// Sums of N values over a group, in every thread of it.  `exchange`: N floats per warp of the block; two areas take turns,
-// so that one meeting a round is enough (a warp that is a round ahead writes to the other area, and cannot be two ahead).
-template <int N, int V>
-__device__ __forceinline__ void group_sum(float (&x)[N], const Place<V>& at, float* exchange) {
+// Sums of four (or, the last ones unused, fewer) values over a group, in every thread of it.  `exchange`: four floats per warp
+// of the block; two such areas take turns, so that one meeting a round is enough (a warp that is a round ahead writes to the
+// other area, and cannot be two ahead).
+//  In a whole warp, a lane passes on half of its values in each of the first steps and adds up the other half: two values
+//  take 6 shuffles, four 6, where each by itself takes 5.  Lane 8 k then has value k (one value: every lane; two: lane 16 k).
+template <int N, class P>
+__device__ __forceinline__ void group_sum(float (&x)[N], const P& at, float* exchange) {
+  constexpr unsigned kAll = 0xffffffffu;
+  if constexpr (P::kSub) {
+    for (int o = at.lanes >> 1; o > 0; o >>= 1)
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] += __shfl_xor_sync(0xffffffffu, x[i], o);
-  if (at.warps == 1) return;
-  float* mine = exchange + at.group * at.warps * N;
-  if (at.lane == 0)
-#pragma unroll
-    for (int i = 0; i < N; ++i) mine[at.warp * N + i] = x[i];
-  asm volatile("bar.sync %0, %1;" ::"r"(at.group + 1), "r"(at.width) : "memory");
-  // every warp adds up the same numbers in the same order
-#pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = at.lane < at.warps ? mine[at.lane * N + i] : 0.f;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] += __shfl_xor_sync(0xffffffffu, x[i], o);
-}
-
-// fp32 copies of a vector's elements at this thread's columns; `otherwise` where there is no vector
-template <class T, int V, int NV>
-__device__ __forceinline__ void load_vector(float (&to)[NV][V], const void* from, int f32, const Place<V>& at, int cols, float otherwise) {
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int c = at.column(i) + j;
-      to[i][j] = otherwise;
-      if (from && c < cols) to[i][j] = f32 ? static_cast<const float*>(from)[c] : static_cast<float>(static_cast<const T*>(from)[c]);
-    }
-}
-
-template <class T, int V, int NV>
-__device__ __forceinline__ void load_row(Piece<T, V> (&to)[NV], const void* from, long long row, long long stride, const Place<V>& at, int cols) {
-  const T* base = static_cast<const T*>(from) + row * stride;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    if (at.column(i) < cols) {
-      load_piece<T, V>(to[i], base + at.column(i));
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; ++j) to[i].e[j] = static_cast<T>(0.f);
-    }
-  }
-}
-
-// Adds up the groups' sums over rows and leaves the block's in `partial` (cols floats).
-template <int V, int NV>
-__device__ __forceinline__ void block_columns(const float (&sum)[NV][V], const Place<V>& at, int cols, float* scratch, float* partial) {
-  if (at.groups == 1) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (at.column(i) + j < cols) partial[at.column(i) + j] = sum[i][j];
+      for (int i = 0; i < N; ++i) x[i] += __shfl_xor_sync(kAll, x[i], o);
     return;
   }
-  // group by group, in their order, through one row of shared memory
-  for (int g = 0; g < at.groups; ++g) {
-    __syncthreads();
-    if (at.group == g) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const int c = at.column(i) + j;
-          if (c < cols) scratch[c] = g == 0 ? sum[i][j] : scratch[c] + sum[i][j];
-        }
-    }
+  const int lane = threadIdx.x & 31;
+  float y = x[0];
+  if constexpr (N > 2) {
+    const bool upper = lane & 16;
+    const float x3 = N > 3 ? x[N - 1] : 0.f;
+    float a0 = (upper ? x[2] : x[0]) + __shfl_xor_sync(kAll, upper ? x[0] : x[2], 16);
+    float a1 = (upper ? x3 : x[1]) + __shfl_xor_sync(kAll, upper ? x[1] : x3, 16);
+    const bool odd = lane & 8;
+    y = (odd ? a1 : a0) + __shfl_xor_sync(kAll, odd ? a0 : a1, 8);
+  } else if constexpr (N == 2) {
+    const bool upper = lane & 16;
+    y = (upper ? x[1] : x[0]) + __shfl_xor_sync(kAll, upper ? x[0] : x[1], 16);
+    y += __shfl_xor_sync(kAll, y, 8);
+  } else {
+    y += __shfl_xor_sync(kAll, y, 16);
+    y += __shfl_xor_sync(kAll, y, 8);
   }
-  __syncthreads();
-  for (int c = threadIdx.x; c < cols; c += blockDim.x) partial[c] = scratch[c];
-  __syncthreads();
-}
-
-template <class T, int V, int NV, int MOST>
-__global__ void __launch_bounds__(MOST, 1) ln_forward_kernel(const __grid_constant__ LnParams p) {
-  extern __shared__ float exchange[];   // two areas of one float per warp
-  pdl_wait();
-  if (threadIdx.x == 0) pdl_launch_dependents();
-  const Place<V> at(p.warps);
-  float w[NV][V], b[NV][V];
-  load_vector<T, V, NV>(w, p.w, p.w_f32, at, p.cols, 1.f);
-  load_vector<T, V, NV>(b, p.b, p.w_f32, at, p.cols, 0.f);
-  const long long step = static_cast<long long>(gridDim.x) * at.groups;
-  for (long long row = static_cast<long long>(blockIdx.x) * at.groups + at.group; row < p.rows; row += step) {
-    Piece<T, V> x[NV];
-    load_row<T, V, NV>(x, p.x, row, p.x_row, at, p.cols);
-    float s[1] = {0.f};
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+  for (int o = 4; o > 0; o >>= 1) y += __shfl_xor_sync(kAll, y, o);
+  constexpr int kStep = N > 2 ? 8 : 16;   // lanes between the values
+  if (at.warps == 1) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) s[0] += static_cast<float>(x[i].e[j]);
-    group_sum<1, V>(s, at, exchange);
-    const float mean = s[0] * p.inv_cols;
-    s[0] = 0.f;
+    for (int i = 0; i < N; ++i) x[i] = __shfl_sync(kAll, y, i * kStep);
+    return;
+  }
+  float4* mine = reinterpret_cast<float4*>(exchange) + at.group * at.warps;
+  if ((lane & (kStep - 1)) == 0) reinterpret_cast<float*>(mine + at.warp)[lane / kStep] = y;
+  at.meet();
+  // every warp adds up the same numbers in the same order
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < N; ++i) x[i] = 0.f;
+  for (int w = 0; w < at.warps; w += 2) {   // (warps is a power of two)
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float d = static_cast<float>(x[i].e[j]) - mean;
-        if (at.column(i) + j < p.cols) s[0] = fmaf(d, d, s[0]);
-      }
-    group_sum<1, V>(s, at, exchange + LN_MAX_WARPS);
-    const float r = 1.f / sqrtf(fmaf(s[0], p.inv_cols, p.eps));
-    T* y = static_cast<T*>(p.y) + row * p.cols;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      Piece<T, V> out;
-#pragma unroll
-      for (int j = 0; j < V; ++j) out.e[j] = static_cast<T>(fmaf((static_cast<float>(x[i].e[j]) - mean) * r, w[i][j], b[i][j]));
-      if (at.column(i) < p.cols) store_piece<T, V>(y + at.column(i), out);
-    }
-    if (at.first == 0) {
-      p.mean[row] = mean;
-      p.rstd[row] = r;
+    for (int h = 0; h < 2; ++h) {
+      const float4 v = mine[w + h];
+      x[0] += v.x;
+      if constexpr (N > 1) x[1] += v.y;
+      if constexpr (N > 2) x[2] += v.z;
+      if constexpr (N > 3) x[3] += v.w;
     }
   }
 }
 
-template <class T, int V, int NV, int MOST>
-__global__ void __launch_bounds__(MOST, 1) ln_backward_kernel(const __grid_constant__ LnParams p) {
-  extern __shared__ float exchange[];   // two areas of two floats per warp, then a row for the sums over rows
-  pdl_wait();
-  if (threadIdx.x == 0) pdl_launch_dependents();
-  const Place<V> at(p.warps);
-  float w[NV][V], dw[NV][V], db[NV][V];
-  load_vector<T, V, NV>(w, p.w, p.w_f32, at, p.cols, 1.f);
-#pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < V; ++j) dw[i][j] = db[i][j] = 0.f;
-  const long long step = static_cast<long long>(gridDim.x) * at.groups;
-  int turn = 0;
-  for (long long row = static_cast<long long>(blockIdx.x) * at.groups + at.group; row < p.rows; row += step, turn ^= 1) {
-    Piece<T, V> x[NV], dy[NV];
-    load_row<T, V, NV>(x, p.x, row, p.x_row, at, p.cols);
-    load_row<T, V, NV>(dy, p.dy, row, p.dy_row, at, p.cols);
-    const float mean = p.mean_in[row], r = p.rstd_in[row];
-    float s[2] = {0.f, 0.f};   // sums of g, g h  (dy is zero behind the last column)
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float h = (static_cast<float>(x[i].e[j]) - mean) * r, d = static_cast<float>(dy[i].e[j]), g = d * w[i][j];
-        dw[i][j] = fmaf(d, h, dw[i][j]);
-        db[i][j] += d;
-        s[0] += g;
-        s[1] = fmaf(g, h, s[1]);
-      }
-    group_sum<2, V>(s, at, exchange + turn * 2 * LN_MAX_WARPS);
-    const float m = s[0] * p.inv_cols, q = s[1] * p.inv_cols;
-    T* dx = static_cast<T*>(p.dx) + row * p.cols;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      Piece<T, V> out;
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float h = (static_cast<float>(x[i].e[j]) - mean) * r, g = static_cast<float>(dy[i].e[j]) * w[i][j];
-        out.e[j] = static_cast<T>(r * (g - m - h * q));
-      }
-      if (at.column(i) < p.cols) store_piece<T, V>(dx + at.column(i), out);
-    }
-  }
-  if (p.partial) {
-    float* scratch = exchange + 4 * LN_MAX_WARPS;
-    float* to = p.partial + static_cast<long long>(blockIdx.x) * 2 * p.cols;
-    if (p.want_dw) block_columns<V, NV>(dw, at, p.cols, scratch, to);
-    if (p.want_db) block_columns<V, NV>(db, at, p.cols, scratch, to + p.cols);
-  }
-}
+// How the three kernels are laid out: blocks of 256, 512 or 1024 threads, 512 threads an SM with 128 registers each (64 in blocks
+// of 1024, which only the longest rows take).
+enum { kLnForward, kLnBackward, kLnBwdbwd };
+constexpr int kLnThreads = 512;
+template <int WHAT, class T, int V, int NV, int THREADS, bool SUB>
+struct LnCfg {
+  static constexpr int kMatrices = WHAT == kLnForward ? 1 : (WHAT == kLnBackward ? 2 : 3);
+  static constexpr int kBlocks = kLnThreads > THREADS ? kLnThreads / THREADS : 1;   // of an SM
+  // Bytes of a row of the ring.  Off the grid a row may start anywhere in a piece of 16 bytes: one more for each group.
+  static constexpr int kRow = THREADS * NV * V * static_cast<int>(sizeof(T)) + (kWide<T, V> ? 0 : 16 * THREADS / (SUB ? 2 : 32));
+  static constexpr int kFit = 200 * 1024 / kBlocks / (kMatrices * kRow);
+  static constexpr int kStages = kFit > 4 ? 4 : kFit;                         // rows of the ring
+  static constexpr int kExchange = 2 * LN_MAX_WARPS * 16;                     // bytes in front of it: two areas for the sums over a row
+  static constexpr int kSmem = kExchange + kMatrices * kRow * kStages;
+  static constexpr bool kHold = WHAT != kLnBwdbwd || NV * V <= 8;             // vectors over the columns stay in registers
+  static_assert(kStages >= 1, "a row of the ring");
+  static_assert(WHAT == kLnForward || THREADS * NV * V * 4 <= kSmem - kExchange, "room for the sums over rows, see block_columns");
+};
 
-template <class T, int V, int NV, int MOST>
-__global__ void __launch_bounds__(MOST, 1) ln_bwdbwd_kernel(const __grid_constant__ LnParams p) {
-  extern __shared__ float exchange[];   // areas of four and of three floats per warp, then a row for the sums over rows
-  pdl_wait();
-  if (threadIdx.x == 0) pdl_launch_dependents();
-  const Place<V> at(p.warps);
-  float w[NV][V], vw[NV][V], vb[NV][V], dw2[NV][V];
-  load_vector<T, V, NV>(w, p.w, p.w_f32, at, p.cols, 1.f);
-  load_vector<T, V, NV>(vw, p.vw, p.w_f32, at, p.cols, 0.f);
-  load_vector<T, V, NV>(vb, p.vb, p.w_f32, at, p.cols, 0.f);
+// The ring.  On the grid it is a thread's own: piece i of (stage, matrix) is THREADS * 16 bytes on from piece i - 1.  Off the
+// grid a row lies as in memory, from the piece of 16 bytes on that holds its first element.
+template <class C, class T, int V, int NV, int THREADS, bool SUB>
+struct Ring {
+  uint32_t base;
+  const Place<T, V, SUB>& at;
+  int cols;
+  __device__ __forceinline__ Ring(const void* smem, const Place<T, V, SUB>& place, int n) : at(place), cols(n) {
+    base = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
+    if (kWide<T, V>) base += threadIdx.x * 16;
+    else base += at.group * (at.width * NV * V * static_cast<int>(sizeof(T)) + 16);
+  }
+  __device__ __forceinline__ uint32_t slot(int stage, int matrix) const { return base + (stage * C::kMatrices + matrix) * C::kRow; }
+  __device__ __forceinline__ void copy(int stage, int matrix, const T* row, bool live) const {
+    const uint32_t to = slot(stage, matrix);
+    if constexpr (kWide<T, V>) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-#pragma unroll
-    for (int j = 0; j < V; ++j) dw2[i][j] = 0.f;
-  const long long step = static_cast<long long>(gridDim.x) * at.groups;
-  for (long long row = static_cast<long long>(blockIdx.x) * at.groups + at.group; row < p.rows; row += step) {
-    Piece<T, V> x[NV], dy[NV], v[NV];
-    load_row<T, V, NV>(x, p.x, row, p.x_row, at, p.cols);
-    load_row<T, V, NV>(dy, p.dy, row, p.dy_row, at, p.cols);
-    if (p.v) {
-      load_row<T, V, NV>(v, p.v, row, p.v_row, at, p.cols);
+      for (int i = 0; i < NV; ++i) {
+        const bool there = live && at.column(i) < cols;
+        cp_async(to + i * (THREADS * 16), there ? row + at.column(i) : row, there ? 16 : 0);
+      }
     } else {
+      // (what lies in front of the row in its first 16 bytes of memory belongs to the same allocation: that starts on 16 bytes)
+      const uintptr_t start = reinterpret_cast<uintptr_t>(row) & ~static_cast<uintptr_t>(15);
+      const int bytes = live ? static_cast<int>(reinterpret_cast<uintptr_t>(row) - start) + cols * static_cast<int>(sizeof(T)) : 0;
+      constexpr int kPieces = NV * V * static_cast<int>(sizeof(T)) / 16;
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[i].e[j] = static_cast<T>(0.f);
-    }
-    const float mean = p.mean_in[row], r = p.rstd_in[row];
-    float s[4] = {0.f, 0.f, 0.f, 0.f};   // v, v h, g, g h
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float h = (static_cast<float>(x[i].e[j]) - mean) * r, u = static_cast<float>(v[i].e[j]);
-        const float g = static_cast<float>(dy[i].e[j]) * w[i][j];
-        s[0] += u;
-        s[1] = fmaf(u, h, s[1]);
-        s[2] += g;
-        s[3] = fmaf(g, h, s[3]);
-      }
-    group_sum<4, V>(s, at, exchange);
-    const float a = s[0] * p.inv_cols, c = s[1] * p.inv_cols, m = s[2] * p.inv_cols, q = s[3] * p.inv_cols;
-    float t[3] = {0.f, 0.f, 0.f};        // p (g - m - h q), e, e h
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float h = (static_cast<float>(x[i].e[j]) - mean) * r, u = static_cast<float>(v[i].e[j]), d = static_cast<float>(dy[i].e[j]);
-        const float g = d * w[i][j], pp = u - a - h * c;
-        const float e = fmaf(vw[i][j], d, -r * (g * c + u * q));   // zero behind the last column, as d and u are
-        dw2[i][j] = fmaf(d * r, pp, dw2[i][j]);
-        if (at.column(i) + j < p.cols) t[0] = fmaf(pp, g - m - h * q, t[0]);
-        t[1] += e;
-        t[2] = fmaf(e, h, t[2]);
-      }
-    group_sum<3, V>(t, at, exchange + 4 * LN_MAX_WARPS);
-    const float k = t[0] * p.inv_cols * r, me = t[1] * p.inv_cols, meh = t[2] * p.inv_cols;
-    T *ddy = static_cast<T*>(p.y) + row * p.cols, *dx2 = static_cast<T*>(p.dx) + row * p.cols;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      Piece<T, V> o1, o2;
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float h = (static_cast<float>(x[i].e[j]) - mean) * r, u = static_cast<float>(v[i].e[j]), d = static_cast<float>(dy[i].e[j]);
-        const float e = fmaf(vw[i][j], d, -r * (d * w[i][j] * c + u * q));
-        o1.e[j] = static_cast<T>(fmaf(r * w[i][j], u - a - h * c, fmaf(vw[i][j], h, vb[i][j])));
-        o2.e[j] = static_cast<T>(r * (e - me - h * (meh + k)));
-      }
-      if (at.column(i) < p.cols) {
-        store_piece<T, V>(ddy + at.column(i), o1);
-        store_piece<T, V>(dx2 + at.column(i), o2);
+      for (int i = 0; i <= kPieces; ++i) {
+        const int from = (at.first + i * at.width) * 16;
+        if (from < bytes) cp_async(to + from, reinterpret_cast<const void*>(start + from), min(16, bytes - from));
       }
     }
   }
-  if (p.partial) block_columns<V, NV>(dw2, at, p.cols, exchange + 7 * LN_MAX_WARPS, p.partial + static_cast<long long>(blockIdx.x) * 2 * p.cols);
+  __device__ __forceinline__ void read(float2 (&to)[NV][V / 2], int stage, int matrix, const T* row, bool live) const {
+    const uint32_t from = slot(stage, matrix);
+    if constexpr (kWide<T, V>) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        uint32_t w[4];
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(from + i * (THREADS * 16)));
+        if constexpr (sizeof(T) == 4) {
+          to[i][0] = f2(w[0], w[1]);
+          to[i][1] = f2(w[2], w[3]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) to[i][j] = unpack<T>(w[j]);
+        }
+      }
+    } else {
+      const uint32_t first = from + (reinterpret_cast<uintptr_t>(row) & 15u);
+      auto element = [&](int c) {
+        float v = 0.f;
+        if (live && c < cols) {
+          if constexpr (sizeof(T) == 4) {
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(first + c * 4));
+          } else {
+            uint16_t u;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(first + c * 2));
+            v = unpack<T>(u).x;
+          }
+        }
+        return v;
+      };
+#pragma unroll
+      for (int i = 0; i < NV; ++i) to[i][0] = make_float2(element(at.column(i, 0)), element(at.column(i, 1)));
+    }
+  }
+};
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+
+// Adds up the groups' sums over rows and leaves the block's in `partial` (cols floats).  `scratch`: a row of cols floats per
+// warp or group of warps, in the ring, which is no longer in use.
+template <class T, int V, int NV, bool SUB>
+__device__ __forceinline__ void block_columns(float2 (&sum)[NV][V / 2], const Place<T, V, SUB>& at, int cols, float* scratch, float* partial) {
+  // the groups of a warp hold the same columns in lanes `lanes` apart
+  for (int o = at.lanes; o < 32; o <<= 1)
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) {
+        sum[i][j].x += __shfl_xor_sync(0xffffffffu, sum[i][j].x, o);
+        sum[i][j].y += __shfl_xor_sync(0xffffffffu, sum[i][j].y, o);
+      }
+  const int rows = (blockDim.x >> 5) / at.warps, mine = (threadIdx.x >> 5) / at.warps;
+  __syncthreads();
+  if (at.above == 0)
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < V / 2; ++j) {
+        const int c0 = at.column(i, 2 * j), c1 = at.column(i, 2 * j + 1);
+        if (c0 < cols) scratch[mine * cols + c0] = sum[i][j].x;
+        if (c1 < cols) scratch[mine * cols + c1] = sum[i][j].y;
+      }
+  __syncthreads();
+  for (int c = threadIdx.x; c < cols; c += blockDim.x) {
+    float total = scratch[c];
+    for (int r = 1; r < rows; ++r) total += scratch[r * cols + c];
+    partial[c] = total;
+  }
 }
 
-// Sums over the blocks: a warp takes 32 columns, eight warps of a block a share of the rows of `partial` each, in order.
+template <class T, int V, int NV, int THREADS, bool SUB>
+__global__ void __launch_bounds__(THREADS, LnCfg<kLnForward, T, V, NV, THREADS, SUB>::kBlocks) ln_forward_kernel(const __grid_constant__ LnParams p) {
+  using C = LnCfg<kLnForward, T, V, NV, THREADS, SUB>;
+  constexpr int H = V / 2;   // pairs of a piece
+  extern __shared__ __align__(16) float exchange[];
+  pdl_wait();
+  if (threadIdx.x == 0) pdl_launch_dependents();
+  const Place<T, V, SUB> at(p.warps, p.lanes);
+  const Ring<C, T, V, NV, THREADS, SUB> ring(reinterpret_cast<char*>(exchange) + C::kExchange, at, p.cols);
+  const int step = gridDim.x * at.groups;
+  int row = blockIdx.x * at.groups + at.group;
+  auto x_of = [&](int r) { return static_cast<const T*>(p.x) + (r < p.rows ? r : 0) * p.x_row; };
+  auto fetch = [&](int stage, int r) {
+    ring.copy(stage, 0, x_of(r), r < p.rows);
+    copies_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < C::kStages - 1; ++i) fetch(i, row + i * step);
+  float2 w[NV][H], b[NV][H];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    at.vector(w[i], p.w, p.w_f32, i, p.cols, 1.f);
+    at.vector(b[i], p.b, p.w_f32, i, p.cols, 0.f);
+  }
+  for (int stage = 0; row - at.above < p.rows; row += step, stage = stage + 1 == C::kStages ? 0 : stage + 1) {
+    fetch(stage == 0 ? C::kStages - 1 : stage - 1, row + (C::kStages - 1) * step);   // where the row before this one was
+    copies_wait<C::kStages - 1>();
+    if (!kWide<T, V>) at.meet();   // the group's copies
+    float2 x[NV][H], s2 = both(0.f);
+    ring.read(x, stage, 0, x_of(row), row < p.rows);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < H; ++j) s2 = __fadd2_rn(s2, x[i][j]);
+    float s[1] = {s2.x + s2.y};
+    group_sum<1>(s, at, exchange);
+    const float mean = s[0] * p.inv_cols;
+    s2 = both(0.f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const float2 minus = at.inside(-mean, i, p.cols);   // zeros stay zeros behind the last column
+#pragma unroll
+      for (int j = 0; j < H; ++j) {
+        x[i][j] = __fadd2_rn(x[i][j], minus);
+        s2 = __ffma2_rn(x[i][j], x[i][j], s2);
+      }
+    }
+    s[0] = s2.x + s2.y;
+    group_sum<1>(s, at, exchange + 4 * LN_MAX_WARPS);
+    const float r = rsqrtf(fmaf(s[0], p.inv_cols, p.eps));
+    if (row < p.rows) {
+      T* y = static_cast<T*>(p.y) + static_cast<long long>(row) * p.cols;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+#pragma unroll
+        for (int j = 0; j < H; ++j) x[i][j] = __ffma2_rn(__fmul2_rn(x[i][j], both(r)), w[i][j], b[i][j]);
+        at.store(y, i, p.cols, x[i]);
+      }
+      if (at.first == 0) {
+        p.mean[row] = mean;
+        p.rstd[row] = r;
+      }
+    }
+  }
+  copies_wait<0>();
+}
+
+template <class T, int V, int NV, int THREADS, bool SUB>
+__global__ void __launch_bounds__(THREADS, LnCfg<kLnBackward, T, V, NV, THREADS, SUB>::kBlocks) ln_backward_kernel(const __grid_constant__ LnParams p) {
+  using C = LnCfg<kLnBackward, T, V, NV, THREADS, SUB>;
+  constexpr int H = V / 2;
+  extern __shared__ __align__(16) float exchange[];
+  pdl_wait();
+  if (threadIdx.x == 0) pdl_launch_dependents();
+  const Place<T, V, SUB> at(p.warps, p.lanes);
+  char* in_ring = reinterpret_cast<char*>(exchange) + C::kExchange;
+  const Ring<C, T, V, NV, THREADS, SUB> ring(in_ring, at, p.cols);
+  const int step = gridDim.x * at.groups;
+  int row = blockIdx.x * at.groups + at.group;
+  auto x_of = [&](int r) { return static_cast<const T*>(p.x) + (r < p.rows ? r : 0) * p.x_row; };
+  auto dy_of = [&](int r) { return static_cast<const T*>(p.dy) + (r < p.rows ? r : 0) * p.dy_row; };
+  auto fetch = [&](int stage, int r) {
+    ring.copy(stage, 0, x_of(r), r < p.rows);
+    ring.copy(stage, 1, dy_of(r), r < p.rows);
+    copies_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < C::kStages - 1; ++i) fetch(i, row + i * step);
+  float2 w[NV][H], dw[NV][H], db[NV][H];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    at.vector(w[i], p.w, p.w_f32, i, p.cols, 1.f);
+#pragma unroll
+    for (int j = 0; j < H; ++j) dw[i][j] = db[i][j] = both(0.f);
+  }
+  float next_mean = 0.f, next_r = 0.f;
+  auto fetch_statistics = [&](int r) {
+    next_mean = r < p.rows ? p.mean_in[r] : 0.f;
+    next_r = r < p.rows ? p.rstd_in[r] : 0.f;
+  };
+  fetch_statistics(row);
+  int turn = 0;
+  for (int stage = 0; row - at.above < p.rows; row += step, turn ^= 1, stage = stage + 1 == C::kStages ? 0 : stage + 1) {
+    fetch(stage == 0 ? C::kStages - 1 : stage - 1, row + (C::kStages - 1) * step);   // where the row before this one was
+    const float mean = next_mean, r = next_r;
+    fetch_statistics(row + step);
+    copies_wait<C::kStages - 1>();
+    if (!kWide<T, V>) at.meet();   // the group's copies
+    float2 h[NV][H], g[NV][H], s0 = both(0.f), s1 = both(0.f);   // sums of g, g h
+    ring.read(h, stage, 0, x_of(row), row < p.rows);
+    ring.read(g, stage, 1, dy_of(row), row < p.rows);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const float2 minus = at.inside(-mean, i, p.cols);   // behind the last column and row h and dy are zero
+#pragma unroll
+      for (int j = 0; j < H; ++j) {
+        h[i][j] = __fmul2_rn(__fadd2_rn(h[i][j], minus), both(r));
+        dw[i][j] = __ffma2_rn(g[i][j], h[i][j], dw[i][j]);
+        db[i][j] = __fadd2_rn(db[i][j], g[i][j]);
+        g[i][j] = __fmul2_rn(g[i][j], w[i][j]);
+        s0 = __fadd2_rn(s0, g[i][j]);
+        s1 = __ffma2_rn(g[i][j], h[i][j], s1);
+      }
+    }
+    float s[2] = {s0.x + s0.y, s1.x + s1.y};
+    group_sum<2>(s, at, exchange + turn * 4 * LN_MAX_WARPS);
+    if (row < p.rows) {
+      const float2 m = both(-s[0] * p.inv_cols), q = both(-s[1] * p.inv_cols);
+      T* dx = static_cast<T*>(p.dx) + static_cast<long long>(row) * p.cols;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+#pragma unroll
+        for (int j = 0; j < H; ++j) g[i][j] = __fmul2_rn(__ffma2_rn(h[i][j], q, __fadd2_rn(g[i][j], m)), both(r));
+        at.store(dx, i, p.cols, g[i]);
+      }
+    }
+  }
+  copies_wait<0>();
+  if (p.partial) {
+    float* to = p.partial + static_cast<long long>(blockIdx.x) * 2 * p.cols;
+    if (p.want_dw) block_columns<T, V, NV, SUB>(dw, at, p.cols, reinterpret_cast<float*>(in_ring), to);
+    if (p.want_db) block_columns<T, V, NV, SUB>(db, at, p.cols, reinterpret_cast<float*>(in_ring), to + p.cols);
+  }
+}
+
+template <class T, int V, int NV, int THREADS, bool SUB>
+__global__ void __launch_bounds__(THREADS, LnCfg<kLnBwdbwd, T, V, NV, THREADS, SUB>::kBlocks) ln_bwdbwd_kernel(const __grid_constant__ LnParams p) {
+  using C = LnCfg<kLnBwdbwd, T, V, NV, THREADS, SUB>;
+  constexpr int H = V / 2;
+  extern __shared__ __align__(16) float exchange[];
+  pdl_wait();
+  if (threadIdx.x == 0) pdl_launch_dependents();
+  const Place<T, V, SUB> at(p.warps, p.lanes);
+  char* in_ring = reinterpret_cast<char*>(exchange) + C::kExchange;
+  const Ring<C, T, V, NV, THREADS, SUB> ring(in_ring, at, p.cols);
+  const int step = gridDim.x * at.groups;
+  int row = blockIdx.x * at.groups + at.group;
+  auto x_of = [&](int r) { return static_cast<const T*>(p.x) + (r < p.rows ? r : 0) * p.x_row; };
+  auto dy_of = [&](int r) { return static_cast<const T*>(p.dy) + (r < p.rows ? r : 0) * p.dy_row; };
+  auto v_of = [&](int r) { return p.v ? static_cast<const T*>(p.v) + (r < p.rows ? r : 0) * p.v_row : x_of(r); };
+  auto fetch = [&](int stage, int r) {
+    ring.copy(stage, 0, x_of(r), r < p.rows);
+    ring.copy(stage, 1, dy_of(r), r < p.rows);
+    ring.copy(stage, 2, v_of(r), p.v && r < p.rows);   // zeros if there is none
+    copies_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < C::kStages - 1; ++i) fetch(i, row + i * step);
+  float2 w[NV][H], vw[NV][H], vb[NV][H], dw2[NV][H];
+  // what of them is not kept in registers is read (from L1) where it is needed
+  auto w_again = [&](int i) { if (!C::kHold) at.vector(w[i], p.w, p.w_f32, i, p.cols, 1.f); };
+  auto vw_again = [&](int i) { if (!C::kHold) at.vector(vw[i], p.vw, p.w_f32, i, p.cols, 0.f); };
+  auto vb_again = [&](int i) { if (!C::kHold) at.vector(vb[i], p.vb, p.w_f32, i, p.cols, 0.f); };
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (C::kHold) {
+      at.vector(w[i], p.w, p.w_f32, i, p.cols, 1.f);
+      at.vector(vw[i], p.vw, p.w_f32, i, p.cols, 0.f);
+      at.vector(vb[i], p.vb, p.w_f32, i, p.cols, 0.f);
+    }
+#pragma unroll
+    for (int j = 0; j < H; ++j) dw2[i][j] = both(0.f);
+  }
+  float next_mean = 0.f, next_r = 0.f;
+  auto fetch_statistics = [&](int r) {
+    next_mean = r < p.rows ? p.mean_in[r] : 0.f;
+    next_r = r < p.rows ? p.rstd_in[r] : 0.f;
+  };
+  fetch_statistics(row);
+  for (int stage = 0; row - at.above < p.rows; row += step, stage = stage + 1 == C::kStages ? 0 : stage + 1) {
+    fetch(stage == 0 ? C::kStages - 1 : stage - 1, row + (C::kStages - 1) * step);   // where the row before this one was
+    const float mean = next_mean, r = next_r;
+    fetch_statistics(row + step);
+    copies_wait<C::kStages - 1>();
+    if (!kWide<T, V>) at.meet();   // the group's copies
+    // h, dy and v; all zero behind the last column and the last row
+    float2 h[NV][H], d[NV][H], u[NV][H], s0 = both(0.f), s1 = both(0.f), s2 = both(0.f), s3 = both(0.f);
+    ring.read(h, stage, 0, x_of(row), row < p.rows);
+    ring.read(d, stage, 1, dy_of(row), row < p.rows);
+    ring.read(u, stage, 2, v_of(row), p.v && row < p.rows);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const float2 minus = at.inside(-mean, i, p.cols);
+      w_again(i);
+#pragma unroll
+      for (int j = 0; j < H; ++j) {
+        h[i][j] = __fmul2_rn(__fadd2_rn(h[i][j], minus), both(r));
+        const float2 g = __fmul2_rn(d[i][j], w[i][j]);
+        s0 = __fadd2_rn(s0, u[i][j]);
+        s1 = __ffma2_rn(u[i][j], h[i][j], s1);
+        s2 = __fadd2_rn(s2, g);
+        s3 = __ffma2_rn(g, h[i][j], s3);
+      }
+    }
+    float s[4] = {s0.x + s0.y, s1.x + s1.y, s2.x + s2.y, s3.x + s3.y};
+    group_sum<4>(s, at, exchange);
+    const float a = s[0] * p.inv_cols, c = s[1] * p.inv_cols, m = s[2] * p.inv_cols, q = s[3] * p.inv_cols;
+    s0 = s1 = s2 = both(0.f);   // sums of p (g - m - h q), e, e h
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const float2 minus = at.inside(-a, i, p.cols);
+      w_again(i);
+      vw_again(i);
+#pragma unroll
+      for (int j = 0; j < H; ++j) {
+        const float2 g = __fmul2_rn(d[i][j], w[i][j]);
+        const float2 e = __ffma2_rn(vw[i][j], d[i][j], __ffma2_rn(g, both(-r * c), __fmul2_rn(u[i][j], both(-r * q))));
+        const float2 pp = __ffma2_rn(h[i][j], both(-c), __fadd2_rn(u[i][j], minus));
+        dw2[i][j] = __ffma2_rn(__fmul2_rn(d[i][j], both(r)), pp, dw2[i][j]);
+        s0 = __ffma2_rn(pp, __ffma2_rn(h[i][j], both(-q), __fadd2_rn(g, both(-m))), s0);
+        s1 = __fadd2_rn(s1, e);
+        s2 = __ffma2_rn(e, h[i][j], s2);
+        u[i][j] = pp;
+        d[i][j] = e;
+      }
+    }
+    float t[3] = {s0.x + s0.y, s1.x + s1.y, s2.x + s2.y};
+    group_sum<3>(t, at, exchange + 4 * LN_MAX_WARPS);
+    if (row < p.rows) {
+      const float k = t[0] * p.inv_cols * r, me = t[1] * p.inv_cols, meh = t[2] * p.inv_cols;
+      T *ddy = static_cast<T*>(p.y) + static_cast<long long>(row) * p.cols, *dx2 = static_cast<T*>(p.dx) + static_cast<long long>(row) * p.cols;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        w_again(i);
+        vw_again(i);
+        vb_again(i);
+#pragma unroll
+        for (int j = 0; j < H; ++j) {
+          u[i][j] = __ffma2_rn(__fmul2_rn(w[i][j], both(r)), u[i][j], __ffma2_rn(vw[i][j], h[i][j], vb[i][j]));
+          d[i][j] = __fmul2_rn(__ffma2_rn(h[i][j], both(-(meh + k)), __fadd2_rn(d[i][j], both(-me))), both(r));
+        }
+        at.store(ddy, i, p.cols, u[i]);
+        at.store(dx2, i, p.cols, d[i]);
+      }
+    }
+  }
+  copies_wait<0>();
+  if (p.partial) block_columns<T, V, NV, SUB>(dw2, at, p.cols, reinterpret_cast<float*>(in_ring), p.partial + static_cast<long long>(blockIdx.x) * 2 * p.cols);
+}
+
+// Sums over the blocks: a block takes 32 columns, its 32 warps a share of the rows of `partial` each, in order.
 template <class W>
-__global__ void __launch_bounds__(256) ln_columns_kernel(const float* partial, int blocks, int cols, W* dw, W* db) {
-  __shared__ float part[8][33];
+__global__ void __launch_bounds__(1024) ln_columns_kernel(const float* partial, int blocks, int cols, W* dw, W* db) {
+  __shared__ float part[32][33];
   pdl_wait();
   if (threadIdx.x == 0) pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -339,67 +581,67 @@ __global__ void __launch_bounds__(256) ln_columns_kernel(const float* partial, i
   const float* from = partial + (second ? cols : 0) + c;
   float sum = 0.f;
   if (c < cols)
-#pragma unroll 8
-    for (int i = warp; i < blocks; i += 8) sum += from[static_cast<long long>(i) * 2 * cols];
+#pragma unroll 10
+    for (int i = warp; i < blocks; i += 32) sum += from[static_cast<long long>(i) * 2 * cols];
   part[warp][lane] = sum;
   __syncthreads();
   if (warp == 0 && c < cols) {
 #pragma unroll
-    for (int i = 1; i < 8; ++i) sum += part[i][lane];
+    for (int i = 1; i < 32; ++i) sum += part[i][lane];
     (second ? db : dw)[c] = static_cast<W>(sum);
   }
 }
 
-enum { kLnForward, kLnBackward, kLnBwdbwd };
-
-// How a call is cut up.  A thread has at most 16 elements of a row: what it keeps of each column besides (weights, sums:
-// two to four fp32 numbers) then stays in registers at two blocks of 256 threads an SM.
+// How a call is cut up.
 struct LnGrid {
-  int v, nv, warps, threads, blocks;
+  bool wide;
+  int each, lanes, warps, threads, blocks;   // elements of a thread; of a group: lanes and warps; threads and blocks
 };
 constexpr int kSms = 148;
 constexpr int kLnMostBlocks = 4 * kSms;
 
-LnGrid ln_grid(int what, long long rows, int cols, int element, int v) {
+LnGrid ln_grid(int what, long long rows, int cols, bool wide) {
   LnGrid g;
-  g.v = v;
-  // 8 elements a thread where that is one warp's row anyway, or where there are too few rows to fill the GPU and
-  // a row's own time counts; else 16
-  const int each = cols <= 256 || rows <= kSms ? 8 : 16;
-  g.nv = each / v;
+  g.wide = wide;
+  // 16 elements a thread.  8 in the double backward (there are more to keep of each), unless rows are long, and where there are
+  // too few rows to fill the GPU and a row's own time counts.
+  g.each = cols <= 4096 && (what == kLnBwdbwd || rows <= kSms) ? 8 : 16;
+  g.lanes = 32;
+  while (g.lanes > 2 && g.lanes / 2 * g.each >= cols) g.lanes >>= 1;
   g.warps = 1;
-  while (g.warps < LN_MAX_WARPS && g.warps * 32 * each < cols) g.warps <<= 1;
-  if (g.warps * 32 * each < cols) g.nv = 16 / v;
+  while (g.warps < LN_MAX_WARPS && g.warps * 32 * g.each < cols) g.warps <<= 1;
   g.threads = g.warps * 32 > 256 ? g.warps * 32 : 256;
-  const int groups = g.threads / (g.warps * 32);
+  const int groups = g.threads / (g.warps * g.lanes);
   const long long wanted = (rows + groups - 1) / groups;
-  const long long resident = static_cast<long long>(kSms) * (what == kLnForward ? 4 : 2) * 256 / g.threads;
-  g.blocks = static_cast<int>(wanted < resident ? wanted : (resident > kSms ? resident : kSms));
+  const int per_sm = kLnThreads / g.threads;
+  const long long resident = static_cast<long long>(kSms) * (per_sm > 0 ? per_sm : 1);
+  g.blocks = static_cast<int>(wanted < resident ? wanted : resident);
   return g;
 }
 
 template <int WHAT, class T, int V, int NV>
 int ln_run(const LnParams& p, const LnGrid& g, cudaStream_t s) {
-  auto go = [&](auto most) -> int {
-    constexpr int kMost = decltype(most)::value;
-    constexpr auto kernel = WHAT == kLnForward ? ln_forward_kernel<T, V, NV, kMost>
-                                               : (WHAT == kLnBackward ? ln_backward_kernel<T, V, NV, kMost> : ln_bwdbwd_kernel<T, V, NV, kMost>);
-    // areas for the sums of a row, and of several groups (rows of up to 4 warps * 32 * 16 elements) a row for the sums over rows
-    const int groups = g.threads / (g.warps * 32);
-    const int smem = 4 * (7 * LN_MAX_WARPS + (groups > 1 ? p.cols : 0));
-    FHOB_CUDA_OK(launch_pdl(kernel, static_cast<unsigned>(g.blocks), static_cast<unsigned>(g.threads), smem, 1, s, p));
+  auto go = [&](auto threads, auto sub) -> int {
+    constexpr int kThreads = decltype(threads)::value;
+    constexpr bool kSub = decltype(sub)::value;
+    using C = LnCfg<WHAT, T, V, NV, kThreads, kSub>;
+    constexpr auto kernel = WHAT == kLnForward ? ln_forward_kernel<T, V, NV, kThreads, kSub>
+                                               : (WHAT == kLnBackward ? ln_backward_kernel<T, V, NV, kThreads, kSub> : ln_bwdbwd_kernel<T, V, NV, kThreads, kSub>);
+    const int st = allow_smem(kernel, C::kSmem);
+    if (st != FHOB_OK) return st;
+    FHOB_CUDA_OK(launch_pdl(kernel, static_cast<unsigned>(g.blocks), kThreads, C::kSmem, 1, s, p));
     return FHOB_OK;
   };
-  return g.threads > 512 ? go(std::integral_constant<int, 1024>{}) : go(std::integral_constant<int, 512>{});
+  if (g.lanes < 32) return go(std::integral_constant<int, 256>{}, std::true_type{});
+  if (g.threads == 256) return go(std::integral_constant<int, 256>{}, std::false_type{});
+  return g.threads == 512 ? go(std::integral_constant<int, 512>{}, std::false_type{}) : go(std::integral_constant<int, 1024>{}, std::false_type{});
 }
 
 template <int WHAT, class T>
 int ln_pick(const LnParams& p, const LnGrid& g, cudaStream_t s) {
-  constexpr int kWide = 16 / sizeof(T);
-  if (g.v == kWide) return g.nv * g.v == 8 ? ln_run<WHAT, T, kWide, 8 / kWide>(p, g, s) : ln_run<WHAT, T, kWide, 16 / kWide>(p, g, s);
-  if constexpr (sizeof(T) == 2)
-    if (g.v == 2) return g.nv == 4 ? ln_run<WHAT, T, 2, 4>(p, g, s) : ln_run<WHAT, T, 2, 8>(p, g, s);
-  return g.nv == 8 ? ln_run<WHAT, T, 1, 8>(p, g, s) : ln_run<WHAT, T, 1, 16>(p, g, s);
+  constexpr int kPiece = 16 / sizeof(T);
+  if (g.wide) return g.each == 8 ? ln_run<WHAT, T, kPiece, 8 / kPiece>(p, g, s) : ln_run<WHAT, T, kPiece, 16 / kPiece>(p, g, s);
+  return g.each == 8 ? ln_run<WHAT, T, 2, 4>(p, g, s) : ln_run<WHAT, T, 2, 8>(p, g, s);
 }
 
 bool bad_type(int t) { return t != FHOB_BF16 && t != FHOB_F32 && t != FHOB_F16; }
@@ -417,16 +659,17 @@ int ln_call(const FhobLayerNorm* n, LnParams& p, void* dw, void* db, cudaStream_
       together |= reinterpret_cast<uintptr_t>(matrices[i]) | static_cast<uintptr_t>(strides[i] * es);
     }
   together |= static_cast<uintptr_t>(n->cols) * es;
+  for (const void* vector : {n->w, p.b, p.vw, p.vb}) together |= reinterpret_cast<uintptr_t>(vector);
   if (together % es) return FHOB_ERR_ALIGN;
-  const int v = together % 16 == 0 ? 16 / es : (es == 2 && together % 4 == 0 ? 2 : 1);
   p.w = n->w;
   p.w_f32 = n->w_dtype == FHOB_F32;
-  p.rows = n->rows;
+  p.rows = static_cast<int>(n->rows);
   p.cols = n->cols;
   p.eps = n->eps;
   p.inv_cols = 1.f / static_cast<float>(n->cols);
-  const LnGrid g = ln_grid(WHAT, n->rows, n->cols, es, v);
+  const LnGrid g = ln_grid(WHAT, n->rows, n->cols, together % 16 == 0);
   p.warps = g.warps;
+  p.lanes = g.lanes;
   if (dw || db) {
     const size_t need = static_cast<size_t>(g.blocks) * 2 * n->cols * sizeof(float);
     if (!n->workspace || (reinterpret_cast<uintptr_t>(n->workspace) & 255u) || n->workspace_bytes < need) return FHOB_ERR_WORKSPACE;
@@ -441,7 +684,7 @@ int ln_call(const FhobLayerNorm* n, LnParams& p, void* dw, void* db, cudaStream_
   const dim3 grid((n->cols + 31) / 32, dw && db ? 2 : 1);
   auto columns = [&](auto type) -> int {
     using W = decltype(type);
-    FHOB_CUDA_OK(launch_pdl(ln_columns_kernel<W>, grid, 256, 0, 1, s, static_cast<const float*>(p.partial), g.blocks, p.cols, static_cast<W*>(dw),
+    FHOB_CUDA_OK(launch_pdl(ln_columns_kernel<W>, grid, 1024, 0, 1, s, static_cast<const float*>(p.partial), g.blocks, p.cols, static_cast<W*>(dw),
                             static_cast<W*>(db)));
     return FHOB_OK;
   };
@@ -453,7 +696,7 @@ int ln_check(const FhobLayerNorm* n) {
   if (!n || n->rows <= 0 || n->cols <= 0 || !n->x) return FHOB_ERR_ARG;
   if (bad_type(n->dtype) || bad_type(n->w_dtype) || (n->w_dtype != FHOB_F32 && n->w_dtype != n->dtype)) return FHOB_ERR_ARG;
   if (!n->mean || !n->rstd) return FHOB_ERR_ARG;
-  return n->cols > FHOB_LAYER_NORM_MAX_COLS ? FHOB_ERR_SHAPE : FHOB_OK;
+  return n->cols > FHOB_LAYER_NORM_MAX_COLS || n->rows > FHOB_LAYER_NORM_MAX_ROWS ? FHOB_ERR_SHAPE : FHOB_OK;
 }
 
 }  // namespace

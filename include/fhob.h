@@ -403,6 +403,7 @@ int fhob_rotary(const FhobRotary* r, void* stream);
  * bytes, 256-byte aligned; they are added up in a fixed order.
  */
 #define FHOB_LAYER_NORM_MAX_COLS 16384
+#define FHOB_LAYER_NORM_MAX_ROWS 2000000000
 typedef struct FhobLayerNorm {
   int64_t rows;
   int32_t cols;
