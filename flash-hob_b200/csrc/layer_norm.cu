@@ -133,7 +133,7 @@ struct Place {
 // of the block; two such areas take turns, so that one meeting a round is enough (a warp that is a round ahead writes to the
 // other area, and cannot be two ahead).
 //  In a whole warp, a lane passes on half of its values in each of the first steps and adds up the other half: two values
-//  take 6 shuffles, four 6, where each by itself takes 5.  Lane 8 k then has value k (one value: every lane; two: lane 16 k).
+//  take 5 shuffles, four 6, where each by itself takes 5.  Lane 8 k then has value k (one value: every lane; two: lane 16 k).
 template <int N, class P>
 __device__ __forceinline__ void group_sum(float (&x)[N], const P& at, float* exchange) {
   constexpr unsigned kAll = 0xffffffffu;
@@ -168,32 +168,40 @@ __device__ __forceinline__ void group_sum(float (&x)[N], const P& at, float* exc
     for (int i = 0; i < N; ++i) x[i] = __shfl_sync(kAll, y, i * kStep);
     return;
   }
-  float4* mine = reinterpret_cast<float4*>(exchange) + at.group * at.warps;
-  if ((lane & (kStep - 1)) == 0) reinterpret_cast<float*>(mine + at.warp)[lane / kStep] = y;
+  float* mine = exchange + at.group * at.warps * 4;
+  if ((lane & (kStep - 1)) == 0) mine[at.warp * 4 + lane / kStep] = y;
   at.meet();
-  // every warp adds up the same numbers in the same order
+  // Every warp adds up the same numbers in the same order.  Few are read by every lane; of more, lane 4 w + i takes value i of
+  // warp w (of every eighth warp), then the lanes of a value add up.
+  if (at.warps <= 4) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = 0.f;
-  for (int w = 0; w < at.warps; w += 2) {   // (warps is a power of two)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float4 v = mine[w + h];
+    for (int i = 0; i < N; ++i) x[i] = 0.f;
+    for (int w = 0; w < at.warps; ++w) {
+      const float4 v = reinterpret_cast<const float4*>(mine)[w];
       x[0] += v.x;
       if constexpr (N > 1) x[1] += v.y;
       if constexpr (N > 2) x[2] += v.z;
       if constexpr (N > 3) x[3] += v.w;
     }
+    return;
   }
+  y = 0.f;
+  if ((lane & 3) < N)
+    for (int j = lane; j < at.warps * 4; j += 32) y += mine[j];
+#pragma unroll
+  for (int o = 16; o > 2; o >>= 1) y += __shfl_xor_sync(kAll, y, o);
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = __shfl_sync(kAll, y, i);
 }
 
 // How the three kernels are laid out: blocks of 256, 512 or 1024 threads, 512 threads an SM with 128 registers each (64 in blocks
 // of 1024, which only the longest rows take).
 enum { kLnForward, kLnBackward, kLnBwdbwd };
-constexpr int kLnThreads = 512;
+constexpr int ln_threads(int what, bool wide) { return what == kLnForward && wide ? 768 : 512; }   // of an SM
 template <int WHAT, class T, int V, int NV, int THREADS, bool SUB>
 struct LnCfg {
   static constexpr int kMatrices = WHAT == kLnForward ? 1 : (WHAT == kLnBackward ? 2 : 3);
-  static constexpr int kBlocks = kLnThreads > THREADS ? kLnThreads / THREADS : 1;   // of an SM
+  static constexpr int kBlocks = ln_threads(WHAT, kWide<T, V>) > THREADS ? ln_threads(WHAT, kWide<T, V>) / THREADS : 1;   // of an SM
   // Bytes of a row of the ring.  Off the grid a row may start anywhere in a piece of 16 bytes: one more for each group.
   static constexpr int kRow = THREADS * NV * V * static_cast<int>(sizeof(T)) + (kWide<T, V> ? 0 : 16 * THREADS / (SUB ? 2 : 32));
   static constexpr int kFit = 200 * 1024 / kBlocks / (kMatrices * kRow);
@@ -238,7 +246,8 @@ struct Ring {
       }
     }
   }
-  __device__ __forceinline__ void read(float2 (&to)[NV][V / 2], int stage, int matrix, const T* row, bool live) const {
+  // `row_address`: the low bits of the row's address
+  __device__ __forceinline__ void read(float2 (&to)[NV][V / 2], int stage, int matrix, uint32_t row_address, bool live) const {
     const uint32_t from = slot(stage, matrix);
     if constexpr (kWide<T, V>) {
 #pragma unroll
@@ -254,7 +263,7 @@ struct Ring {
         }
       }
     } else {
-      const uint32_t first = from + (reinterpret_cast<uintptr_t>(row) & 15u);
+      const uint32_t first = from + (row_address & 15u);
       auto element = [&](int c) {
         float v = 0.f;
         if (live && c < cols) {
@@ -271,6 +280,30 @@ struct Ring {
 #pragma unroll
       for (int i = 0; i < NV; ++i) to[i][0] = make_float2(element(at.column(i, 0)), element(at.column(i, 1)));
     }
+  }
+};
+// The rows of a matrix that a group goes through: one to copy next, one to work on next.
+template <class T>
+struct Walk {
+  const T* start;
+  const T* ahead;
+  long long by;        // elements from a row to the group's next
+  uint32_t address;    // of the row to work on, low bits
+  __device__ __forceinline__ Walk(const void* matrix, long long stride, int row, int step) {
+    start = static_cast<const T*>(matrix);
+    ahead = start + row * stride;
+    by = step * stride;
+    address = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ahead));
+  }
+  __device__ __forceinline__ const T* next(bool live) {   // rows that do not exist are not read
+    const T* at = live ? ahead : start;
+    ahead += by;
+    return at;
+  }
+  __device__ __forceinline__ uint32_t worked() {
+    const uint32_t at = address;
+    address += static_cast<uint32_t>(by) * static_cast<uint32_t>(sizeof(T));
+    return at;
   }
 };
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -320,9 +353,9 @@ __global__ void __launch_bounds__(THREADS, LnCfg<kLnForward, T, V, NV, THREADS, 
   const Ring<C, T, V, NV, THREADS, SUB> ring(reinterpret_cast<char*>(exchange) + C::kExchange, at, p.cols);
   const int step = gridDim.x * at.groups;
   int row = blockIdx.x * at.groups + at.group;
-  auto x_of = [&](int r) { return static_cast<const T*>(p.x) + (r < p.rows ? r : 0) * p.x_row; };
+  Walk<T> xs(p.x, p.x_row, row, step);
   auto fetch = [&](int stage, int r) {
-    ring.copy(stage, 0, x_of(r), r < p.rows);
+    ring.copy(stage, 0, xs.next(r < p.rows), r < p.rows);
     copies_commit();
   };
 #pragma unroll
@@ -338,7 +371,7 @@ __global__ void __launch_bounds__(THREADS, LnCfg<kLnForward, T, V, NV, THREADS, 
     copies_wait<C::kStages - 1>();
     if (!kWide<T, V>) at.meet();   // the group's copies
     float2 x[NV][H], s2 = both(0.f);
-    ring.read(x, stage, 0, x_of(row), row < p.rows);
+    ring.read(x, stage, 0, xs.worked(), row < p.rows);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -388,11 +421,10 @@ __global__ void __launch_bounds__(THREADS, LnCfg<kLnBackward, T, V, NV, THREADS,
   const Ring<C, T, V, NV, THREADS, SUB> ring(in_ring, at, p.cols);
   const int step = gridDim.x * at.groups;
   int row = blockIdx.x * at.groups + at.group;
-  auto x_of = [&](int r) { return static_cast<const T*>(p.x) + (r < p.rows ? r : 0) * p.x_row; };
-  auto dy_of = [&](int r) { return static_cast<const T*>(p.dy) + (r < p.rows ? r : 0) * p.dy_row; };
+  Walk<T> xs(p.x, p.x_row, row, step), dys(p.dy, p.dy_row, row, step);
   auto fetch = [&](int stage, int r) {
-    ring.copy(stage, 0, x_of(r), r < p.rows);
-    ring.copy(stage, 1, dy_of(r), r < p.rows);
+    ring.copy(stage, 0, xs.next(r < p.rows), r < p.rows);
+    ring.copy(stage, 1, dys.next(r < p.rows), r < p.rows);
     copies_commit();
   };
 #pragma unroll
@@ -418,8 +450,8 @@ __global__ void __launch_bounds__(THREADS, LnCfg<kLnBackward, T, V, NV, THREADS,
     copies_wait<C::kStages - 1>();
     if (!kWide<T, V>) at.meet();   // the group's copies
     float2 h[NV][H], g[NV][H], s0 = both(0.f), s1 = both(0.f);   // sums of g, g h
-    ring.read(h, stage, 0, x_of(row), row < p.rows);
-    ring.read(g, stage, 1, dy_of(row), row < p.rows);
+    ring.read(h, stage, 0, xs.worked(), row < p.rows);
+    ring.read(g, stage, 1, dys.worked(), row < p.rows);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const float2 minus = at.inside(-mean, i, p.cols);   // behind the last column and row h and dy are zero
@@ -466,13 +498,11 @@ __global__ void __launch_bounds__(THREADS, LnCfg<kLnBwdbwd, T, V, NV, THREADS, S
   const Ring<C, T, V, NV, THREADS, SUB> ring(in_ring, at, p.cols);
   const int step = gridDim.x * at.groups;
   int row = blockIdx.x * at.groups + at.group;
-  auto x_of = [&](int r) { return static_cast<const T*>(p.x) + (r < p.rows ? r : 0) * p.x_row; };
-  auto dy_of = [&](int r) { return static_cast<const T*>(p.dy) + (r < p.rows ? r : 0) * p.dy_row; };
-  auto v_of = [&](int r) { return p.v ? static_cast<const T*>(p.v) + (r < p.rows ? r : 0) * p.v_row : x_of(r); };
+  Walk<T> xs(p.x, p.x_row, row, step), dys(p.dy, p.dy_row, row, step), vs(p.v ? p.v : p.x, p.v ? p.v_row : p.x_row, row, step);
   auto fetch = [&](int stage, int r) {
-    ring.copy(stage, 0, x_of(r), r < p.rows);
-    ring.copy(stage, 1, dy_of(r), r < p.rows);
-    ring.copy(stage, 2, v_of(r), p.v && r < p.rows);   // zeros if there is none
+    ring.copy(stage, 0, xs.next(r < p.rows), r < p.rows);
+    ring.copy(stage, 1, dys.next(r < p.rows), r < p.rows);
+    ring.copy(stage, 2, vs.next(r < p.rows), p.v && r < p.rows);   // zeros if there is none
     copies_commit();
   };
 #pragma unroll
@@ -506,9 +536,9 @@ __global__ void __launch_bounds__(THREADS, LnCfg<kLnBwdbwd, T, V, NV, THREADS, S
     if (!kWide<T, V>) at.meet();   // the group's copies
     // h, dy and v; all zero behind the last column and the last row
     float2 h[NV][H], d[NV][H], u[NV][H], s0 = both(0.f), s1 = both(0.f), s2 = both(0.f), s3 = both(0.f);
-    ring.read(h, stage, 0, x_of(row), row < p.rows);
-    ring.read(d, stage, 1, dy_of(row), row < p.rows);
-    ring.read(u, stage, 2, v_of(row), p.v && row < p.rows);
+    ring.read(h, stage, 0, xs.worked(), row < p.rows);
+    ring.read(d, stage, 1, dys.worked(), row < p.rows);
+    ring.read(u, stage, 2, vs.worked(), p.v && row < p.rows);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const float2 minus = at.inside(-mean, i, p.cols);
@@ -605,7 +635,7 @@ LnGrid ln_grid(int what, long long rows, int cols, bool wide) {
   g.wide = wide;
   // 16 elements a thread.  8 in the double backward (there are more to keep of each), unless rows are long, and where there are
   // too few rows to fill the GPU and a row's own time counts.
-  g.each = cols <= 4096 && (what == kLnBwdbwd || rows <= kSms) ? 8 : 16;
+  g.each = what == kLnBwdbwd ? (cols <= (wide ? 4096 : 8192) ? 8 : 16) : (rows <= kSms && cols <= 4096 ? 8 : 16);
   g.lanes = 32;
   while (g.lanes > 2 && g.lanes / 2 * g.each >= cols) g.lanes >>= 1;
   g.warps = 1;
@@ -613,7 +643,7 @@ LnGrid ln_grid(int what, long long rows, int cols, bool wide) {
   g.threads = g.warps * 32 > 256 ? g.warps * 32 : 256;
   const int groups = g.threads / (g.warps * g.lanes);
   const long long wanted = (rows + groups - 1) / groups;
-  const int per_sm = kLnThreads / g.threads;
+  const int per_sm = ln_threads(what, wide) / g.threads;
   const long long resident = static_cast<long long>(kSms) * (per_sm > 0 ? per_sm : 1);
   g.blocks = static_cast<int>(wanted < resident ? wanted : resident);
   return g;
