@@ -96,6 +96,24 @@ __global__ void row_stats_kernel(const float* k1, const float* ndd, const float*
   if (b_out) b_out[i] = -(k23[v] + k1[v] * ndd[v]);
 }
 
+// One block a first key of a head: its rows of sums, of the near queries and of the far ones' parts, in that order.
+template <typename T>
+__global__ void first_keys_kernel(const float* sums, int parts, int sinks, int d, int d_v, int n_k, float scale, T* out0, T* out1) {
+  pdl_wait();
+  if (threadIdx.x == 0) pdl_launch_dependents();
+  const int head = blockIdx.x / sinks, row = blockIdx.x - head * sinks, cols = d + d_v;
+  const size_t slot = static_cast<size_t>(sinks) * cols;
+  const float* from = sums + (static_cast<size_t>(head) * (parts + 1) * sinks + row) * cols;
+  for (int c = threadIdx.x; c < cols; c += blockDim.x) {
+    float total = 0.f;
+#pragma unroll 8
+    for (int i = 0; i <= parts; ++i) total += from[i * slot + c];
+    const size_t at = static_cast<size_t>(head) * n_k + row;
+    if (c < d) out0[at * d + c] = static_cast<T>(total * scale);
+    else out1[at * d_v + c - d] = static_cast<T>(total);
+  }
+}
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Status word of the library itself: receives the device-side conditions of fhob_forward calls
@@ -191,6 +209,9 @@ bool use_tc(const FhobProblem& p) {
   return tc_supported(p);
 }
 
+// Where the sums of the first keys' far queries go: behind everything else in the workspace.
+size_t far_offset(const FhobProblem& p, bool split) { return align256(split ? split_workspace_bytes(p) : fhob_workspace_bytes(p.bh, p.n_q)); }
+
 // The problem of a call with first tokens that stay visible: FHOB_ERR_ARG for sinks without a window.  Where that
 // leaves no key in front of a diagonal hidden, the mask is the window's (it hides none) or plainly causal.
 int attention_problem(const FhobProblem* p, int32_t sink_tokens, Problem* q) {
@@ -200,6 +221,18 @@ int attention_problem(const FhobProblem* p, int32_t sink_tokens, Problem* q) {
   if (sink_tokens == 0 || p->window >= p->n_k) return FHOB_OK;
   if (static_cast<long long>(sink_tokens) + p->window >= p->n_k) q->window = 0;
   else q->sinks = sink_tokens;
+  return FHOB_OK;
+}
+// ... of a backward, whose far queries are split if the workspace has the room for their sums.
+int backward_problem(const FhobProblem* p, int32_t sink_tokens, Problem* q) {
+  const int st = attention_problem(p, sink_tokens, q);
+  if (st != FHOB_OK) return st;
+  const int parts = far_parts(q->n_q, q->n_k, q->window, q->sinks);
+  const size_t at = far_offset(*q, q->impl != FHOB_IMPL_SIMT && tc_split_supported(*q));
+  if (parts > 0 && q->workspace_bytes >= at + far_bytes(*q, q->sinks, parts)) {
+    q->far_parts = parts;
+    q->far_sums = reinterpret_cast<float*>(static_cast<char*>(q->workspace) + at);
+  }
   return FHOB_OK;
 }
 Problem plain_problem(const FhobProblem& p) {
@@ -216,6 +249,20 @@ int run_pass(int pass, const FhobProblem* p, void* stream) {
 }
 
 }  // namespace
+
+int finish_first_keys(const Problem& p, void* out0, void* out1, cudaStream_t s) {
+  const long long blocks = static_cast<long long>(p.bh) * p.sinks;
+  if (blocks > 0x7fffffffLL) return FHOB_ERR_SHAPE;
+  const int d_v = head_dim_v(p);
+  auto go = [&](auto type) {
+    using T = decltype(type);
+    return launch_pdl(first_keys_kernel<T>, static_cast<unsigned>(blocks), 128, 0, 1, s, static_cast<const float*>(p.far_sums), p.far_parts, p.sinks, p.d,
+                      d_v, p.n_k, p.scale, static_cast<T*>(out0), static_cast<T*>(out1));
+  };
+  FHOB_CUDA_OK(p.dtype == FHOB_BF16 ? go(__nv_bfloat16{}) : (p.dtype == FHOB_F16 ? go(__half{}) : go(float{})));
+  return FHOB_OK;
+}
+
 }  // namespace fhob
 
 using namespace fhob;
@@ -251,6 +298,14 @@ size_t fhob_workspace_bytes_problem(const FhobProblem* p) {
   if (!p || p->bh <= 0 || p->n_q <= 0 || p->n_k <= 0) return 0;
   if (p->impl != FHOB_IMPL_SIMT && split_dims_ok(*p)) return split_workspace_bytes(*p);
   return fhob_workspace_bytes(p->bh, p->n_q);
+}
+
+size_t fhob_workspace_bytes_sinks(const FhobProblem* p, int32_t sink_tokens) {
+  const size_t plain = fhob_workspace_bytes_problem(p);
+  Problem q;
+  if (plain == 0 || sink_tokens <= 0 || attention_problem(p, sink_tokens, &q) != FHOB_OK) return plain;
+  const int parts = far_parts(q.n_q, q.n_k, q.window, q.sinks);
+  return parts > 0 ? align256(plain) + far_bytes(q, q.sinks, parts) : plain;
 }
 
 size_t fhob_workspace_bytes(int32_t bh, int32_t n_q) {
@@ -317,7 +372,7 @@ int fhob_bwdbwd_sinks(const FhobProblem* given, int32_t sink_tokens, void* strea
   int st = validate(given, true, true, true);
   if (st != FHOB_OK) return st;
   Problem problem;
-  st = attention_problem(given, sink_tokens, &problem);
+  st = backward_problem(given, sink_tokens, &problem);
   if (st != FHOB_OK) return st;
   const Problem* p = &problem;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -449,7 +504,7 @@ int fhob_backward_sinks(const FhobProblem* given, int32_t sink_tokens, void* dq,
   int st = validate(given, false, false);
   if (st != FHOB_OK) return st;
   Problem problem;
-  st = attention_problem(given, sink_tokens, &problem);
+  st = backward_problem(given, sink_tokens, &problem);
   if (st != FHOB_OK) return st;
   const Problem* p = &problem;
   if (!aligned16(dq) || !aligned16(dk) || !aligned16(dv)) return FHOB_ERR_ALIGN;

@@ -42,6 +42,9 @@ struct RowVectors {
 // sinks > 0 only with a window that hides some key, and then sinks < n_k (see attention_problem in fhob_api.cu).
 struct Problem : FhobProblem {
   int32_t sinks = 0;
+  // Shares of the first keys' far queries, and where their sums go; 0: none (see far_parts)
+  int32_t far_parts = 0;
+  float* far_sums = nullptr;   // [head][far_parts + 1][sinks][d + d_v]
 };
 
 // Head dim of V, ddV, dO, O and of the results ddO, dV2 (0 in the struct = same as d).
@@ -184,6 +187,35 @@ __host__ __device__ inline TileList streamed_tiles(bool q_stationary, int m0, in
   t.count = t.first + end - t.begin;
   return t;
 }
+
+// A first key is seen by every query behind it, a key of the window by `window` of them: the CTA of the first keys would
+// go on for long after the others.  So the queries that see the first keys alone (those behind their window: the far ones) are
+// cut into parts of about as many 64-row tiles as any other key tile has, each the work of a CTA of its own.  These parts, and
+// the CTA with the first keys' near queries, leave fp32 rows of sums, which a last kernel adds up in a fixed order.
+// A function of the lengths alone, as every split of a head.  0: not worth while (few far queries), or too many first keys
+// (their rows of sums are (parts + 1) * sinks: 2048 rows and the near ones).
+inline int far_parts(int n_q, int n_k, int window, int sinks) {
+  if (sinks <= 0 || sinks > 2048) return 0;
+  const int off = n_k - n_q, first_far = window > off ? window - off : 0;
+  const int far = first_far < n_q ? (n_q - first_far + 63) / 64 : 0, usual = static_cast<int>((static_cast<long long>(window) + 127) / 64) + 2;
+  if (far <= usual / 2) return 0;
+  int parts = (far + usual - 1) / usual;
+  if (parts > 64) parts = 64;
+  if (parts > 2048 / sinks) parts = 2048 / sinks;
+  return parts;
+}
+inline size_t far_bytes(const FhobProblem& p, int sinks, int parts) {
+  return parts ? static_cast<size_t>(p.bh) * (parts + 1) * sinks * (p.d + head_dim_v(p)) * sizeof(float) : 0;
+}
+// Streamed query tiles [begin, end) of one part of the far queries of the key tile at m0.
+__host__ __device__ inline void far_tiles(int m0, int tn, int n_q, int off, int window, int part, int parts, int& begin, int& end) {
+  const int first = m0 - off + window, all = (n_q + tn - 1) / tn;
+  const int b = first <= 0 ? 0 : (first < n_q ? first / tn : all);
+  begin = b + static_cast<int>(static_cast<long long>(all - b) * part / parts);
+  end = b + static_cast<int>(static_cast<long long>(all - b) * (part + 1) / parts);
+}
+// Adds up the rows of the first keys and stores them to the two results: out0 (d columns, times scale), out1 (d_v columns).
+int finish_first_keys(const Problem& p, void* out0, void* out1, cudaStream_t s);
 
 // Per-thread record of the last CUDA error (read through fhob_last_cuda_error).
 void set_cuda_error(cudaError_t e, const char* where);

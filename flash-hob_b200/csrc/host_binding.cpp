@@ -124,10 +124,10 @@ bool fill_lse(Call& c, const Tensor& lse) {
 // The stream and its workspace, from the dict the Python path uses too (needs the GIL).  Threads on one stream
 // share it: the library queues the kernels of a call without another's between them.  Memory
 // allocated while a stream is captured belongs to the graph: that is left to the Python path.
-bool take_workspace(Call& c, Tensor& keep) {
+bool take_workspace(Call& c, Tensor& keep, const Mask& m, bool backward) {
   if (at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None) return false;
   c.stream = at::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(c.device)).stream();
-  const size_t need = fhob_workspace_bytes_problem(&c.p);
+  const size_t need = backward && m.sinks ? fhob_workspace_bytes_sinks(&c.p, static_cast<int32_t>(m.sinks)) : fhob_workspace_bytes_problem(&c.p);
   py::tuple key = py::make_tuple(c.device, reinterpret_cast<uintptr_t>(c.stream));
   PyObject* have = PyDict_GetItemWithError(g_workspaces, key.ptr());   // borrowed
   if (have && THPVariable_Check(have)) keep = THPVariable_Unpack(have);
@@ -165,7 +165,7 @@ bool run_bwdbwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor*
   Call c;
   Tensor ws;
   if (!fill(c, {&q, &k, &v, o, &d_o, &ddq, &ddk, &ddv}, scale, m, impl) || !fill_lse(c, lse)) return false;
-  if (!take_workspace(c, ws)) return false;
+  if (!take_workspace(c, ws, m, true)) return false;
   const Tensor* like[4] = {&q, &k, &v, &d_o};
   for (int i = 0; i < 4; ++i) out[i] = empty_like_shape(*like[i]);
   c.p.dq2 = out[0].data_ptr(); c.p.dk2 = out[1].data_ptr(); c.p.dv2 = out[2].data_ptr(); c.p.ddo = out[3].data_ptr();
@@ -177,7 +177,7 @@ bool run_forward(const Tensor& q, const Tensor& k, const Tensor& v, double scale
   Call c;
   Tensor ws;
   if (!fill(c, {&q, &k, &v, nullptr, nullptr, nullptr, nullptr, nullptr}, scale, m, impl)) return false;
-  if (!take_workspace(c, ws)) return false;
+  if (!take_workspace(c, ws, m, false)) return false;
   at::DimVector shape(q.sizes().begin(), q.sizes().end());
   if (need_o) {
     shape.back() = v.size(-1);
@@ -193,7 +193,7 @@ bool run_backward(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
   Call c;
   Tensor ws;
   if (!fill(c, {&q, &k, &v, &o, &d_o, nullptr, nullptr, nullptr}, scale, m, impl) || !fill_lse(c, lse)) return false;
-  if (!take_workspace(c, ws)) return false;
+  if (!take_workspace(c, ws, m, true)) return false;
   const Tensor* like[3] = {&q, &k, &v};
   for (int i = 0; i < 3; ++i) out[i] = empty_like_shape(*like[i]);
   return launched(c, [&] { return fhob_backward_sinks(&c.p, static_cast<int32_t>(m.sinks), out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(), c.stream); });

@@ -31,6 +31,7 @@ struct SimtParams {
   int items_q, items_k;   // (head, tile) pairs of either kind
   int split_q, split_k;   // CTAs that share the streamed tiles of such a pair
   int cluster;            // CTAs of a cluster (a multiple of both)
+  FarWork far;            // of the key-tiled passes; its CTAs come in front of all others
 };
 
 template <typename T>
@@ -194,8 +195,8 @@ __device__ __forceinline__ void store4(void* base, size_t at, const float2& a, c
 
 // Streamed tiles of an item.  Elements are masked pair by pair here, so a tile that holds both first keys and keys of
 // the window comes once.
-__device__ __forceinline__ TileList simt_tiles(bool q_stationary, int m0, int tile, int n_strm, const SimtParams& p) {
-  TileList list = streamed_tiles(q_stationary, m0, OM, tile, n_strm, p.n_k - p.n_q, p.causal, p.window, p.sinks);
+__device__ __forceinline__ TileList simt_tiles(bool q_stationary, int m0, int tile, int n_strm, const SimtParams& p, int sinks) {
+  TileList list = streamed_tiles(q_stationary, m0, OM, tile, n_strm, p.n_k - p.n_q, p.causal, p.window, sinks);
   if (list.begin < list.first) {
     const int twice = min(list.first - list.begin, list.count - list.first);
     list.begin += twice;
@@ -204,8 +205,9 @@ __device__ __forceinline__ TileList simt_tiles(bool q_stationary, int m0, int ti
   return list;
 }
 
+// `far`: a key-tiled pass over a part of the queries that see first keys behind their window.
 template <typename T, int MODE>
-__device__ __forceinline__ void simt_body(const SimtParams& p, int block) {
+__device__ __forceinline__ void simt_body(const SimtParams& p, int block, bool far) {
   using C = Tiles<MODE>;
   constexpr bool kQStat = C::kQStat, kFirst = C::kFirst;
   extern __shared__ float smem[];
@@ -224,8 +226,9 @@ __device__ __forceinline__ void simt_body(const SimtParams& p, int block) {
   const int ty = tid >> 3, tx = tid & 7;     // scores: rows 4 ty + i, streamed rows tx + 8 j
   const int ry = tid >> 4, cx = tid & 15;    // outputs: rows 8 ry + i, columns 4 cx.. and 64 + 4 cx..
   // with few tiles a head the streamed axis is split over the CTAs of a cluster
-  const int split = kQStat ? p.split_q : p.split_k;
-  const CtaWork work = cta_work(block, split, kQStat ? p.items_q : p.items_k);   // the grid is padded to whole clusters
+  const int split = far ? 1 : (kQStat ? p.split_q : p.split_k);
+  // the grid is padded to whole clusters
+  const CtaWork work = far ? cta_work(block, p.far.parts, p.far.blocks) : cta_work(block, split, kQStat ? p.items_q : p.items_k);
   const int item = work.item, begin_part = work.part;
   const bool padding = !work.live;
   const int tile_no = item / p.bh, bh = item - tile_no * p.bh;   // causal: the longest tiles of all heads first
@@ -267,9 +270,14 @@ __device__ __forceinline__ void simt_body(const SimtParams& p, int block) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) out[i][j] = make_float2(0.f, 0.f);
 
-  const TileList list = simt_tiles(kQStat, m0, ON, n_strm, p);
+  const int key_sinks = !kQStat && p.far.sums ? 0 : p.sinks;   // first keys whose far queries are among this CTA's
+  TileList list = simt_tiles(kQStat, m0, ON, n_strm, p, key_sinks);
   int t_begin = 0, t_end = list.count;
   if (split > 1) split_range(begin_part, split, t_begin, t_end);
+  if (far) {
+    far_tiles(m0, ON, p.n_q, off, p.window, begin_part, p.far.parts, t_begin, t_end);
+    list.begin = 0;
+  }
   if (padding) t_end = t_begin;
   const float sl2 = p.scale * kLog2e;
 
@@ -294,12 +302,14 @@ __device__ __forceinline__ void simt_body(const SimtParams& p, int block) {
     bool masked = n0 + ON > n_strm;
     if (p.causal) {
       if (kQStat) masked = masked || n0 + ON - 1 > m0 + off || (p.window > 0 && m0 + OM - 1 + off - n0 >= p.window);
+      else if (far) masked = masked || n0 < m0 + OM - 1 - off + p.window;
       else masked = masked || n0 + off < m0 + OM - 1 || (p.window > 0 && n0 + ON - 1 + off - m0 >= p.window);
     }
     auto allowed = [&](int i, int j) {
       if (!masked) return true;
       const int r = m0 + 4 * ty + i, c = n0 + tx + 8 * j;
-      return c < n_strm && pair_visible(kQStat ? r : c, kQStat ? c : r, off, p.causal, p.window, p.sinks);
+      if (far) return c < n_strm && c + off - r >= p.window;   // (rows that are no first key are not stored)
+      return c < n_strm && pair_visible(kQStat ? r : c, kQStat ? c : r, off, p.causal, p.window, key_sinks);
     };
 
     float2 u0[4][4], u1[4][4];   // group 0: S, A2; group 1: dP, X
@@ -436,7 +446,21 @@ __device__ __forceinline__ void simt_body(const SimtParams& p, int block) {
   // Worked out again from the block number: kept in registers through the loop, these cost spills in it.
   uint32_t block_again;
   asm volatile("mov.u32 %0, %%ctaid.x;" : "=r"(block_again));
-  block_again -= kQStat ? 0 : p.q_blocks;
+  if (!kQStat && p.far.sums && m0 < p.sinks) {
+    // first keys: rows of fp32 sums, added up with the other parts
+    const int slot = block_again < static_cast<uint32_t>(p.far.blocks) ? 1 + static_cast<int>(block_again % p.far.parts) : 0;
+    const int cols = group == 0 ? d : dv, col = 4 * cx;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = m0 + 8 * ry + i;
+      if (r >= p.sinks) continue;
+      float* to = far_row(p.far, bh, slot, r, p.sinks, d + dv) + (group == 0 ? 0 : d);
+      if (col < cols) store4<float>(to, col, out[i][0], out[i][1], 1.f);
+      if (col + 64 < cols) store4<float>(to, col + 64, out[i][2], out[i][3], 1.f);
+    }
+    if (slot > 0) return;   // (no clusters in such a launch)
+  }
+  block_again -= p.far.blocks + (kQStat ? 0 : p.q_blocks);
   const bool live = block_again / split < static_cast<uint32_t>(kQStat ? p.items_q : p.items_k);
   const int part = static_cast<int>(block_again % split);
 
@@ -470,7 +494,7 @@ __device__ __forceinline__ void simt_body(const SimtParams& p, int block) {
         continue;
       }
       const int r = m0 + 8 * ry + i;
-      if (!live || r >= n_stat) continue;
+      if (!live || r >= n_stat || (!kQStat && p.far.sums && r < p.sinks)) continue;
       const size_t at = head + static_cast<size_t>(r) * cols + col;
       if (col < cols) store4<T>(first ? base0 : base1, at, out[i][0], out[i][1], mul);
       if (MODE != 5 && col + 64 < cols) store4<T>(first ? base0 : base1, at + 64, out[i][2], out[i][3], mul);
@@ -503,9 +527,9 @@ template <typename T, int MODE_Q, int MODE_K>
 __global__ void __launch_bounds__(NT, 1) simt_pass_kernel(const __grid_constant__ SimtParams p) {
   pdl_wait();
   if (threadIdx.x == 0) pdl_launch_dependents();
-  const int block = blockIdx.x;
-  if (block < p.q_blocks) simt_body<T, MODE_Q>(p, block);
-  else if constexpr (MODE_K != 0) simt_body<T, MODE_K>(p, block - p.q_blocks);
+  const int block = static_cast<int>(blockIdx.x) - p.far.blocks;
+  if (block >= 0 && block < p.q_blocks) simt_body<T, MODE_Q>(p, block, false);
+  else if constexpr (MODE_K != 0) simt_body<T, MODE_K>(p, block < 0 ? blockIdx.x : block - p.q_blocks, block < 0);
 }
 
 // O(N)-memory forward: online softmax.  A CTA owns OM = 64 queries and streams FN = 128 keys; a warp owns eight
@@ -556,7 +580,7 @@ __global__ void __launch_bounds__(NT, 1) simt_forward_kernel(const __grid_consta
   const size_t qoff = static_cast<size_t>(bh) * p.n_q * d, ooff = static_cast<size_t>(bh) * p.n_q * dv;
   const size_t koff = static_cast<size_t>(bh) * p.n_k * d, voff = static_cast<size_t>(bh) * p.n_k * dv;
   const int off = p.n_k - p.n_q;
-  const TileList list = simt_tiles(true, m0, FN, p.n_k, p);
+  const TileList list = simt_tiles(true, m0, FN, p.n_k, p, p.sinks);
   int t_begin = 0, t_end = list.count;
   if (split > 1) split_range(part, split, t_begin, t_end);
   if (!live) t_end = t_begin;
@@ -721,6 +745,7 @@ SimtParams make_params(const Problem& p) {
   s.q = p.q; s.k = p.k; s.v = p.v; s.d_o = p.d_o; s.ddq = p.ddq; s.ddk = p.ddk; s.ddv = p.ddv;
   s.dq2 = p.dq2; s.dk2 = p.dk2; s.dv2 = p.dv2; s.ddo = p.ddo;
   s.nlc = rv.nlc; s.k1 = rv.k1; s.ndd = rv.ndd; s.k23 = rv.k23;
+  s.far = FarWork{nullptr, 0, 0, 0};
   s.bh = p.bh; s.n_q = p.n_q; s.n_k = p.n_k; s.d = p.d; s.dv = head_dim_v(p); s.causal = p.causal; s.window = p.window; s.sinks = p.sinks; s.scale = p.scale;
   return s;
 }
@@ -750,8 +775,10 @@ int launch_modes(const Problem& problem, SimtParams& p, bool q_side, bool k_side
   p.split_q = g.split_q; p.split_k = g.split_k;
   p.cluster = g.cluster;
   p.q_blocks = g.q_blocks;
-  FHOB_CUDA_OK(launch_pdl(kernel, static_cast<unsigned>(g.blocks), NT, kSmem, g.cluster, st, p));
-  return FHOB_OK;
+  p.far = far_work(problem, !k_side || g.cluster > 1, OM);
+  if (g.blocks + p.far.blocks > 0x7fffffffLL) return FHOB_ERR_SHAPE;
+  FHOB_CUDA_OK(launch_pdl(kernel, static_cast<unsigned>(g.blocks + p.far.blocks), NT, kSmem, g.cluster, st, p));
+  return p.far.sums ? finish_first_keys(problem, p.dk2, p.dv2, st) : FHOB_OK;
 }
 
 // `pass` as in the entry points; passes 1 and 2 are one sweep, whichever is asked for

@@ -79,6 +79,7 @@ struct BwParams {
   int cluster;            // CTAs of a cluster (a multiple of both)
   int heads;              // heads per batch entry of the input tensor maps (4-D: columns, rows, head, batch)
   int d, d_v;             // columns in memory (<= the tile widths; see bw_launch)
+  FarWork far;            // of BK; its CTAs come in front of all others
   float scale;
 };
 
@@ -101,9 +102,10 @@ __device__ __forceinline__ void bw_split_pack(float x, float y, uint32_t& hi, ui
   lo = pack_bf16(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
 }
 
-// One half over one 128-row tile of one head; `block` numbers the (head, tile, part) triples.
+// One half over one 128-row tile of one head; `block` numbers the (head, tile, part) triples.  `far`: BK over a part of the
+// queries that see first keys behind their window.
 template <bool KSIDE, int DQK, int DV, bool F16, bool SPLIT>
-__device__ __forceinline__ void bw_body(const BwParams& p, int block) {
+__device__ __forceinline__ void bw_body(const BwParams& p, int block, bool far) {
   using C = BwCfg<KSIDE, DQK, DV, SPLIT>;
   static_assert(!SPLIT || (DQK == 128 && DV == 128 && !F16), "split fp32 operands are [hi(64) | lo(64)] bf16 rows");
   constexpr int BN = C::BN, CPT = BN / 2;   // CPT: columns of a score tile per elementwise thread
@@ -114,20 +116,23 @@ __device__ __forceinline__ void bw_body(const BwParams& p, int block) {
   int* status = p.status;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int split = KSIDE ? p.split_k : p.split_q;
-  const CtaWork work = cta_work(block, split, KSIDE ? p.items_k : p.items_q);   // the grid is padded to whole clusters
+  const int split = far ? 1 : (KSIDE ? p.split_k : p.split_q);
+  // the grid is padded to whole clusters
+  const CtaWork work = far ? cta_work(block, p.far.parts, p.far.blocks) : cta_work(block, split, KSIDE ? p.items_k : p.items_q);
   const int item = work.item, part = work.part;
   const bool live = work.live;
-  const int tiles_per_head = KSIDE ? p.tiles_k : p.tiles_q;
+  const int tiles_per_head = far ? p.far.tiles : (KSIDE ? p.tiles_k : p.tiles_q);
   const int head = item / tiles_per_head;
   const int tile_in_head = item - head * tiles_per_head;
   const int tile = KSIDE ? tile_in_head : tiles_per_head - 1 - tile_in_head;  // causal: longest first
   const int m0 = tile * BM;
   const int n_stat = KSIDE ? p.n_k : p.n_q, n_strm = KSIDE ? p.n_q : p.n_k;
   const int off = p.n_k - p.n_q;
-  const TileList list = streamed_tiles(!KSIDE, m0, BM, BN, n_strm, off, p.causal, p.window, p.sinks);
+  const int key_sinks = KSIDE && p.far.sums ? 0 : p.sinks;   // first keys whose far queries are among this CTA's
+  TileList list = streamed_tiles(!KSIDE, m0, BM, BN, n_strm, off, p.causal, p.window, key_sinks);
   int t_begin = 0, t_end = list.count;
   if (split > 1) split_range(part, split, t_begin, t_end);
+  if (far) far_tiles(m0, BN, p.n_q, off, p.window, part, p.far.parts, t_begin, t_end), list.begin = 0;
   const int n_iter = live ? t_end - t_begin : 0;
   auto stat_map = [&](int i) { return &p.map[KSIDE ? kBwK + i : kBwQ + i]; };   // Q, dO | K, V
   auto strm_map = [&](int i) { return &p.map[KSIDE ? kBwQ + i : kBwK + i]; };
@@ -319,7 +324,8 @@ __device__ __forceinline__ void bw_body(const BwParams& p, int block) {
       lo = p.causal ? g_row - off : 0;
       if (lo < 0) lo = 0;
       hi = p.n_q - 1;
-      if (p.window > 0 && g_row >= p.sinks && g_row - off + p.window - 1 < hi) hi = g_row - off + p.window - 1;
+      if (far) lo = max(lo, g_row - off + p.window);   // (rows that are no first key are not stored)
+      else if (p.window > 0 && g_row >= key_sinks && g_row - off + p.window - 1 < hi) hi = g_row - off + p.window - 1;
     }
     bool ok = true;
     constexpr int NC = CPT / 32;
@@ -414,6 +420,7 @@ __device__ __forceinline__ void bw_body(const BwParams& p, int block) {
         else masked = masked || (n0 + off < m0 + BM - 1);
         if (p.window > 0) {
           if (!KSIDE) masked = masked || (first ? n0 + BN > p.sinks : m0 + BM - 1 + off - n0 >= p.window || n0 < p.sinks);
+          else if (far) masked = masked || n0 < min(p.sinks, m0 + BM) - 1 - off + p.window;
           else masked = masked || (n0 + BN - 1 + off - m0 >= p.window);
         }
       }
@@ -431,6 +438,13 @@ __device__ __forceinline__ void bw_body(const BwParams& p, int block) {
       stage_row<C::W0 / 2, SPLIT>(dst + half * (C::W0 / 2), lane_base + half * (C::W0 / 2), n_iter > 0);
       if constexpr (KSIDE) stage_row<C::W1 / 2, SPLIT>(dst + C::W0 + half * (C::W1 / 2), lane_base + C::OUT0 + half * (C::W1 / 2), n_iter > 0);
     } else if (ok && live) {
+      const bool sums = KSIDE && p.far.sums && g_row < p.sinks;   // a first key: added up with the other parts
+      if (KSIDE && p.far.sums && m0 < p.sinks) {
+        float* dst = far_row(p.far, head, far ? 1 + part : 0, sums ? g_row : 0, p.sinks, p.d + p.d_v);
+        store_sums<C::W0 / 2, SPLIT>(dst, lane_base + half * (C::W0 / 2), half * (C::W0 / 2), p.d, n_iter > 0, sums);
+        if constexpr (KSIDE)
+          store_sums<C::W1 / 2, SPLIT>(dst + p.d, lane_base + C::OUT0 + half * (C::W1 / 2), half * (C::W1 / 2), p.d_v, n_iter > 0, sums);
+      }
       // `width` columns from TMEM column col0 on; dS was stored without the scale
       auto store_out = [&](auto width, int d_mem, uint32_t col0, void* base, float mul) {
         constexpr int W = decltype(width)::value;   // columns of the result; d_mem <= W of them exist in memory
@@ -439,7 +453,7 @@ __device__ __forceinline__ void bw_body(const BwParams& p, int block) {
         for (int c = half * (W / 2); c < (half + 1) * (W / 2); c += 16) {
           uint32_t v[16];
           load_result<SPLIT>(lane_base + col0 + c, n_iter > 0, v);
-          if (g_row >= n_stat) continue;
+          if (g_row >= n_stat || sums) continue;
           if constexpr (SPLIT) {
 #pragma unroll
             for (int j = 0; j < 16; j += 4)   // rows are whole 16-byte pieces
@@ -458,8 +472,10 @@ __device__ __forceinline__ void bw_body(const BwParams& p, int block) {
           }
         }
       };
-      store_out(std::integral_constant<int, C::W0>{}, p.d, 0, KSIDE ? p.dk : p.dq, p.scale);
-      if constexpr (KSIDE) store_out(std::integral_constant<int, C::W1>{}, p.d_v, C::OUT0, p.dv, 1.f);
+      if (!far) {
+        store_out(std::integral_constant<int, C::W0>{}, p.d, 0, KSIDE ? p.dk : p.dq, p.scale);
+        if constexpr (KSIDE) store_out(std::integral_constant<int, C::W1>{}, p.d_v, C::OUT0, p.dv, 1.f);
+      }
     }
   }
 
@@ -488,9 +504,9 @@ __device__ __forceinline__ void bw_body(const BwParams& p, int block) {
 
 template <int DQK, int DV, bool F16, bool SPLIT>
 __global__ void __launch_bounds__(NTHREADS, 1) bw_kernel(const __grid_constant__ BwParams p) {
-  const int block = blockIdx.x;
-  if (block < p.q_blocks) bw_body<false, DQK, DV, F16, SPLIT>(p, block);
-  else bw_body<true, DQK, DV, F16, SPLIT>(p, block - p.q_blocks);
+  const int block = static_cast<int>(blockIdx.x) - p.far.blocks;
+  if (block >= 0 && block < p.q_blocks) bw_body<false, DQK, DV, F16, SPLIT>(p, block, false);
+  else bw_body<true, DQK, DV, F16, SPLIT>(p, block < 0 ? blockIdx.x : block - p.q_blocks, block < 0);
 }
 
 // ------------------------------------------------------------------ host side
@@ -539,8 +555,10 @@ int bw_launch(const Problem& p, void* dq, void* dk, void* dv, cudaStream_t s) {
     tp.split_q = g.split_q; tp.split_k = g.split_k;
     tp.cluster = g.cluster;
     tp.q_blocks = g.q_blocks;
-    FHOB_CUDA_OK(launch_pdl(kernel, static_cast<unsigned>(g.blocks), NTHREADS, kSmem, g.cluster, s, tp));
-    return FHOB_OK;
+    tp.far = far_work(p, !k_side || tc_parts(true, p) > 1 || tc_parts(false, p) > 1, BM);
+    if (g.blocks + tp.far.blocks > 0x7fffffffLL) return FHOB_ERR_SHAPE;
+    FHOB_CUDA_OK(launch_pdl(kernel, static_cast<unsigned>(g.blocks + tp.far.blocks), NTHREADS, kSmem, g.cluster, s, tp));
+    return tp.far.sums ? finish_first_keys(p, dk, dv, s) : FHOB_OK;
   };
   if (!launch_apart(pair_grid(tp.items_q, tc_parts(true, p), tp.items_k, tc_parts(false, p)))) return go(true, true);
   const int first = go(true, false);

@@ -430,6 +430,40 @@ inline int tc_parts(bool q_stationary, const Problem& p) {
   return split_parts(((q_stationary ? p.n_q : p.n_k) + BM - 1) / BM, longest(q_stationary, q_stationary ? p.n_k : p.n_q, 64, BM, p.window, p.sinks));
 }
 
+// Which CTAs of a launch take the far queries of first keys: the first `blocks` of it (bh * tiles * parts).
+struct FarWork {
+  float* sums;              // NULL: none
+  int parts, tiles, blocks;
+};
+// (Where items are split, their CTAs share the far queries too.)
+inline FarWork far_work(const Problem& p, bool split, int rows) {
+  FarWork f = {nullptr, 0, 0, 0};
+  const int tiles = (p.sinks + rows - 1) / rows;
+  const long long blocks = static_cast<long long>(p.bh) * tiles * p.far_parts;
+  if (split || blocks == 0 || blocks > 0x3fffffffLL) return f;
+  f.sums = p.far_sums;
+  f.parts = p.far_parts;
+  f.tiles = tiles;
+  f.blocks = static_cast<int>(blocks);
+  return f;
+}
+// Row of sums (d + d_v floats) of key `row` of a head: slot 0 for the near queries, 1 + part for the far ones.
+__device__ __forceinline__ float* far_row(const FarWork& f, int head, int slot, int row, int sinks, int cols) {
+  return f.sums + ((static_cast<size_t>(head) * (f.parts + 1) + slot) * sinks + row) * cols;
+}
+// This thread's W fp32 result columns (TMEM addresses taddr..) of its row, those below d_mem, to a row of sums.
+template <int W, bool HALVES>
+__device__ __forceinline__ void store_sums(float* dst, uint32_t taddr, int c0, int d_mem, bool any, bool live) {
+#pragma unroll
+  for (int c = 0; c < W; c += 16) {
+    uint32_t v[16];
+    load_result<HALVES>(taddr + c, any, v);
+#pragma unroll
+    for (int j = 0; j < 16; j += 4)
+      if (live && c0 + c + j < d_mem) *reinterpret_cast<uint4*>(dst + c0 + c + j) = make_uint4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+  }
+}
+
 }  // namespace
 
 // Grid of a launch that holds query-tiled and key-tiled CTAs (of which either may have none): the CTAs of

@@ -129,6 +129,7 @@ struct TcParams {
   int heads;              // heads per batch entry of the input tensor maps (4-D: columns, rows, head, batch)
   int d, d_v;             // columns in memory (<= the tile widths DQK, DV; see fill_params)
   int first_live;         // first query with a visible key (causal, n_k < n_q)
+  FarWork far;            // of pass 4; its CTAs come in front of all others
   float scale;
 };
 
@@ -422,9 +423,9 @@ __device__ __forceinline__ float row_dot(const void* o, const void* d_o, int c0,
 
 // One pass over one 128-row tile of one head; `block` numbers the (head, tile, part) triples of the pass.
 // With few tiles a head the streamed axis is split over the CTAs of a cluster (see split_parts); each computes its
-// part's sums and the cluster adds them up.
+// part's sums and the cluster adds them up.  `far`: pass 4 over a part of the queries that see first keys behind their window.
 template <int PASS, int DQK, int DV, int BN, int FUSED, bool F16, bool SPLIT>
-__device__ __forceinline__ void tc_pass_body(const TcParams& p, int block) {
+__device__ __forceinline__ void tc_pass_body(const TcParams& p, int block, bool far = false) {
   static_assert(FUSED == 0 || PASS == 2, "only pass 2 has a fused form");
   static_assert(!SPLIT || (DQK == 128 && DV == 128 && !F16), "split fp32 operands are [hi(64) | lo(64)] bf16 rows");
   using C = Cfg<PASS, DQK, DV, BN>;
@@ -439,9 +440,10 @@ __device__ __forceinline__ void tc_pass_body(const TcParams& p, int block) {
   Bars* bars = reinterpret_cast<Bars*>(strm_tiles + C::NSLOT * C::SLOT_BYTES);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int tiles_per_head = kQStat ? p.tiles_q : p.tiles_k;
-  const int split = kQStat ? p.split_q : p.split_k;
-  const CtaWork work = cta_work(block, split, kQStat ? p.items_q : p.items_k);   // the grid is padded to whole clusters
+  const int tiles_per_head = far ? p.far.tiles : (kQStat ? p.tiles_q : p.tiles_k);
+  const int split = far ? 1 : (kQStat ? p.split_q : p.split_k);
+  // the grid is padded to whole clusters
+  const CtaWork work = far ? cta_work(block, p.far.parts, p.far.blocks) : cta_work(block, split, kQStat ? p.items_q : p.items_k);
   const int item = work.item, part = work.part;
   const bool live = work.live;
   const int head = item / tiles_per_head;
@@ -453,9 +455,14 @@ __device__ __forceinline__ void tc_pass_body(const TcParams& p, int block) {
   const int n_strm = kQStat ? p.n_k : p.n_q;
   const int off = p.n_k - p.n_q;
 
-  const TileList list = streamed_tiles(kQStat, m0, BM, BN, n_strm, off, p.causal, p.window, p.sinks);
+  const int key_sinks = !kQStat && p.far.sums ? 0 : p.sinks;   // first keys whose far queries are among this CTA's
+  TileList list = streamed_tiles(kQStat, m0, BM, BN, n_strm, off, p.causal, p.window, key_sinks);
   int t_begin = 0, t_end = list.count;
   if (split > 1) split_range(part, split, t_begin, t_end);
+  if (far) {
+    far_tiles(m0, BN, p.n_q, off, p.window, part, p.far.parts, t_begin, t_end);
+    list.begin = 0;
+  }
   const int n_iter = live ? t_end - t_begin : 0;
 
   auto stat_map = [&](int i) { return &p.map[kQStat ? kMapQ + i : kMapK + i]; };   // Q, ddQ, dO | K, ddK, V, ddV
@@ -759,7 +766,8 @@ __device__ __forceinline__ void tc_pass_body(const TcParams& p, int block) {
       c.lo = p.causal ? g_row - off : 0;
       if (c.lo < 0) c.lo = 0;
       c.hi = p.n_q - 1;
-      if (p.window > 0 && g_row >= p.sinks && g_row - off + p.window - 1 < c.hi) c.hi = g_row - off + p.window - 1;
+      if (far) c.lo = max(c.lo, g_row - off + p.window);   // (rows that are no first key are not stored)
+      else if (p.window > 0 && g_row >= key_sinks && g_row - off + p.window - 1 < c.hi) c.hi = g_row - off + p.window - 1;
     }
     [[maybe_unused]] const int row_lo = c.lo, row_hi = c.hi;
     float2 racc[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -781,6 +789,7 @@ __device__ __forceinline__ void tc_pass_body(const TcParams& p, int block) {
         if (p.window > 0) {
           // the pair of the tile that is furthest apart: last query row against first key row
           if (kQStat) masked = masked || (first ? n0 + BN > p.sinks : m0 + BM - 1 + off - n0 >= p.window || n0 < p.sinks);
+          else if (far) masked = masked || n0 < min(p.sinks, m0 + BM) - 1 - off + p.window;
           else masked = masked || (n0 + BN - 1 + off - m0 >= p.window);
         }
       }
@@ -905,6 +914,14 @@ __device__ __forceinline__ void tc_pass_body(const TcParams& p, int block) {
           stage_row<DV / 2>(dst + DQK + half * (DV / 2), acc + C::OUT0_COLS + half * (DV / 2), n_iter > 0);
         }
       } else if (ok && live) {   // a CTA that only fills up a cluster has no tile to store
+        const bool sums = !kQStat && p.far.sums && g_row < p.sinks;   // a first key: added up with the other parts
+        if (!kQStat && p.far.sums && m0 < p.sinks) {
+          constexpr int W0 = SPLIT ? 64 : DQK, W1 = SPLIT ? 64 : DV;
+          float* dst = far_row(p.far, head, far ? 1 + part : 0, sums ? g_row : 0, p.sinks, p.d + p.d_v);
+          const uint32_t acc = tmem_base + lane_base;
+          store_sums<W0 / 2, SPLIT>(dst, acc + half * (W0 / 2), half * (W0 / 2), p.d, n_iter > 0, sums);
+          store_sums<W1 / 2, SPLIT>(dst + p.d, acc + C::OUT0_COLS + half * (W1 / 2), half * (W1 / 2), p.d_v, n_iter > 0, sums);
+        }
         auto store_out = [&](auto width, int d_mem, uint32_t col0, void* base, float mul) {
           constexpr int DO = decltype(width)::value;   // columns of the accumulator; d_mem <= DO of them exist in memory
           uint16_t* dst = static_cast<uint16_t*>(base) + (static_cast<size_t>(head) * n_stat + (g_row < n_stat ? g_row : 0)) * d_mem + half * (DO / 2);
@@ -918,7 +935,7 @@ __device__ __forceinline__ void tc_pass_body(const TcParams& p, int block) {
 #pragma unroll
               for (int j = 0; j < 16; ++j) v[j] = 0u;
             }
-            if (g_row < n_stat) {
+            if (g_row < n_stat && !sums) {
               uint32_t w[8];
 #pragma unroll
               for (int j = 0; j < 8; ++j)
@@ -945,7 +962,7 @@ __device__ __forceinline__ void tc_pass_body(const TcParams& p, int block) {
 #pragma unroll
               for (int j = 0; j < 16; ++j) a[j] = b[j] = 0u;
             }
-            if (g_row < n_stat) {
+            if (g_row < n_stat && !sums) {
               float4* d4 = reinterpret_cast<float4*>(dst + 16 * ch);
 #pragma unroll
               for (int j = 0; j < 4; ++j)
@@ -959,7 +976,8 @@ __device__ __forceinline__ void tc_pass_body(const TcParams& p, int block) {
         };
         // dS and dS2 were stored without the factor `scale`: it is applied to dQ2 | dK2 here
         void *out0 = kQStat ? p.dq2 : p.dk2, *out1 = kQStat ? p.ddo : p.dv2;
-        if constexpr (SPLIT) {
+        if (far) {
+        } else if constexpr (SPLIT) {
           store_out_split(p.d, 0, out0, c.scale);
           store_out_split(p.d_v, C::OUT0_COLS, out1, 1.f);
         } else {
@@ -1022,9 +1040,9 @@ __global__ void __launch_bounds__(NTHREADS, 1) tc_pass_kernel(const __grid_const
 // SMs that run out of pass-3 work (and a small problem runs both side by side).
 template <int DQK, int DV, bool F16, bool SPLIT>
 __global__ void __launch_bounds__(NTHREADS, 1) tc_pass34_kernel(const __grid_constant__ TcParams p) {
-  const int block = blockIdx.x;
-  if (block < p.q_blocks) tc_pass_body<3, DQK, DV, 64, 0, F16, SPLIT>(p, block);
-  else tc_pass_body<4, DQK, DV, 64, 0, F16, SPLIT>(p, block - p.q_blocks);
+  const int block = static_cast<int>(blockIdx.x) - p.far.blocks;
+  if (block >= 0 && block < p.q_blocks) tc_pass_body<3, DQK, DV, 64, 0, F16, SPLIT>(p, block);
+  else tc_pass_body<4, DQK, DV, 64, 0, F16, SPLIT>(p, block < 0 ? blockIdx.x : block - p.q_blocks, block < 0);
 }
 
 // ------------------------------------------------------------------ host side
@@ -1110,6 +1128,7 @@ int fill_params(const Problem& p, TcParams& tp) {
   tp.d = p.d;
   tp.d_v = dv;
   tp.first_live = first_live_query(p);
+  tp.far = FarWork{nullptr, 0, 0, 0};
   return FHOB_OK;
 }
 
@@ -1144,7 +1163,9 @@ int launch_34(const Problem& p, TcParams& tp, bool pass3, bool pass4, cudaStream
   tp.split_q = g.split_q; tp.split_k = g.split_k;
   tp.cluster = g.cluster;
   tp.q_blocks = g.q_blocks;
-  return launch(kernel, tp, g.blocks, kSmem, s);
+  tp.far = far_work(p, !pass4 || tc_parts(true, p) > 1 || tc_parts(false, p) > 1, BM);
+  const int st = launch(kernel, tp, g.blocks + tp.far.blocks, kSmem, s);
+  return st == FHOB_OK && tp.far.sums ? finish_first_keys(p, p.dk2, p.dv2, s) : st;
 }
 
 // `pass`: 1, 2, 3, 4 alone, 12 = passes 1 and 2 in one sweep, kWholeOperator = the sweep, then passes 3 and 4

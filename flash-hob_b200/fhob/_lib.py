@@ -18,7 +18,7 @@ SYMBOLS = (
     "fhob_read_status", "fhob_forward", "fhob_backward", "fhob_bwdbwd_static_scratch",
     "fhob_selftest_expired_wait", "fhob_visible_tiles", "fhob_static_scratch_status",
     "fhob_workspace_bytes_problem", "fhob_cta_work",
-    "fhob_visible_tiles_sinks", "fhob_bwdbwd_sinks", "fhob_forward_sinks", "fhob_backward_sinks",
+    "fhob_visible_tiles_sinks", "fhob_workspace_bytes_sinks", "fhob_bwdbwd_sinks", "fhob_forward_sinks", "fhob_backward_sinks",
     "fhob_rotary", "fhob_layer_norm", "fhob_layer_norm_backward", "fhob_layer_norm_bwdbwd",
     "fhob_layer_norm_workspace_bytes",
 )
@@ -111,6 +111,8 @@ def load() -> C.CDLL:
     lib.fhob_static_scratch_status.argtypes = [C.c_void_p]
     lib.fhob_forward.restype = C.c_int
     lib.fhob_forward.argtypes = [P, C.c_void_p, C.c_void_p, C.c_void_p]
+    lib.fhob_workspace_bytes_sinks.restype = C.c_size_t
+    lib.fhob_workspace_bytes_sinks.argtypes = [P, C.c_int32]
     lib.fhob_visible_tiles_sinks.restype = C.c_int
     lib.fhob_visible_tiles_sinks.argtypes = [C.c_int] * 8 + [C.POINTER(C.c_int)] * 3
     lib.fhob_bwdbwd_sinks.restype = C.c_int

@@ -190,7 +190,7 @@ class _Problem:
         if workspace is None:
             # what lets the library take its fastest path (fp32 with head dim 64: room for the bf16
             # hi/lo copies of the inputs, so that the problem runs on the tensor cores)
-            self.ws = _workspace(dev, self.stream, lib.fhob_workspace_bytes_problem(C.byref(p)))
+            self.ws = _workspace(dev, self.stream, lib.fhob_workspace_bytes_sinks(C.byref(p), self.sinks))
         else:
             nbytes = lib.fhob_workspace_bytes(bh, n_q)
             if (workspace.device != dev or workspace.dtype != torch.uint8 or not workspace.is_contiguous()
@@ -400,7 +400,9 @@ def _run_host(mats, L, scale, is_causal, impl, check, dev, window=None, out=None
     sizing.bh, sizing.n_q, sizing.n_k, sizing.d = widest, mats3[0].shape[1], mats3[1].shape[1], mats3[0].shape[2]
     sizing.d_v = 0 if mats3[2].shape[2] == mats3[0].shape[2] else mats3[2].shape[2]
     sizing.dtype, sizing.impl = _lib.DTYPES[str(mats3[0].dtype)], _lib.IMPL[impl]
-    ws = _workspace(dev, main.cuda_stream, _lib.load().fhob_workspace_bytes_problem(C.byref(sizing)))
+    sizing.causal, sizing.window = (1 if is_causal else 0), _window(is_causal, window)
+    ws = _workspace(dev, main.cuda_stream,
+                    _lib.load().fhob_workspace_bytes_sinks(C.byref(sizing), _sinks(sizing.window, sinks)))
     # Device staging: a ring of HOST_STAGES sets of buffers (nine inputs and four results of the widest
     # range), kept per device and shape, so that a call allocates nothing on the device and the
     # pipeline's timing does not depend on the state of the caching allocator.  Set s is reused by

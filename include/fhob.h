@@ -292,7 +292,13 @@ int fhob_backward(const FhobProblem* p, void* dq, void* dk, void* dv, void* stre
  * j < sink_tokens).  sink_tokens = 0 is the call without it; sink_tokens < 0, or
  * > 0 without a window, FHOB_ERR_ARG.  A forward's L and O go with a backward of
  * the same window and sink_tokens.  The reference has no counterpart.
+ *
+ * With a workspace of fhob_workspace_bytes_sinks() bytes the backward calls cut
+ * the queries that see the first keys behind their window into parts that run
+ * side by side, with fhob_workspace_bytes_problem() bytes one CTA goes through
+ * them all (slower, other orders of sums).
  */
+size_t fhob_workspace_bytes_sinks(const FhobProblem* p, int32_t sink_tokens);
 int fhob_bwdbwd_sinks(const FhobProblem* p, int32_t sink_tokens, void* stream);
 int fhob_forward_sinks(const FhobProblem* p, int32_t sink_tokens, void* o_out, float* lse_out, void* stream);
 int fhob_backward_sinks(const FhobProblem* p, int32_t sink_tokens, void* dq, void* dk, void* dv, void* stream);
