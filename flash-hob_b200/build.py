@@ -23,7 +23,7 @@ OUT = HERE / "fhob" / "libfhob.so"
 NATIVE = HERE / "fhob" / "_native.so"          # host path of the Python package, against torch's C++ API
 NATIVE_SOURCES = ["host_binding.cpp", "host_layer.cpp"]
 SOURCES = ["fhob_api.cu", "simt_kernels.cu", "tc_kernels.cu", "tc_forward.cu", "tc_backward.cu", "static_scratch.cu",
-           "rotary.cu", "layer_norm.cu"]
+           "token_forward.cu", "rotary.cu", "layer_norm.cu"]
 HEADERS = ["fhob_common.cuh", "sm100_ptx.cuh", "tc_common.cuh", "../../include/fhob.h"]
 FLAGS = ["-Xcompiler", "-fPIC", "-O3", "-std=c++17", "-lineinfo", "-gencode", "arch=compute_100a,code=sm_100a"]
 

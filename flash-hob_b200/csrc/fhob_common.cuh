@@ -260,6 +260,9 @@ int tc_operator(const Problem& p, cudaStream_t s);   // the whole double backwar
 bool tc_first_order_supported(const FhobProblem& p);
 int tc_forward(const Problem& p, void* o_out, float* lse_out, int* status, cudaStream_t s);
 int tc_backward(const Problem& p, void* dq, void* dk, void* dv, cudaStream_t s);
+// a few queries against a window and first keys: token_forward.cu
+bool token_supported(const Problem& p, const void* o_out);
+int token_forward(const Problem& p, void* o_out, float* lse_out, int* status, cudaStream_t s);
 int tc_selftest_expired_wait(int* status, cudaStream_t s);
 
 }  // namespace fhob

@@ -1,0 +1,297 @@
+// Forward of a few queries (one token a sequence, or a handful) against a window and first keys: O and the logsumexp.
+//
+//   s_j = scale q . k_j,  O = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),  L = m + log sum_j exp(s_j - m)
+//
+// What bounds it: every visible key and value is read once for up to eight queries, so the memory: 128 heads of one query,
+// W = 1024 and 4 first keys, D = 128 read 67 MB.  The tensor-core forward has 128-row query tiles and goes through a head
+// in one CTA, tile after tile: 26 us there.  Here
+//  - the lanes of a group (16 for rows of 256 bytes) read one key's row, 16 bytes a lane: a product takes a few shuffles.  Each
+//    group goes through keys of its own with a running maximum and sum of its own: groups, warps and CTAs meet at the end;
+//  - a group takes kBatch keys at a time: their rows of K and V are all on their way before the first is used;
+//  - a head's keys are shared by the CTAs of a cluster, at least 128 a CTA and up to 8 of them: a number that depends on the
+//    lengths alone, as the order in which their results are added up.
+#include "tc_common.cuh"
+
+namespace fhob {
+namespace {
+
+constexpr int TK_WARPS = 4, TK_THREADS = 32 * TK_WARPS;
+
+struct TkParams {
+  const void *q, *k, *v;
+  void* o;             // NULL: L alone
+  float* lse;
+  int* status;
+  View vq, vk, vv;
+  int n_q, n_k, d, d_v, window, sinks;
+  int first, count;    // keys that any query sees: 0 .. sinks - 1, then first .. first + count - sinks - 1
+  float sl2;           // scale * log2(e)
+};
+
+template <class T>
+struct Lane {   // 16 bytes of a row
+  static constexpr int V = 16 / sizeof(T);
+  static __device__ __forceinline__ void unpack(const uint4& w, float2 (&x)[V / 2]) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    if constexpr (sizeof(T) == 4) {
+      x[0] = f2(u[0], u[1]);
+      x[1] = f2(u[2], u[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, __half>::value) x[i] = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+        else x[i] = make_float2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
+      }
+    }
+  }
+};
+
+// Puts the results of two sets of keys on a common maximum: (m, l, a) += (m2, l2, a2).
+template <int H>
+__device__ __forceinline__ void merge(float& m, float& l, float2 (&a)[H], float m2, float l2, const float2 (&a2)[H]) {
+  const float top = fmaxf(m, m2);
+  // (no maximum but a sum: NaN is kept)
+  const float w1 = m == -INFINITY ? 1.f : ex2(m - top), w2 = m2 == -INFINITY ? 1.f : ex2(m2 - top);
+  // a side without a sum has nothing to add: its weight may be anything
+  const bool none1 = l == 0.f, none2 = l2 == 0.f;
+  l = (none1 ? 0.f : l * w1) + (none2 ? 0.f : l2 * w2);
+#pragma unroll
+  for (int h = 0; h < H; ++h) {
+    const float2 x = none1 ? make_float2(0.f, 0.f) : make_float2(a[h].x * w1, a[h].y * w1);
+    const float2 y = none2 ? make_float2(0.f, 0.f) : make_float2(a2[h].x * w2, a2[h].y * w2);
+    a[h] = __fadd2_rn(x, y);
+  }
+  m = top;
+}
+
+// G lanes a key, R queries
+template <class T, int G, int R>
+__global__ void __launch_bounds__(TK_THREADS) token_kernel(const __grid_constant__ TkParams p, int parts) {
+  constexpr int V = Lane<T>::V, H = V / 2, kGroups = 32 / G, kBatch = R > 2 ? 4 : 8;
+  constexpr int kPitch = G * V + 4;   // floats of a staged row: O, maximum, sum
+  __shared__ float staged[TK_WARPS][R][kPitch];
+  pdl_wait();
+  if (threadIdx.x == 0) {
+    pdl_launch_dependents();
+    if (blockIdx.x == 0 && p.status) *p.status = 0;   // every call starts clean
+  }
+  const int head = blockIdx.x / parts, part = blockIdx.x - head * parts;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = lane / G, at = (lane % G) * V;
+  const int hb = head / p.vk.heads, hh = head - hb * p.vk.heads;
+  auto base = [&](const void* x, const View& v) { return static_cast<const T*>(x) + hb * v.batch + hh * v.head + at; };
+  const T *q = base(p.q, p.vq), *k = base(p.k, p.vk), *v = base(p.v, p.vv);
+  const bool in_k = at < p.d, in_v = at < p.d_v && p.o;
+  const int off = p.n_k - p.n_q;
+
+  float2 qs[R][H], acc[R][H];
+  float m[R], l[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    uint4 w = make_uint4(0u, 0u, 0u, 0u);
+    if (in_k && r < p.n_q) w = *reinterpret_cast<const uint4*>(q + r * p.vq.row);
+    Lane<T>::unpack(w, qs[r]);
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int h = 0; h < H; ++h) acc[r][h] = make_float2(0.f, 0.f);
+  }
+
+  // this group's keys: every streams-th one of the part's, counted over first keys and window
+  const int begin = static_cast<int>(static_cast<long long>(p.count) * part / parts);
+  const int end = static_cast<int>(static_cast<long long>(p.count) * (part + 1) / parts);
+  constexpr int kStreams = TK_WARPS * kGroups;
+  for (int x0 = begin; x0 < end; x0 += kStreams * kBatch) {   // (the same number of rounds for all: the shuffles are the warp's)
+    uint4 kw[kBatch], vw[kBatch];
+    int key[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int x = x0 + (u * TK_WARPS + warp) * kGroups + group;
+      key[u] = x >= end ? -1 : (x < p.sinks ? x : p.first + x - p.sinks);
+      kw[u] = vw[u] = make_uint4(0u, 0u, 0u, 0u);
+      if (key[u] >= 0 && in_k) kw[u] = *reinterpret_cast<const uint4*>(k + key[u] * p.vk.row);
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+      if (key[u] >= 0 && in_v) vw[u] = *reinterpret_cast<const uint4*>(v + key[u] * p.vv.row);
+    float s[R][kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      float2 ks[H];
+      Lane<T>::unpack(kw[u], ks);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float2 dot = __fmul2_rn(qs[r][0], ks[0]);
+#pragma unroll
+        for (int h = 1; h < H; ++h) dot = __ffma2_rn(qs[r][h], ks[h], dot);
+        s[r][u] = dot.x + dot.y;
+      }
+    }
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1)
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u)
+#pragma unroll
+        for (int r = 0; r < R; ++r) s[r][u] += __shfl_xor_sync(0xffffffffu, s[r][u], o);
+    uint32_t hidden[R];   // bit u: key u of the batch, for a query that others share it with
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float top = m[r];
+      hidden[r] = 0u;
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const bool seen = key[u] >= 0 && r < p.n_q && pair_visible(r, key[u], off, 1, p.window, p.sinks);
+        s[r][u] = seen ? s[r][u] * p.sl2 : -INFINITY;
+        if (R > 1 && !seen) hidden[r] |= 1u << u;
+        top = fmaxf(top, s[r][u]);
+      }
+      const float from = top == -INFINITY ? 0.f : top;   // no maximum yet: 0 for hidden keys, NaN for NaN scores
+      const float alpha = m[r] == -INFINITY ? 1.f : ex2(m[r] - from);
+      m[r] = top;
+      float sum = 0.f;
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        s[r][u] = ex2(s[r][u] - from);
+        sum += s[r][u];
+      }
+      l[r] = fmaf(l[r], alpha, sum);
+#pragma unroll
+      for (int h = 0; h < H; ++h) acc[r][h] = __fmul2_rn(acc[r][h], make_float2(alpha, alpha));
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      float2 vs[H];
+      Lane<T>::unpack(vw[u], vs);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          // a hidden key's value may be anything
+          const float2 x = R > 1 && (hidden[r] >> u & 1u) ? make_float2(0.f, 0.f) : vs[h];
+          acc[r][h] = __ffma2_rn(make_float2(s[r][u], s[r][u]), x, acc[r][h]);
+        }
+    }
+  }
+
+  // groups of the warp, then warps, then the CTAs of the cluster
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+#pragma unroll
+    for (int o = G; o < 32; o <<= 1) {
+      float2 a2[H];
+      const float m2 = __shfl_xor_sync(0xffffffffu, m[r], o), l2 = __shfl_xor_sync(0xffffffffu, l[r], o);
+#pragma unroll
+      for (int h = 0; h < H; ++h) a2[h] = make_float2(__shfl_xor_sync(0xffffffffu, acc[r][h].x, o), __shfl_xor_sync(0xffffffffu, acc[r][h].y, o));
+      // both sides of a pair add up in the same order
+      if (lane & o) {
+        float mm = m2, ll = l2;
+        merge<H>(mm, ll, a2, m[r], l[r], acc[r]);
+        m[r] = mm;
+        l[r] = ll;
+#pragma unroll
+        for (int h = 0; h < H; ++h) acc[r][h] = a2[h];
+      } else {
+        merge<H>(m[r], l[r], acc[r], m2, l2, a2);
+      }
+    }
+    if (group == 0) {
+      float* to = &staged[warp][r][at];
+#pragma unroll
+      for (int h = 0; h < H; ++h) *reinterpret_cast<float2*>(to + 2 * h) = acc[r][h];
+      if (at == 0) {
+        staged[warp][r][G * V] = m[r];
+        staged[warp][r][G * V + 1] = l[r];
+      }
+    }
+  }
+  if (parts > 1) cluster_sync();
+  else __syncthreads();
+  // part `part` finishes every parts-th row; a warp a row
+  for (int r = part + parts * warp; r < p.n_q; r += parts * TK_WARPS) {
+    constexpr int kMine = (G * V + 63) / 64;   // pairs of columns of a lane
+    float mt = -INFINITY, lt = 0.f;
+    float2 a[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) a[i] = make_float2(0.f, 0.f);
+    for (int c = 0; c < parts; ++c)
+      for (int w = 0; w < TK_WARPS; ++w) {
+        const uint32_t from = smem_u32(&staged[w][r][0]);
+        const uint32_t there = parts > 1 ? cluster_map(from, c) : from;
+        auto load = [&](int i) { return parts > 1 ? cluster_ld(there + 4 * i) : staged[w][r][i]; };
+        float2 b[kMine];
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          const int col = 2 * lane + 64 * i;
+          b[i] = col < G * V ? make_float2(load(col), load(col + 1)) : make_float2(0.f, 0.f);
+        }
+        merge<kMine>(mt, lt, a, load(G * V), load(G * V + 1), b);
+      }
+    const size_t row = static_cast<size_t>(head) * p.n_q + r;
+    if (lane == 0) p.lse[row] = lt == 0.f ? -INFINITY : (mt + log2f(lt)) * 0.6931471805599453f;
+    if (p.o) {
+      const float inv = lt == 0.f ? 0.f : 1.f / lt;
+      T* o = static_cast<T*>(p.o) + row * p.d_v;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int col = 2 * lane + 64 * i;
+        if (col < p.d_v) {   // an even number of columns
+          o[col] = static_cast<T>(a[i].x * inv);
+          o[col + 1] = static_cast<T>(a[i].y * inv);
+        }
+      }
+    }
+  }
+  if (parts > 1) cluster_sync();   // the others are done with this CTA's shared memory
+}
+
+template <class T>
+int token_launch(const TkParams& p, int heads, int parts, cudaStream_t s) {
+  const int pieces = ((p.d > p.d_v ? p.d : p.d_v) * static_cast<int>(sizeof(T)) + 15) / 16;
+  auto go = [&](auto lanes, auto rows) -> int {
+    constexpr auto kernel = token_kernel<T, decltype(lanes)::value, decltype(rows)::value>;
+    FHOB_CUDA_OK(launch_pdl(kernel, static_cast<unsigned>(heads * parts), TK_THREADS, 0, parts, s, p, parts));
+    return FHOB_OK;
+  };
+  auto rows = [&](auto lanes) -> int {
+    if (p.n_q == 1) return go(lanes, std::integral_constant<int, 1>{});
+    if (p.n_q == 2) return go(lanes, std::integral_constant<int, 2>{});
+    return p.n_q <= 4 ? go(lanes, std::integral_constant<int, 4>{}) : go(lanes, std::integral_constant<int, 8>{});
+  };
+  if (pieces <= 4) return rows(std::integral_constant<int, 4>{});
+  if (pieces <= 8) return rows(std::integral_constant<int, 8>{});
+  return pieces <= 16 ? rows(std::integral_constant<int, 16>{}) : rows(std::integral_constant<int, 32>{});
+}
+
+}  // namespace
+
+// Rows of whole 16-byte pieces at 16-byte addresses and strides.  (Calls without first keys keep the kernels they had.)
+bool token_supported(const Problem& p, const void* o_out) {
+  const int es = p.dtype == FHOB_F32 ? 4 : 2, d_v = head_dim_v(p);
+  const uintptr_t all = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) |
+                        static_cast<uintptr_t>(p.d * es) | static_cast<uintptr_t>(d_v * es);
+  return p.sinks > 0 && p.n_q <= 8 && (all & 15u) == 0 && (reinterpret_cast<uintptr_t>(o_out) & 3u) == 0 && p.d <= 128 && d_v <= 128 &&
+         static_cast<long long>(p.bh) * 8 <= 0x7fffffffLL;
+}
+
+int token_forward(const Problem& p, void* o_out, float* lse_out, int* status, cudaStream_t s) {
+  TkParams t;
+  const int d_v = head_dim_v(p);
+  t.q = p.q; t.k = p.k; t.v = p.v;
+  t.o = o_out;
+  t.lse = lse_out;
+  t.status = status;
+  t.vq = tensor_view(p, kTenQ, p.n_q, p.d);
+  t.vk = tensor_view(p, kTenK, p.n_k, p.d);
+  t.vv = tensor_view(p, kTenV, p.n_k, d_v);
+  t.n_q = p.n_q; t.n_k = p.n_k; t.d = p.d; t.d_v = d_v; t.window = p.window; t.sinks = p.sinks;
+  // the first query's window starts earliest; query i sees up to key i + n_k - n_q
+  const int first = p.n_k - p.n_q - p.window + 1;
+  t.first = first > p.sinks ? first : p.sinks;
+  t.count = p.sinks + p.n_k - t.first;
+  t.sl2 = p.scale * kLog2e;
+  int parts = (t.count + 127) / 128;
+  if (parts > 8) parts = 8;
+  if (p.dtype == FHOB_F32) return token_launch<float>(t, p.bh, parts, s);
+  return p.dtype == FHOB_F16 ? token_launch<__half>(t, p.bh, parts, s) : token_launch<__nv_bfloat16>(t, p.bh, parts, s);
+}
+
+}  // namespace fhob
