@@ -5,17 +5,17 @@
 // What bounds it: every visible key and value is read once for up to eight queries, so the memory: 128 heads of one query,
 // W = 1024 and 4 first keys, D = 128 read 67 MB.  The tensor-core forward has 128-row query tiles and goes through a head
 // in one CTA, tile after tile: 26 us there.  Here
-//  - the lanes of a group (16 for rows of 256 bytes) read one key's row, 16 bytes a lane: a product takes a few shuffles.  Each
-//    group goes through keys of its own with a running maximum and sum of its own: groups, warps and CTAs meet at the end;
-//  - a group takes kBatch keys at a time: their rows of K and V are all on their way before the first is used;
-//  - a head's keys are shared by the CTAs of a cluster, at least 128 a CTA and up to 8 of them: a number that depends on the
+//  - eight lanes read one key's row, one, two or four times 16 bytes a lane: a product takes three shuffles.  Each such group goes
+//    through keys of its own with a running maximum and sum of its own: groups, warps and CTAs meet at the end;
+//  - a group takes four keys at a time: their rows of K and V are all on their way before the first is used.  What counts besides is
+//    the number of instructions, since a call of few heads has one warp a scheduler: with 16 lanes a key, 51 a key and warp
+//    (and a ring of asynchronous copies, which gained nothing), now about 20;
+//  - a head's keys are shared by the CTAs of a cluster, four batches a CTA and up to 8 CTAs: a number that depends on the
 //    lengths alone, as the order in which their results are added up.
 #include "tc_common.cuh"
 
 namespace fhob {
 namespace {
-
-constexpr int TK_WARPS = 4, TK_THREADS = 32 * TK_WARPS;
 
 struct TkParams {
   const void *q, *k, *v;
@@ -28,10 +28,12 @@ struct TkParams {
   float sl2;           // scale * log2(e)
 };
 
+constexpr int TK_LANES = 8, TK_GROUPS = 32 / TK_LANES, TK_BATCH = 4;
+
 template <class T>
 struct Lane {   // 16 bytes of a row
   static constexpr int V = 16 / sizeof(T);
-  static __device__ __forceinline__ void unpack(const uint4& w, float2 (&x)[V / 2]) {
+  static __device__ __forceinline__ void unpack(const uint4& w, float2* x) {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
     if constexpr (sizeof(T) == 4) {
       x[0] = f2(u[0], u[1]);
@@ -45,6 +47,13 @@ struct Lane {   // 16 bytes of a row
     }
   }
 };
+
+// A load that stays where it is written: the compiler would move those of a batch to their uses, one behind the other.
+__device__ __forceinline__ uint4 load16(const void* from) {
+  uint4 w;
+  asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "l"(from) : "memory");
+  return w;
+}
 
 // Puts the results of two sets of keys on a common maximum: (m, l, a) += (m2, l2, a2).
 template <int H>
@@ -64,32 +73,35 @@ __device__ __forceinline__ void merge(float& m, float& l, float2 (&a)[H], float 
   m = top;
 }
 
-// G lanes a key, R queries
-template <class T, int G, int R>
-__global__ void __launch_bounds__(TK_THREADS) token_kernel(const __grid_constant__ TkParams p, int parts) {
-  constexpr int V = Lane<T>::V, H = V / 2, kGroups = 32 / G, kBatch = R > 2 ? 4 : 8;
-  constexpr int kPitch = G * V + 4;   // floats of a staged row: O, maximum, sum
-  __shared__ float staged[TK_WARPS][R][kPitch];
+// P pieces of 16 bytes a lane (piece i of lane j is the row's piece 8 i + j), R queries
+template <class T, int P, int R, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, WARPS > 4 ? 1 : (R > 1 ? 3 : 4)) token_kernel(const __grid_constant__ TkParams p, int parts) {
+  constexpr int V = Lane<T>::V, H = P * V / 2, kCols = TK_LANES * P * V;
+  constexpr int kPitch = kCols + 4;   // floats of a staged row: O, maximum, sum
+  __shared__ __align__(16) float staged[WARPS][R][kPitch];
   pdl_wait();
   if (threadIdx.x == 0) {
     pdl_launch_dependents();
     if (blockIdx.x == 0 && p.status) *p.status = 0;   // every call starts clean
   }
   const int head = blockIdx.x / parts, part = blockIdx.x - head * parts;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = lane / G, at = (lane % G) * V;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = lane / TK_LANES, at = (lane % TK_LANES) * V;
   const int hb = head / p.vk.heads, hh = head - hb * p.vk.heads;
   auto base = [&](const void* x, const View& v) { return static_cast<const T*>(x) + hb * v.batch + hh * v.head + at; };
   const T *q = base(p.q, p.vq), *k = base(p.k, p.vk), *v = base(p.v, p.vv);
-  const bool in_k = at < p.d, in_v = at < p.d_v && p.o;
+  auto column = [&](int i) { return at + i * TK_LANES * V; };   // of piece i
   const int off = p.n_k - p.n_q;
 
   float2 qs[R][H], acc[R][H];
   float m[R], l[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    uint4 w = make_uint4(0u, 0u, 0u, 0u);
-    if (in_k && r < p.n_q) w = *reinterpret_cast<const uint4*>(q + r * p.vq.row);
-    Lane<T>::unpack(w, qs[r]);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      uint4 w = make_uint4(0u, 0u, 0u, 0u);
+      if (column(i) < p.d && r < p.n_q) w = *reinterpret_cast<const uint4*>(q + r * p.vq.row + i * TK_LANES * V);
+      Lane<T>::unpack(w, &qs[r][i * V / 2]);
+    }
     m[r] = -INFINITY;
     l[r] = 0.f;
 #pragma unroll
@@ -97,27 +109,40 @@ __global__ void __launch_bounds__(TK_THREADS) token_kernel(const __grid_constant
   }
 
   // this group's keys: every streams-th one of the part's, counted over first keys and window
-  const int begin = static_cast<int>(static_cast<long long>(p.count) * part / parts);
-  const int end = static_cast<int>(static_cast<long long>(p.count) * (part + 1) / parts);
-  constexpr int kStreams = TK_WARPS * kGroups;
-  for (int x0 = begin; x0 < end; x0 += kStreams * kBatch) {   // (the same number of rounds for all: the shuffles are the warp's)
-    uint4 kw[kBatch], vw[kBatch];
-    int key[kBatch];
+  constexpr int kStreams = WARPS * TK_GROUPS, kRound = kStreams * TK_BATCH;
+  const int rounds = (p.count + kRound - 1) / kRound;   // shared out whole
+  const int begin = static_cast<int>(static_cast<long long>(rounds) * part / parts) * kRound;
+  const int end = min(p.count, static_cast<int>(static_cast<long long>(rounds) * (part + 1) / parts) * kRound);
+  // (the same number of rounds for all groups: the shuffles are the warp's)
+  for (int x0 = begin; x0 < end; x0 += kRound) {
+    uint4 kw[TK_BATCH][P], vw[TK_BATCH][P];
+    int key[TK_BATCH];
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int x = x0 + (u * TK_WARPS + warp) * kGroups + group;
+    for (int u = 0; u < TK_BATCH; ++u) {
+      const int x = x0 + (u * WARPS + warp) * TK_GROUPS + group;
       key[u] = x >= end ? -1 : (x < p.sinks ? x : p.first + x - p.sinks);
-      kw[u] = vw[u] = make_uint4(0u, 0u, 0u, 0u);
-      if (key[u] >= 0 && in_k) kw[u] = *reinterpret_cast<const uint4*>(k + key[u] * p.vk.row);
+      const T* from = k + (key[u] < 0 ? 0 : key[u]) * p.vk.row;
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        kw[u][i] = make_uint4(0u, 0u, 0u, 0u);
+        if (key[u] >= 0 && column(i) < p.d) kw[u][i] = load16(from + i * TK_LANES * V);
+      }
     }
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u)
-      if (key[u] >= 0 && in_v) vw[u] = *reinterpret_cast<const uint4*>(v + key[u] * p.vv.row);
-    float s[R][kBatch];
+    for (int u = 0; u < TK_BATCH; ++u) {
+      const T* from = v + (key[u] < 0 ? 0 : key[u]) * p.vv.row;
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
+      for (int i = 0; i < P; ++i) {
+        vw[u][i] = make_uint4(0u, 0u, 0u, 0u);
+        if (key[u] >= 0 && column(i) < p.d_v && p.o) vw[u][i] = load16(from + i * TK_LANES * V);
+      }
+    }
+    float s[R][TK_BATCH];
+#pragma unroll
+    for (int u = 0; u < TK_BATCH; ++u) {
       float2 ks[H];
-      Lane<T>::unpack(kw[u], ks);
+#pragma unroll
+      for (int i = 0; i < P; ++i) Lane<T>::unpack(kw[u][i], &ks[i * V / 2]);
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         float2 dot = __fmul2_rn(qs[r][0], ks[0]);
@@ -127,19 +152,20 @@ __global__ void __launch_bounds__(TK_THREADS) token_kernel(const __grid_constant
       }
     }
 #pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1)
+    for (int o = TK_LANES / 2; o > 0; o >>= 1)
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u)
+      for (int u = 0; u < TK_BATCH; ++u)
 #pragma unroll
         for (int r = 0; r < R; ++r) s[r][u] += __shfl_xor_sync(0xffffffffu, s[r][u], o);
-    uint32_t hidden[R];   // bit u: key u of the batch, for a query that others share it with
+    uint32_t hidden[R];   // bit u: key u of the batch, for a query that another shares it with
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       float top = m[r];
       hidden[r] = 0u;
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        const bool seen = key[u] >= 0 && r < p.n_q && pair_visible(r, key[u], off, 1, p.window, p.sinks);
+      for (int u = 0; u < TK_BATCH; ++u) {
+        bool seen = key[u] >= 0;   // by a single query: every key of the list
+        if (R > 1) seen = seen && r < p.n_q && pair_visible(r, key[u], off, 1, p.window, p.sinks);
         s[r][u] = seen ? s[r][u] * p.sl2 : -INFINITY;
         if (R > 1 && !seen) hidden[r] |= 1u << u;
         top = fmaxf(top, s[r][u]);
@@ -149,7 +175,7 @@ __global__ void __launch_bounds__(TK_THREADS) token_kernel(const __grid_constant
       m[r] = top;
       float sum = 0.f;
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
+      for (int u = 0; u < TK_BATCH; ++u) {
         s[r][u] = ex2(s[r][u] - from);
         sum += s[r][u];
       }
@@ -158,9 +184,10 @@ __global__ void __launch_bounds__(TK_THREADS) token_kernel(const __grid_constant
       for (int h = 0; h < H; ++h) acc[r][h] = __fmul2_rn(acc[r][h], make_float2(alpha, alpha));
     }
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
+    for (int u = 0; u < TK_BATCH; ++u) {
       float2 vs[H];
-      Lane<T>::unpack(vw[u], vs);
+#pragma unroll
+      for (int i = 0; i < P; ++i) Lane<T>::unpack(vw[u][i], &vs[i * V / 2]);
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -176,7 +203,7 @@ __global__ void __launch_bounds__(TK_THREADS) token_kernel(const __grid_constant
 #pragma unroll
   for (int r = 0; r < R; ++r) {
 #pragma unroll
-    for (int o = G; o < 32; o <<= 1) {
+    for (int o = TK_LANES; o < 32; o <<= 1) {
       float2 a2[H];
       const float m2 = __shfl_xor_sync(0xffffffffu, m[r], o), l2 = __shfl_xor_sync(0xffffffffu, l[r], o);
 #pragma unroll
@@ -194,48 +221,79 @@ __global__ void __launch_bounds__(TK_THREADS) token_kernel(const __grid_constant
       }
     }
     if (group == 0) {
-      float* to = &staged[warp][r][at];
 #pragma unroll
-      for (int h = 0; h < H; ++h) *reinterpret_cast<float2*>(to + 2 * h) = acc[r][h];
+      for (int i = 0; i < P; ++i)
+#pragma unroll
+        for (int h = 0; h < V / 2; ++h) *reinterpret_cast<float2*>(&staged[warp][r][column(i) + 2 * h]) = acc[r][i * V / 2 + h];
       if (at == 0) {
-        staged[warp][r][G * V] = m[r];
-        staged[warp][r][G * V + 1] = l[r];
+        staged[warp][r][kCols] = m[r];
+        staged[warp][r][kCols + 1] = l[r];
+      }
+    }
+  }
+  __syncthreads();
+  // A warp a query, a lane the columns 2 lane, 2 lane + 64, ...  What is added up is read before the first sum.
+  constexpr int kMine = (kCols + 63) / 64;   // pairs of columns of a lane
+  float2 a[kMine];
+  float mt, lt;
+  auto add_up = [&](auto most, int count, auto&& load) {   // load(i, at): element `at` of the i-th result
+    constexpr int kMost = decltype(most)::value;
+    float2 all[kMost][kMine];
+    float ms[kMost], ls[kMost];
+#pragma unroll
+    for (int i = 0; i < kMost; ++i) {
+      ms[i] = -INFINITY;
+      ls[i] = 0.f;
+#pragma unroll
+      for (int c = 0; c < kMine; ++c) {
+        const int col = 2 * lane + 64 * c;
+        all[i][c] = i < count && col < kCols ? make_float2(load(i, col), load(i, col + 1)) : make_float2(0.f, 0.f);
+      }
+      if (i < count) {
+        ms[i] = load(i, kCols);
+        ls[i] = load(i, kCols + 1);
+      }
+    }
+    mt = ms[0];
+    lt = ls[0];
+#pragma unroll
+    for (int c = 0; c < kMine; ++c) a[c] = all[0][c];
+#pragma unroll
+    for (int i = 1; i < kMost; ++i)
+      if (i < count) merge<kMine>(mt, lt, a, ms[i], ls[i], all[i]);
+  };
+  if (warp < R) {
+    add_up(std::integral_constant<int, WARPS>{}, WARPS, [&](int i, int c) { return staged[i][warp][c]; });
+    __syncwarp();
+    if (parts > 1) {   // this CTA's result, where its first warp's was
+#pragma unroll
+      for (int c = 0; c < kMine; ++c)
+        if (2 * lane + 64 * c < kCols) *reinterpret_cast<float2*>(&staged[0][warp][2 * lane + 64 * c]) = a[c];
+      if (lane == 0) {
+        staged[0][warp][kCols] = mt;
+        staged[0][warp][kCols + 1] = lt;
       }
     }
   }
   if (parts > 1) cluster_sync();
-  else __syncthreads();
-  // part `part` finishes every parts-th row; a warp a row
-  for (int r = part + parts * warp; r < p.n_q; r += parts * TK_WARPS) {
-    constexpr int kMine = (G * V + 63) / 64;   // pairs of columns of a lane
-    float mt = -INFINITY, lt = 0.f;
-    float2 a[kMine];
+  if (warp < p.n_q && warp < R && warp % parts == part) {
+    if (parts > 1) {
+      uint32_t there[kMaxParts];
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) a[i] = make_float2(0.f, 0.f);
-    for (int c = 0; c < parts; ++c)
-      for (int w = 0; w < TK_WARPS; ++w) {
-        const uint32_t from = smem_u32(&staged[w][r][0]);
-        const uint32_t there = parts > 1 ? cluster_map(from, c) : from;
-        auto load = [&](int i) { return parts > 1 ? cluster_ld(there + 4 * i) : staged[w][r][i]; };
-        float2 b[kMine];
-#pragma unroll
-        for (int i = 0; i < kMine; ++i) {
-          const int col = 2 * lane + 64 * i;
-          b[i] = col < G * V ? make_float2(load(col), load(col + 1)) : make_float2(0.f, 0.f);
-        }
-        merge<kMine>(mt, lt, a, load(G * V), load(G * V + 1), b);
-      }
-    const size_t row = static_cast<size_t>(head) * p.n_q + r;
+      for (int c = 0; c < kMaxParts; ++c) there[c] = cluster_map(smem_u32(&staged[0][warp][0]), c < parts ? c : 0);
+      add_up(std::integral_constant<int, kMaxParts>{}, parts, [&](int i, int c) { return cluster_ld(there[i] + 4 * c); });
+    }
+    const size_t row = static_cast<size_t>(head) * p.n_q + warp;
     if (lane == 0) p.lse[row] = lt == 0.f ? -INFINITY : (mt + log2f(lt)) * 0.6931471805599453f;
     if (p.o) {
       const float inv = lt == 0.f ? 0.f : 1.f / lt;
       T* o = static_cast<T*>(p.o) + row * p.d_v;
 #pragma unroll
-      for (int i = 0; i < kMine; ++i) {
-        const int col = 2 * lane + 64 * i;
+      for (int c = 0; c < kMine; ++c) {
+        const int col = 2 * lane + 64 * c;
         if (col < p.d_v) {   // an even number of columns
-          o[col] = static_cast<T>(a[i].x * inv);
-          o[col + 1] = static_cast<T>(a[i].y * inv);
+          o[col] = static_cast<T>(a[c].x * inv);
+          o[col + 1] = static_cast<T>(a[c].y * inv);
         }
       }
     }
@@ -244,21 +302,26 @@ __global__ void __launch_bounds__(TK_THREADS) token_kernel(const __grid_constant
 }
 
 template <class T>
-int token_launch(const TkParams& p, int heads, int parts, cudaStream_t s) {
+int token_launch(const TkParams& p, int heads, cudaStream_t s) {
   const int pieces = ((p.d > p.d_v ? p.d : p.d_v) * static_cast<int>(sizeof(T)) + 15) / 16;
-  auto go = [&](auto lanes, auto rows) -> int {
-    constexpr auto kernel = token_kernel<T, decltype(lanes)::value, decltype(rows)::value>;
-    FHOB_CUDA_OK(launch_pdl(kernel, static_cast<unsigned>(heads * parts), TK_THREADS, 0, parts, s, p, parts));
+  // Four rounds of 64 keys a CTA of 4 warps; what 8 such CTAs would take long for, CTAs of 16 warps share.
+  constexpr int kRound = 4 * TK_GROUPS * TK_BATCH;
+  int parts = (p.count + 4 * kRound - 1) / (4 * kRound);
+  parts = parts > kMaxParts ? kMaxParts : parts;
+  auto go = [&](auto each, auto rows) -> int {
+    constexpr int P = decltype(each)::value, R = decltype(rows)::value;
+    const unsigned grid = static_cast<unsigned>(heads * parts);
+    if (p.count <= 8192) FHOB_CUDA_OK(launch_pdl(token_kernel<T, P, R, 4>, grid, 128, 0, parts, s, p, parts));
+    else FHOB_CUDA_OK(launch_pdl(token_kernel<T, P, R, 16>, grid, 512, 0, parts, s, p, parts));
     return FHOB_OK;
   };
-  auto rows = [&](auto lanes) -> int {
-    if (p.n_q == 1) return go(lanes, std::integral_constant<int, 1>{});
-    if (p.n_q == 2) return go(lanes, std::integral_constant<int, 2>{});
-    return p.n_q <= 4 ? go(lanes, std::integral_constant<int, 4>{}) : go(lanes, std::integral_constant<int, 8>{});
+  auto rows = [&](auto each) -> int {
+    return p.n_q == 1 ? go(each, std::integral_constant<int, 1>{}) : go(each, std::integral_constant<int, 2>{});
   };
-  if (pieces <= 4) return rows(std::integral_constant<int, 4>{});
-  if (pieces <= 8) return rows(std::integral_constant<int, 8>{});
-  return pieces <= 16 ? rows(std::integral_constant<int, 16>{}) : rows(std::integral_constant<int, 32>{});
+  if (pieces <= TK_LANES) return rows(std::integral_constant<int, 1>{});
+  if constexpr (sizeof(T) == 4)
+    if (pieces > 2 * TK_LANES) return rows(std::integral_constant<int, 4>{});
+  return rows(std::integral_constant<int, 2>{});
 }
 
 }  // namespace
@@ -268,8 +331,8 @@ bool token_supported(const Problem& p, const void* o_out) {
   const int es = p.dtype == FHOB_F32 ? 4 : 2, d_v = head_dim_v(p);
   const uintptr_t all = reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) |
                         static_cast<uintptr_t>(p.d * es) | static_cast<uintptr_t>(d_v * es);
-  return p.sinks > 0 && p.n_q <= 8 && (all & 15u) == 0 && (reinterpret_cast<uintptr_t>(o_out) & 3u) == 0 && p.d <= 128 && d_v <= 128 &&
-         static_cast<long long>(p.bh) * 8 <= 0x7fffffffLL;
+  return p.sinks > 0 && p.n_q <= 2 && (all & 15u) == 0 && (reinterpret_cast<uintptr_t>(o_out) & 3u) == 0 && p.d <= 128 && d_v <= 128 &&
+         static_cast<long long>(p.bh) * kMaxParts <= 0x7fffffffLL;
 }
 
 int token_forward(const Problem& p, void* o_out, float* lse_out, int* status, cudaStream_t s) {
@@ -288,10 +351,8 @@ int token_forward(const Problem& p, void* o_out, float* lse_out, int* status, cu
   t.first = first > p.sinks ? first : p.sinks;
   t.count = p.sinks + p.n_k - t.first;
   t.sl2 = p.scale * kLog2e;
-  int parts = (t.count + 127) / 128;
-  if (parts > 8) parts = 8;
-  if (p.dtype == FHOB_F32) return token_launch<float>(t, p.bh, parts, s);
-  return p.dtype == FHOB_F16 ? token_launch<__half>(t, p.bh, parts, s) : token_launch<__nv_bfloat16>(t, p.bh, parts, s);
+  if (p.dtype == FHOB_F32) return token_launch<float>(t, p.bh, s);
+  return p.dtype == FHOB_F16 ? token_launch<__half>(t, p.bh, s) : token_launch<__nv_bfloat16>(t, p.bh, s);
 }
 
 }  // namespace fhob
