@@ -157,22 +157,34 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
   }
   const int n_tiles = t_end > t_begin ? t_end - t_begin : 0;
   auto key_tile = [&](int t) { return !SINKS || t < n_first ? t : w_begin + t - n_first; };
-  auto active = [&](int x, int t) {
-    if constexpr (!SINKS) return t >= begin[x] && t < end[x];
-    if (t >= t_end) return false;
-    return t < n_first ? live(x) : key_tile(t) >= begin[x] && key_tile(t) < end[x];
-  };
-  // with first keys: the steps between them and x's window
-  auto skipped = [&](int x) { return end[x] > begin[x] ? begin[x] - w_begin : 0; };
+  // Of query tile x (worked out once: the issuing thread asks for every product): steps [w0, w1) are the window's, `late` of them
+  // come between the first keys and w0, `total` steps in all.
+  int w0[2], w1[2], late[2], total[2], firsts[2];
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    w0[x] = begin[x];
+    w1[x] = end[x];
+    late[x] = firsts[x] = 0;
+    total[x] = end[x] - begin[x];
+    if constexpr (SINKS) {
+      const bool any = end[x] > begin[x];
+      late[x] = any ? begin[x] - w_begin : 0;
+      w0[x] = n_first + late[x];
+      w1[x] = min(w0[x] + total[x], t_end);
+      firsts[x] = live(x) ? min(n_first, t_end) : 0;
+      total[x] = p.split > 1 ? (x == 0 ? n_tiles : 0) : firsts[x] + total[x];
+    }
+  }
+  auto active = [&](int x, int t) { return (t >= w0[x] && t < w1[x]) || (SINKS && t < firsts[x]); };
   // how many steps of x there are, and how many of them come before t
-  auto steps = [&](int x) {
-    if constexpr (!SINKS) return end[x] - begin[x];
-    return p.split > 1 ? (x == 0 ? n_tiles : 0) : (live(x) ? n_first : 0) + end[x] - begin[x];
-  };
+  auto steps = [&](int x) { return total[x]; };
   auto step_no = [&](int x, int t) {
     if constexpr (!SINKS) return t - begin[x];
-    return t - t_begin - (t < n_first ? 0 : skipped(x));
+    return t - t_begin - (t < n_first ? 0 : late[x]);
   };
+
+  // Up to 32 first keys: their step works on 32 columns instead of BN.
+  const bool few = SINKS && p.sinks <= 32;
 
   int fault = 0;   // thread 0: what to report at the end
   if (threadIdx.x == 0) {
@@ -261,7 +273,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
   } else if (warp == MMA_WARP) {
     // ================================================= MMA issuer (one thread: the pipe runs its products in order)
     if (n_tiles > 0 && elect_one()) {
-      constexpr uint32_t idesc_s = umma_idesc_bf16(BM, BN, false, false, F16);
+      constexpr uint32_t idesc_s_all = umma_idesc_bf16(BM, BN, false, false, F16), idesc_s_few = umma_idesc_bf16(BM, 32, false, false, F16);
       constexpr uint32_t idesc_o = umma_idesc_bf16(BM, kO, false, true, F16);
       constexpr uint32_t idesc_o64 = umma_idesc_bf16(BM, 64, false, true, F16);   // split operands: the hi box alone
       constexpr int kBox = BM * 128;
@@ -280,6 +292,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
         if (!wait(&bars->kv_full[slot], (i / C::NSLOT) & 1)) return;
         tc_fence_after();
         const uint32_t a = q_lo + x * kQ16, b = ring_lo + slot * kSlot16;
+        const uint32_t idesc_s = few && t < n_first ? idesc_s_few : idesc_s_all;
         if constexpr (SPLIT) {
 #pragma unroll
           for (int term = 0; term < 3; ++term)   // (hi, hi), (hi, lo), (lo, hi)
@@ -307,16 +320,22 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
             umma_ts_split(o_cols(x), s_cols(x, stage) + 8 * ks, b + ((ks * 2048) >> 4), kDescHi, idesc_o, accumulate || ks > k0 ? 1u : 0u);
         };
         constexpr int kFirst = kHalves ? BN / 32 : BN / 16;
-        pv(0, kFirst, it > 0);
-        if (kHalves) {
-          if (!wait(&bars->p_full[x][stage], it & 1)) return;
-          tc_fence_after();
-          pv(kFirst, BN / 16, true);
+        const bool short_step = few && t < n_first;   // 32 keys
+        if (short_step) {
+          pv(0, 2, it > 0);
+          if (kHalves && !wait(&bars->p_full[x][stage], it & 1)) return;
+        } else {
+          pv(0, kFirst, it > 0);
+          if (kHalves) {
+            if (!wait(&bars->p_full[x][stage], it & 1)) return;
+            tc_fence_after();
+            pv(kFirst, BN / 16, true);
+          }
         }
         if (SPLIT) {   // above P_hi . [V_hi | V_lo]; here P_lo . V_hi on top of the second half
 #pragma unroll
           for (int ks = 0; ks < BN / 16; ++ks)
-            umma_ts_split(o_cols(x) + 64, s_cols(x, stage) + BN / 2 + 8 * ks, b + ((ks * 2048) >> 4), kDescHi, idesc_o64, 1u);
+            if (!short_step || ks < 2) umma_ts_split(o_cols(x) + 64, s_cols(x, stage) + BN / 2 + 8 * ks, b + ((ks * 2048) >> 4), kDescHi, idesc_o64, 1u);
         }
         umma_commit(&bars->o_done[x]);
         if (it + 1 == steps(x)) umma_commit(&bars->out_full[x]);
@@ -324,17 +343,20 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
       };
       if (OUT) {
         for (int t = t_begin; ok && t < t_begin + kStages; ++t)
-          for (int x = 0; ok && x < 2; ++x)
-            if (active(x, t)) scores(x, t);
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            if (ok && active(x, t)) scores(x, t);
         for (int t = t_begin; ok && t < t_end; ++t)
-          for (int x = 0; ok && x < 2; ++x) {
-            if (active(x, t)) output(x, t);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (ok && active(x, t)) output(x, t);
             if (ok && active(x, t + kStages)) scores(x, t + kStages);
           }
       } else {
         for (int t = t_begin; ok && t < t_end; ++t)
-          for (int x = 0; ok && x < 2; ++x)
-            if (active(x, t)) scores(x, t);
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            if (ok && active(x, t)) scores(x, t);
       }
       if (!ok) {
         // abort path: no tcgen05.mma may still be reading shared memory or TMEM at exit
@@ -348,7 +370,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const int m0 = m_of(x), g_row = m0 + row;
-    const int n_iter = steps(x);
+    const int n_iter = SINKS ? (x ? total[1] : total[0]) : steps(x), my_late = x ? late[1] : late[0];
     const float sl2 = p.scale * kLog2e, abs_sl2 = fabsf(sl2);
     // visible keys of this row
     int lo = 0, hi = p.n_k - 1;
@@ -359,13 +381,13 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
     bool ok = true;
     const uint32_t o_addr = lane_base + o_cols(x);
 
-    // One key tile; tiles that need masking take a copy of the code of their own.
-    auto step = [&](auto masked_tile, int it, int n0, int stage, int lo, int hi) {
+    // One key tile, COLS keys of it; tiles that need masking take a copy of the code of their own.
+    auto step = [&](auto masked_tile, auto cols, int it, int n0, int stage, int lo, int hi) {
       ok = __all_sync(0xffffffffu, wait_bar(&bars->s_full[x][stage], (it / kStages) & 1, bars, p.status));
       if (!ok) return;
       tc_fence_after();
       const uint32_t s_addr = lane_base + s_cols(x, stage);
-      constexpr int NC = BN / 32;
+      constexpr int COLS = decltype(cols)::value, NC = COLS / 32;
       uint32_t s[NC][32];
 #pragma unroll
       for (int c = 0; c < NC; ++c) tmem_ld32(s_addr + 32 * c, s[c]);
@@ -393,10 +415,10 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
       float mx[MXC];
 #pragma unroll
       for (int i = 0; i < MXC; ++i) {
-        mx[i] = fmaxf(__uint_as_float(s[i * NC / MXC][(i * (BN / MXC)) % 32]), __uint_as_float(s[i * NC / MXC][(i * (BN / MXC)) % 32 + 1]));
+        mx[i] = fmaxf(__uint_as_float(s[i * NC / MXC][(i * (COLS / MXC)) % 32]), __uint_as_float(s[i * NC / MXC][(i * (COLS / MXC)) % 32 + 1]));
 #pragma unroll
-        for (int j = 2; j < BN / MXC; j += 2) {
-          const int g = i * (BN / MXC) + j;
+        for (int j = 2; j < COLS / MXC; j += 2) {
+          const int g = i * (COLS / MXC) + j;
           mx[i] = max3(mx[i], __uint_as_float(s[g / 32][g % 32]), __uint_as_float(s[g / 32][g % 32 + 1]));
         }
       }
@@ -449,7 +471,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
         // the row's scores are in registers: P goes over them, 16 packed columns per 32 keys
         if constexpr (OUT) tmem_st16(s_addr + 16 * c, w);
         if constexpr (OUT && SPLIT) tmem_st16(s_addr + BN / 2 + 16 * c, w_lo);
-        if (kHalves && c == NC / 2 - 1) {
+        if (kHalves && (COLS == BN ? c == NC / 2 - 1 : true)) {   // (of a short step all of P)
           tmem_wait_st();
           tc_fence_before();
           mbar_arrive(&bars->p_half[x]);
@@ -464,7 +486,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
     };
     for (int it = 0; it < n_iter; ++it) {
       const bool first = SINKS && t_begin + it < n_first;   // a tile of the first keys: [0, sinks) of it
-      const int t = SINKS ? t_begin + it + (first ? 0 : skipped(x)) : begin[x] + it;
+      const int t = SINKS ? t_begin + it + (first ? 0 : my_late) : begin[x] + it;
       const int n0 = key_tile(t) * BN, stage = it % kStages;
       // does any score of this tile need masking?  (uniform over the tile's warps)
       bool masked = n0 + BN > p.n_k;
@@ -473,8 +495,10 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
         if (p.window > 0) masked = masked || (first ? n0 + BN > p.sinks : m0 + BM - 1 + off - n0 >= p.window || (SINKS && n0 < p.sinks));
       }
       const int lo_t = first ? 0 : lo, hi_t = first && p.sinks <= hi ? p.sinks - 1 : hi;   // (lo, hi without first keys)
-      if (masked) step(std::true_type{}, it, n0, stage, lo_t, hi_t);
-      else step(std::false_type{}, it, n0, stage, lo_t, hi_t);
+      using All = std::integral_constant<int, BN>;
+      if (SINKS && few && first) step(std::true_type{}, std::integral_constant<int, SINKS ? 32 : BN>{}, it, n0, stage, lo_t, hi_t);
+      else if (masked) step(std::true_type{}, All{}, it, n0, stage, lo_t, hi_t);
+      else step(std::false_type{}, All{}, it, n0, stage, lo_t, hi_t);
       if (!ok) break;
     }
 
