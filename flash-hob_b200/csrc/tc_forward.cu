@@ -183,8 +183,9 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
     return t - t_begin - (t < n_first ? 0 : late[x]);
   };
 
-  // Up to 32 first keys: their step works on 32 columns instead of BN.
-  const bool few = SINKS && p.sinks <= 32;
+  // Up to 32 first keys: their step works on 32 columns instead of 128 (32 heads N = 4096 W = 1024 D = 128 146 -> 141 us).  Not at 64-key
+  // tiles, where a third copy of the step costs more (64 heads N = 8192 W = 512 D = 64 267 -> 311 us).
+  const bool few = SINKS && BN == 128 && p.sinks <= 32;
 
   int fault = 0;   // thread 0: what to report at the end
   if (threadIdx.x == 0) {
@@ -496,7 +497,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
       }
       const int lo_t = first ? 0 : lo, hi_t = first && p.sinks <= hi ? p.sinks - 1 : hi;   // (lo, hi without first keys)
       using All = std::integral_constant<int, BN>;
-      if (SINKS && few && first) step(std::true_type{}, std::integral_constant<int, SINKS ? 32 : BN>{}, it, n0, stage, lo_t, hi_t);
+      if (SINKS && BN == 128 && few && first) step(std::true_type{}, std::integral_constant<int, SINKS && BN == 128 ? 32 : BN>{}, it, n0, stage, lo_t, hi_t);
       else if (masked) step(std::true_type{}, All{}, it, n0, stage, lo_t, hi_t);
       else step(std::false_type{}, All{}, it, n0, stage, lo_t, hi_t);
       if (!ok) break;
