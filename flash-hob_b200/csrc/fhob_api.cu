@@ -241,6 +241,11 @@ Problem plain_problem(const FhobProblem& p) {
   return q;
 }
 
+// Backwards with first keys in fp32: the CUDA cores, unless the caller asks for the tensor cores.  Split operands
+// leave 2-norm errors of 0.8e-5 to 3e-5 (the longer the window, the larger), the CUDA cores 6e-7 (8 heads N = 2048 D = 64 W = 512, double
+// backward: 122 us against 916).  Problems without first keys keep the kernels they had.
+bool use_tc_backward(const Problem& p) { return use_tc(p) && !(p.sinks > 0 && p.dtype == FHOB_F32 && p.impl == FHOB_IMPL_AUTO); }
+
 int run_pass(int pass, const FhobProblem* p, void* stream) {
   int st = validate(p, pass >= 3);
   if (st != FHOB_OK) return st;
@@ -379,8 +384,10 @@ int fhob_bwdbwd_sinks(const FhobProblem* given, int32_t sink_tokens, void* strea
   std::lock_guard<std::mutex> together(workspace_lock(p->workspace));
   // tensor cores: dd and b come out of one sweep (sum_j P dP = D makes b linear in sums that need no
   // dd), which also computes D and clears the status word, so there is no pre-pass
-  if (use_tc(*p)) return tc_operator(*p, s);
-  st = run_prepass(p, stream);
+  if (use_tc_backward(*p)) return tc_operator(*p, s);
+  if (p->layout) return FHOB_ERR_SHAPE;   // (views are read by the tensor-core kernels)
+  if (!p->o) return FHOB_ERR_ARG;
+  st = run_prepass(p, stream, false);
   if (st != FHOB_OK) return st;
   st = simt_pass(12, *p, s);
   return st != FHOB_OK ? st : simt_pass(34, *p, s);
@@ -509,11 +516,12 @@ int fhob_backward_sinks(const FhobProblem* given, int32_t sink_tokens, void* dq,
   if (st != FHOB_OK) return st;
   const Problem* p = &problem;
   if (!aligned16(dq) || !aligned16(dk) || !aligned16(dv)) return FHOB_ERR_ALIGN;
+  const bool tc = (p->impl == FHOB_IMPL_TCGEN05 || (p->impl == FHOB_IMPL_AUTO && tc_first_order_supported(*p))) && use_tc_backward(*p);
+  if (p->layout && !tc) return FHOB_ERR_SHAPE;
   std::lock_guard<std::mutex> together(workspace_lock(p->workspace));
   st = run_prepass(p, stream, false);  // stores -L*log2(e) and -D in the workspace
   if (st != FHOB_OK) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool tc = p->impl == FHOB_IMPL_TCGEN05 || (p->impl == FHOB_IMPL_AUTO && tc_first_order_supported(*p));
   return tc ? tc_backward(*p, dq, dk, dv, s) : simt_backward(*p, dq, dk, dv, s);
 }
 

@@ -150,7 +150,8 @@ class _Problem:
         # stays on the 16-byte grid; anything else is made contiguous first (a copy).
         batches, heads = (Q.shape[0], Q.shape[1]) if Q.dim() == 4 else (1, Q.shape[0])
         strides = None
-        if (allow_views and impl != "simt" and _tc_capable(dt, Q.shape[-1], V.shape[-1])
+        on_cuda_cores = impl == "simt" or (impl == "auto" and sinks and dt == torch.float32)
+        if (allow_views and not on_cuda_cores and _tc_capable(dt, Q.shape[-1], V.shape[-1])
                 and not all(t.is_contiguous() for t in tensors)):
             strides = [_strides_of(t, batches, heads) for t in tensors]
             if any(st is None for st in strides):
@@ -297,7 +298,8 @@ def flash_bwdbwd(Q, K, V, O, dO, ddQ, ddK, ddV, L, scale, *, is_causal: bool = F
     the oracle's ``sliding_window_length`` W (needs ``is_causal``): query i
     then sees only the W keys that end at its causal diagonal; ``sink_tokens``
     S (needs ``sliding_window``): the first S keys stay visible to every query
-    from their own on; ``impl`` one of
+    from their own on (float32 then runs on the CUDA cores unless ``impl`` is
+    "tcgen05", which is several times faster and good to 3e-5); ``impl`` one of
     "auto", "simt", "tcgen05"; ``check`` read the device status word after
     the kernels and raise if a bounded device wait ran out.  Reading it
     synchronises the stream, so the default is ``False`` for device tensors

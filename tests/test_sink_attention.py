@@ -93,6 +93,22 @@ def test_all_directions(bh, nq, nk, window, sinks, dtype, d, impl):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_fp32_is_fp32(d):
+    """2-norm errors of a long fp32 problem: the backwards run on the CUDA cores, whose rows of sums have up to 2000 / 2 terms in a
+    part, off by 2^-24 of the running sum each: 1e-6 if they average out over a tenth of them; the forward's split operands (2^-17
+    each, and their product) stay below 1e-5.  impl="tcgen05" asks for the tensor cores all the way: 4e-5."""
+    x = make_inputs(2, 2000, 2300, d, seed=d, dtype=torch.float32, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = {n: t + 1e-3 * torch.randn(t.shape, generator=g, device="cuda") for n, t in x.items()}   # values that bf16 does not hold
+    ref = dense(x, d ** -0.5, 700, 20)
+    for impl in ("auto", "tcgen05") if d <= 64 else ("auto",):
+        for n, a, b in zip(NAMES, ours(x, d ** -0.5, 700, 20, impl), ref):
+            err = float((a.reshape(b.shape).double() - b).norm() / b.norm())
+            assert err < (4e-5 if impl == "tcgen05" else 1e-5), (impl, n, err)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("d,d_v", [(64, 128), (128, 64), (32, 96)])
 def test_two_head_dims_and_no_o(d, d_v):
     x = make_inputs(2, 400, 450, d, seed=5, dtype=torch.bfloat16, device="cuda")
