@@ -22,6 +22,7 @@ import ctypes as C
 import torch
 
 from . import _lib
+from .layer import RotaryPositions, rotary as _rotary
 from .ops import _native, _Problem, _sinks, _window
 
 
@@ -57,11 +58,26 @@ def attention_backward(Q, K, V, O, dO, L, scale, *, is_causal: bool = False, sli
     return dq, dk, dv
 
 
-def attention(q, k, v, scale=None, *, is_causal: bool = False, sliding_window=None, sink_tokens: int = 0):
+def _turned(q, k, r: RotaryPositions):
+    """Queries and keys at their positions: the positions are the keys', the queries are the last of them (as in a causal mask)."""
+    n_q, n_k = q.shape[-2], k.shape[-2]
+    if r.positions.shape[-1] != n_k or n_q > n_k:
+        raise ValueError(f"rotary positions: expected one for each of the {n_k} keys, of which the {n_q} queries are the last, "
+                         f"got {tuple(r.positions.shape)}")
+    turn = lambda x, at: _rotary(x, at, r.frequencies, r.axis_of_pair, interleaved=r.interleaved)   # noqa: E731
+    if n_q == n_k:
+        return turn((q, k), r.positions)
+    return turn(q, r.positions[..., n_k - n_q:]), turn(k, r.positions)
+
+
+def attention(q, k, v, scale=None, *, is_causal: bool = False, sliding_window=None, sink_tokens: int = 0, rotary=None):
     """``softmax(q k^T scale) v`` for CUDA bfloat16/float32 tensors ``(BH, N, D)`` or ``(B, H, N, D)``,
     differentiable twice (``create_graph=True``).  ``sliding_window`` W: a query sees the W keys up to its diagonal;
-    ``sink_tokens`` S: and the first S keys."""
+    ``sink_tokens`` S: and the first S keys.  ``rotary``: a ``fhob.RotaryPositions``; queries and keys are turned by it first."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
     window = _window(is_causal, sliding_window)
-    return _native().attention(q, k, v, float(scale), bool(is_causal), window, _sinks(window, sink_tokens))
+    sinks = _sinks(window, sink_tokens)
+    if rotary is not None:
+        q, k = _turned(q, k, rotary)
+    return _native().attention(q, k, v, float(scale), bool(is_causal), window, sinks)

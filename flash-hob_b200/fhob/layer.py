@@ -5,7 +5,19 @@ native, csrc/host_layer.cpp).  The reference has no counterpart of either.
 """
 from __future__ import annotations
 
+from typing import NamedTuple, Optional, Sequence
+
+import torch
+
 from .ops import _native
+
+
+class RotaryPositions(NamedTuple):
+    """What ``rotary`` needs besides the tensors, for ``fhob.attention(..., rotary=...)``: ``positions`` are the keys'."""
+    positions: torch.Tensor
+    frequencies: torch.Tensor
+    axis_of_pair: Optional[Sequence[int]] = None
+    interleaved: bool = False
 
 
 def rotary(x, positions, frequencies, axis_of_pair=None, *, interleaved: bool = False, inverse: bool = False):
