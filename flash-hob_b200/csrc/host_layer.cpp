@@ -119,7 +119,12 @@ struct Rotary : torch::autograd::Function<Rotary> {
     const bool interleaved = ctx->saved_data["interleaved"].toBool(), inverse = !ctx->saved_data["inverse"].toBool();
     Tensor d[2];
     const bool has0 = g[0].defined(), has1 = ctx->saved_data["both"].toBool() && g[1].defined();
-    if (has0 || has1) {
+    if (!has0 && !has1) return variable_list(7);
+    if (!at::GradMode::is_enabled()) {   // no graph is asked for
+      const auto r = rotate(has0 ? g[0] : g[1], has0 && has1 ? g[1] : Tensor(), s[0], s[1], axes, interleaved, inverse);
+      d[has0 ? 0 : 1] = r[0];
+      if (has0 && has1) d[1] = r[1];
+    } else {
       const auto r = Rotary::apply(has0 ? g[0] : g[1], has0 && has1 ? Maybe(g[1]) : Maybe(), s[0], s[1], axes, interleaved, inverse);
       d[has0 ? 0 : 1] = r[0];
       if (has0 && has1) d[1] = r[1];
@@ -331,6 +336,11 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const auto s = ctx->get_saved_variables();
     const bool has_w = s[1].defined();   // (inputs are counted without those that are missing)
     const bool want_dw = has_w && ctx->needs_input_grad(1), want_db = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(1 + has_w);
+    if (!at::GradMode::is_enabled()) {   // no graph is asked for
+      Tensor dx, dw, db;
+      norm_backward(g[0], s[0], s[1], s[2], s[3], want_dw, want_db, static_cast<at::ScalarType>(ctx->saved_data["type"].toInt()), dx, dw, db);
+      return {dx, dw, db, Tensor()};
+    }
     const auto r = LayerNormBackward::apply(g[0], s[0], maybe(s[1]), s[2], s[3], want_dw, want_db, ctx->saved_data["type"].toInt());
     return {r[0], want_dw ? r[1] : Tensor(), want_db ? r[1 + want_dw] : Tensor(), Tensor()};
   }

@@ -10,7 +10,7 @@
 //  - a group takes four keys at a time: their rows of K and V are all on their way before the first is used.  What counts besides is
 //    the number of instructions, since a call of few heads has one warp a scheduler: with 16 lanes a key, 51 a key and warp
 //    (and a ring of asynchronous copies, which gained nothing), now about 20;
-//  - a head's keys are shared by the CTAs of a cluster, four batches a CTA and up to 8 CTAs: a number that depends on the
+//  - a head's keys are shared by the CTAs of a cluster, five batches a CTA and up to 8 CTAs: a number that depends on the
 //    lengths alone, as the order in which their results are added up.
 #include "tc_common.cuh"
 
@@ -304,9 +304,10 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS > 4 ? 1 : (R > 1 ? 3 : 4)) t
 template <class T>
 int token_launch(const TkParams& p, int heads, cudaStream_t s) {
   const int pieces = ((p.d > p.d_v ? p.d : p.d_v) * static_cast<int>(sizeof(T)) + 15) / 16;
-  // Four rounds of 64 keys a CTA of 4 warps; what 8 such CTAs would take long for, CTAs of 16 warps share.
+  // Up to five rounds of 64 keys a CTA of 4 warps (128 heads W = 1024: 15.6 us; with four 21.8, with six 16.3; 16 heads 6.4, 5.7 and 6.8).
+  // What 8 such CTAs would take long for, CTAs of 16 warps share.
   constexpr int kRound = 4 * TK_GROUPS * TK_BATCH;
-  int parts = (p.count + 4 * kRound - 1) / (4 * kRound);
+  int parts = (p.count + 5 * kRound - 1) / (5 * kRound);
   parts = parts > kMaxParts ? kMaxParts : parts;
   auto go = [&](auto each, auto rows) -> int {
     constexpr int P = decltype(each)::value, R = decltype(rows)::value;

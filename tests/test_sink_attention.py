@@ -166,9 +166,10 @@ def test_masks_that_are_another(dtype):
 
 
 @pytest.mark.gpu
-def test_views_and_neighbouring_heads():
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_views_and_neighbouring_heads(dtype):
     """A head's bits depend neither on its neighbours nor on where the tensors lie."""
-    x = make_inputs(6, 500, 500, 64, seed=9, dtype=torch.bfloat16, device="cuda")
+    x = make_inputs(6, 500, 500, 64, seed=9, dtype=dtype, device="cuda")
     whole = ours(x, 0.125, 100, 4)
     one = ours({n: t[4:5] for n, t in x.items()}, 0.125, 100, 4)
     assert all(torch.equal(w[4:5], o) for w, o in zip(whole, one))
