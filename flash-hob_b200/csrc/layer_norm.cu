@@ -47,9 +47,12 @@ struct LnParams {
   float eps, inv_cols;
 };
 
-// How a thread's elements lie in a row: in pieces of 16 bytes (V elements each), or, V == 2, one here and one there.
+// How a thread's elements lie in a row: in pieces of 16 bytes (V elements each), or, V == 2, in pairs of neighbours (16 bits), or
+// one here and one there (fp32).
 template <class T, int V>
 constexpr bool kWide = V * sizeof(T) == 16;
+template <class T, int V>
+constexpr bool kTogether = V * sizeof(T) == 16 || sizeof(T) == 2;
 
 // `bytes` of 16 are read, the others zero
 __device__ __forceinline__ void cp_async(uint32_t to, const void* from, int bytes) {
@@ -86,7 +89,7 @@ struct Place {
     width = warps * lanes;
   }
   __device__ __forceinline__ int column(int i, int e = 0) const {
-    return kWide<T, V> ? (first + i * width) * V + e : first + (i * V + e) * width;
+    return kTogether<T, V> ? (first + i * width) * V + e : first + (i * V + e) * width;
   }
   // x at the columns of a pair of piece i, zero behind the last column.  (Pieces of 16 bytes are whole.)
   __device__ __forceinline__ float2 inside(float x, int i, int cols) const {
@@ -102,6 +105,11 @@ struct Place {
     const int c = column(i);
     if (c >= cols) return;
     if constexpr (!kWide<T, V>) {
+      if constexpr (sizeof(T) == 2)
+        if (c + 1 < cols && (reinterpret_cast<uintptr_t>(row) & 2) == 0) {
+          *reinterpret_cast<uint32_t*>(row + c) = pack<T>(x[0]);
+          return;
+        }
       row[c] = static_cast<T>(x[0].x);
       if (column(i, 1) < cols) row[column(i, 1)] = static_cast<T>(x[0].y);
     } else if constexpr (sizeof(T) == 4) {
@@ -202,7 +210,8 @@ template <int WHAT, class T, int V, int NV, int THREADS, bool SUB>
 struct LnCfg {
   static constexpr int kMatrices = WHAT == kLnForward ? 1 : (WHAT == kLnBackward ? 2 : 3);
   static constexpr int kBlocks = ln_threads(WHAT, kWide<T, V>) > THREADS ? ln_threads(WHAT, kWide<T, V>) / THREADS : 1;   // of an SM
-  // Bytes of a row of the ring.  Off the grid a row may start anywhere in a piece of 16 bytes: one more for each group.
+  // Bytes of a row of the ring.  Off the grid a row may start anywhere in a piece of 16 bytes: one more for each group (and a word
+  // that the last pair of the last group looks into).
   static constexpr int kRow = THREADS * NV * V * static_cast<int>(sizeof(T)) + (kWide<T, V> ? 0 : 16 * THREADS / (SUB ? 2 : 32));
   static constexpr int kFit = 200 * 1024 / kBlocks / (kMatrices * kRow);
   static constexpr int kStages = kFit > 4 ? 4 : kFit;                         // rows of the ring
@@ -241,13 +250,14 @@ struct Ring {
       constexpr int kPieces = NV * V * static_cast<int>(sizeof(T)) / 16;
 #pragma unroll
       for (int i = 0; i <= kPieces; ++i) {
-        const int from = (at.first + i * at.width) * 16;
-        if (from < bytes) cp_async(to + from, reinterpret_cast<const void*>(start + from), min(16, bytes - from));
+        // (behind the row zeros: nothing that is read later is older)
+        const int from = (at.first + i * at.width) * 16, left = min(16, bytes - from);
+        if (i < kPieces || at.first == 0) cp_async(to + from, reinterpret_cast<const void*>(left > 0 ? start + from : start), left > 0 ? left : 0);
       }
     }
   }
-  // `row_address`: the low bits of the row's address
-  __device__ __forceinline__ void read(float2 (&to)[NV][V / 2], int stage, int matrix, uint32_t row_address, bool live) const {
+  // `row_address`: the low bits of the row's address.  Zeros behind the last column and for rows that do not exist.
+  __device__ __forceinline__ void read(float2 (&to)[NV][V / 2], int stage, int matrix, uint32_t row_address) const {
     const uint32_t from = slot(stage, matrix);
     if constexpr (kWide<T, V>) {
 #pragma unroll
@@ -264,21 +274,23 @@ struct Ring {
       }
     } else {
       const uint32_t first = from + (row_address & 15u);
-      auto element = [&](int c) {
-        float v = 0.f;
-        if (live && c < cols) {
-          if constexpr (sizeof(T) == 4) {
-            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(first + c * 4));
-          } else {
-            uint16_t u;
-            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(first + c * 2));
-            v = unpack<T>(u).x;
-          }
-        }
-        return v;
-      };
 #pragma unroll
-      for (int i = 0; i < NV; ++i) to[i][0] = make_float2(element(at.column(i, 0)), element(at.column(i, 1)));
+      for (int i = 0; i < NV; ++i) {
+        const uint32_t here = first + at.column(i) * static_cast<uint32_t>(sizeof(T));
+        uint32_t w, next = 0u;
+        if constexpr (sizeof(T) == 4) {
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(here));
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(next) : "r"(here + at.width * 4));
+          to[i][0] = f2(w, next);
+        } else if (here & 2u) {   // the pair lies in two words
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(here - 2));
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(next) : "r"(here + 2));
+          to[i][0] = unpack<T>(__funnelshift_r(w, next, 16));
+        } else {
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w) : "r"(here));
+          to[i][0] = unpack<T>(w);
+        }
+      }
     }
   }
 };
@@ -371,7 +383,7 @@ __global__ void __launch_bounds__(THREADS, LnCfg<kLnForward, T, V, NV, THREADS, 
     copies_wait<C::kStages - 1>();
     if (!kWide<T, V>) at.meet();   // the group's copies
     float2 x[NV][H], s2 = both(0.f);
-    ring.read(x, stage, 0, xs.worked(), row < p.rows);
+    ring.read(x, stage, 0, xs.worked());
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -450,8 +462,8 @@ __global__ void __launch_bounds__(THREADS, LnCfg<kLnBackward, T, V, NV, THREADS,
     copies_wait<C::kStages - 1>();
     if (!kWide<T, V>) at.meet();   // the group's copies
     float2 h[NV][H], g[NV][H], s0 = both(0.f), s1 = both(0.f);   // sums of g, g h
-    ring.read(h, stage, 0, xs.worked(), row < p.rows);
-    ring.read(g, stage, 1, dys.worked(), row < p.rows);
+    ring.read(h, stage, 0, xs.worked());
+    ring.read(g, stage, 1, dys.worked());
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const float2 minus = at.inside(-mean, i, p.cols);   // behind the last column and row h and dy are zero
@@ -536,9 +548,9 @@ __global__ void __launch_bounds__(THREADS, LnCfg<kLnBwdbwd, T, V, NV, THREADS, S
     if (!kWide<T, V>) at.meet();   // the group's copies
     // h, dy and v; all zero behind the last column and the last row
     float2 h[NV][H], d[NV][H], u[NV][H], s0 = both(0.f), s1 = both(0.f), s2 = both(0.f), s3 = both(0.f);
-    ring.read(h, stage, 0, xs.worked(), row < p.rows);
-    ring.read(d, stage, 1, dys.worked(), row < p.rows);
-    ring.read(u, stage, 2, vs.worked(), p.v && row < p.rows);
+    ring.read(h, stage, 0, xs.worked());
+    ring.read(d, stage, 1, dys.worked());
+    ring.read(u, stage, 2, vs.worked());
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const float2 minus = at.inside(-mean, i, p.cols);
