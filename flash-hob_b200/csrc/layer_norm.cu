@@ -652,7 +652,10 @@ LnGrid ln_grid(int what, long long rows, int cols, bool wide) {
   while (g.lanes > 2 && g.lanes / 2 * g.each >= cols) g.lanes >>= 1;
   g.warps = 1;
   while (g.warps < LN_MAX_WARPS && g.warps * 32 * g.each < cols) g.warps <<= 1;
-  g.threads = g.warps * 32 > 256 ? g.warps * 32 : 256;
+  // Larger blocks leave fewer sums over rows to add up (16384 x 2048 bf16, backward 44.2 -> 43.0 us), which in the double backward pays
+  // for rows of few warps only (512 columns 80 -> 77 us, 2048 90 -> 102).
+  const int least = what == kLnForward || g.lanes < 32 || (what == kLnBwdbwd && g.warps > 4) ? 256 : 512;
+  g.threads = g.warps * 32 > least ? g.warps * 32 : least;
   const int groups = g.threads / (g.warps * g.lanes);
   const long long wanted = (rows + groups - 1) / groups;
   const int per_sm = ln_threads(what, wide) / g.threads;
