@@ -640,7 +640,7 @@ struct LnGrid {
   int each, lanes, warps, threads, blocks;   // elements of a thread; of a group: lanes and warps; threads and blocks
 };
 constexpr int kSms = 148;
-constexpr int kLnMostBlocks = 4 * kSms;
+constexpr int kLnMostBlocks = 2 * kSms;   // that leave sums over rows: of 256 threads or more, 512 threads an SM
 
 LnGrid ln_grid(int what, long long rows, int cols, bool wide) {
   LnGrid g;
@@ -704,8 +704,13 @@ int ln_call(const FhobLayerNorm* n, LnParams& p, void* dw, void* db, cudaStream_
       together |= reinterpret_cast<uintptr_t>(matrices[i]) | static_cast<uintptr_t>(strides[i] * es);
     }
   together |= static_cast<uintptr_t>(n->cols) * es;
-  for (const void* vector : {n->w, p.b, p.vw, p.vb}) together |= reinterpret_cast<uintptr_t>(vector);
   if (together % es) return FHOB_ERR_ALIGN;
+  uintptr_t vectors = reinterpret_cast<uintptr_t>(dw) | reinterpret_cast<uintptr_t>(db);
+  for (const void* vector : {n->w, p.b, p.vw, p.vb}) {
+    vectors |= reinterpret_cast<uintptr_t>(vector);
+    together |= reinterpret_cast<uintptr_t>(vector);
+  }
+  if (vectors % (n->w_dtype == FHOB_F32 ? 4 : 2) || (reinterpret_cast<uintptr_t>(n->mean) | reinterpret_cast<uintptr_t>(n->rstd)) % 4) return FHOB_ERR_ALIGN;
   p.w = n->w;
   p.w_f32 = n->w_dtype == FHOB_F32;
   p.rows = static_cast<int>(n->rows);

@@ -334,6 +334,8 @@ extern "C" int fhob_rotary(const FhobRotary* r, void* stream) {
     if (r->axis_of_pair[i] >= r->axes) return FHOB_ERR_ARG;
     p.axis[i] = r->axis_of_pair[i];
   }
+  if (reinterpret_cast<uintptr_t>(r->positions) % (r->positions_are_64_bit ? 8 : 4) || reinterpret_cast<uintptr_t>(r->frequencies) % (r->frequencies_are_64_bit ? 8 : 4))
+    return FHOB_ERR_ALIGN;
   p.positions = r->positions;
   p.pos_axis = r->pos_axis; p.pos_batch = r->pos_batch; p.pos_n = r->pos_n;
   p.frequencies = r->frequencies;

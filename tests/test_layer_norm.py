@@ -267,3 +267,24 @@ def test_c_refusals():
     assert lib.fhob_layer_norm_bwdbwd(problem(), 1024, 64, 0, 0, 0, 0, 2048, 4096, 8192, None) == 4
     assert lib.fhob_layer_norm_bwdbwd(problem(), None, 64, 0, 0, 0, 0, 2048, 4096, None, None) == 1
     assert lib.fhob_layer_norm_workspace_bytes(0) == 0 and lib.fhob_layer_norm_workspace_bytes(10) > 0
+
+
+def test_c_refuses_misplaced_vectors():
+    """Vectors and statistics of 4 bytes an element at addresses of 2, next to rows that may lie there."""
+    lib = _lib.load()
+
+    def problem(**over):
+        n = _lib.FhobLayerNorm()
+        n.rows, n.cols, n.dtype, n.w_dtype, n.x, n.x_row, n.mean, n.rstd, n.workspace, n.workspace_bytes = 4, 63, 0, 1, 258, 63, 512, 768, 4096, 1 << 30
+        for k, v in over.items():
+            setattr(n, k, v)
+        return C.byref(n)
+
+    for over in ({"w": 1026}, {"b": 1026}, {"mean": 514}, {"rstd": 770}):
+        assert lib.fhob_layer_norm(problem(**over), 2048, None) == 3, over
+    for dw, db in ((4098, None), (None, 4098)):
+        assert lib.fhob_layer_norm_backward(problem(), 1024, 63, 2048, dw, db, None) == 3
+    for vw, vb, dw2 in ((1026, None, None), (None, 1026, None), (None, None, 1026)):
+        assert lib.fhob_layer_norm_bwdbwd(problem(), 1024, 63, 0, 0, vw, vb, 2048, 4096, dw2, None) == 3
+    # 16-bit vectors may lie at addresses of 2, not of 1
+    assert lib.fhob_layer_norm(problem(w_dtype=0, w=1025), 2048, None) == 3

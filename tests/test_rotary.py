@@ -223,3 +223,15 @@ def test_structs_match_header():
         body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
         names = [re.sub(r"\[.*?\]", "", n).replace("*", "").split()[-1] for line in body.split(";") if line.strip() for n in line.split(",")]
         assert names == [f[0] for f in cls._fields_], cls.__name__
+
+
+def test_c_refuses_misplaced_vectors():
+    lib = _lib.load()
+    axes = (C.c_uint8 * 512)()
+    for positions, frequencies, wide in ((1026, 2048, 0), (1024, 2050, 0), (1028, 2048, 1), (1024, 2052, 1)):
+        r = _lib.FhobRotary()
+        r.dtype, r.tensors, r.batch, r.n, r.d, r.pairs, r.axes, r.axis_of_pair = 0, 1, 1, 4, 64, 32, 1, axes
+        setattr(r.tensor[0], "in", 256)
+        r.tensor[0].out, r.tensor[0].heads = 512, 1
+        r.positions, r.frequencies, r.positions_are_64_bit, r.frequencies_are_64_bit = positions, frequencies, wide, wide
+        assert lib.fhob_rotary(C.byref(r), None) == 3
