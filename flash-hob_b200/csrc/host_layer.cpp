@@ -177,13 +177,17 @@ struct Rows {
 Rows rows_of(const Tensor& x) {
   Rows r;
   const int64_t cols = x.size(-1);
-  if (x.dim() == 2 && (x.stride(1) == 1 || cols == 1)) {
-    r.t = x;
-    r.stride = x.size(0) > 1 ? x.stride(0) : cols;
-  } else {
-    r.t = x.contiguous();
-    r.stride = cols;
+  // the dims in front of the last, from the inside: one stride for all their rows?
+  bool one = x.stride(-1) == 1 || cols == 1;
+  int64_t inside = 0;   // rows of the dims seen so far
+  for (int64_t i = x.dim() - 2; i >= 0 && one; --i) {
+    if (x.size(i) == 1) continue;
+    if (!inside) r.stride = x.stride(i);
+    else one = x.stride(i) == r.stride * inside;
+    inside = (inside ? inside : 1) * x.size(i);
   }
+  r.t = one ? x : x.contiguous();
+  if (!one || !inside) r.stride = cols;
   return r;
 }
 

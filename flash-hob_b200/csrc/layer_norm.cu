@@ -677,9 +677,17 @@ int ln_run(const LnParams& p, const LnGrid& g, cudaStream_t s) {
     FHOB_CUDA_OK(launch_pdl(kernel, static_cast<unsigned>(g.blocks), kThreads, C::kSmem, 1, s, p));
     return FHOB_OK;
   };
-  if (g.lanes < 32) return go(std::integral_constant<int, 256>{}, std::true_type{});
-  if (g.threads == 256) return go(std::integral_constant<int, 256>{}, std::false_type{});
-  return g.threads == 512 ? go(std::integral_constant<int, 512>{}, std::false_type{}) : go(std::integral_constant<int, 1024>{}, std::false_type{});
+  // (what ln_grid does not ask for is not built)
+  constexpr bool kFew = NV * V == 8, kSecond = WHAT == kLnBwdbwd;   // 16 elements a thread in the double backward: long rows alone
+  if constexpr (kFew || !kSecond)
+    if (g.lanes < 32) return go(std::integral_constant<int, 256>{}, std::true_type{});
+  if constexpr (kSecond ? kFew : WHAT == kLnForward)
+    if (g.threads == 256) return go(std::integral_constant<int, 256>{}, std::false_type{});
+  if constexpr (!kFew || (kSecond && !kWide<T, V>))
+    if (g.threads == 1024) return go(std::integral_constant<int, 1024>{}, std::false_type{});
+  if constexpr (!kSecond || kFew || kWide<T, V>)
+    if (g.threads == 512) return go(std::integral_constant<int, 512>{}, std::false_type{});
+  return FHOB_ERR_SHAPE;
 }
 
 template <int WHAT, class T>

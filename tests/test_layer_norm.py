@@ -288,3 +288,21 @@ def test_c_refuses_misplaced_vectors():
         assert lib.fhob_layer_norm_bwdbwd(problem(), 1024, 63, 0, 0, vw, vb, 2048, 4096, dw2, None) == 3
     # 16-bit vectors may lie at addresses of 2, not of 1
     assert lib.fhob_layer_norm(problem(w_dtype=0, w=1025), 2048, None) == 3
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("view", ["slice", "one_row", "transposed", "expanded", "expanded_rows", "one_column", "one_batch"])
+def test_views_of_three_dims(view):
+    """The same bits as of a contiguous copy, whether the rows lie at one stride (read in place) or not (copied)."""
+    base = torch.randn(3, 5, 160, device="cuda", generator=torch.Generator("cuda").manual_seed(11)).bfloat16()
+    x = {"slice": base[..., 16:144], "one_row": base[:, 2:3, :128], "transposed": base.transpose(0, 1), "expanded": base[:1, :, :128].expand(4, 5, 128),
+         "expanded_rows": base[:, :1, :128].expand(3, 7, 128), "one_column": base[..., 3:4], "one_batch": base[1:2, 1:4, 8:]}[view]
+    cols = x.shape[-1]
+    w, b = (torch.randn(cols, device="cuda") for _ in range(2))
+    dy, v = (torch.randn(x.shape, device="cuda").bfloat16() for _ in range(2))
+    for got, want in ((fhob.layer_norm_forward(x, w, b), fhob.layer_norm_forward(x.contiguous(), w, b)),):
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+    _, mean, rstd = want
+    for got, want in ((fhob.layer_norm_backward(x, dy, w, mean, rstd), fhob.layer_norm_backward(x.contiguous(), dy, w, mean, rstd)),
+                      (fhob.layer_norm_bwdbwd(v, w, b, dy, x, w, mean, rstd), fhob.layer_norm_bwdbwd(v, w, b, dy, x.contiguous(), w, mean, rstd))):
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
