@@ -11,13 +11,13 @@
 //   terms do not cancel when v or g have a large common part.
 //
 // What bounds it: each matrix is read once and written once, so the memory.
-//  - A row belongs to a group: 2 to 32 lanes of a warp or 2 to 32 warps, 8 or 16 elements a lane.  It is in registers, in fp32,
+//  - A row belongs to a group: 2 to 32 lanes of a warp or 2 to 32 warps, 8 to 32 elements a lane.  It is in registers, in fp32,
 //    from its only load to its results; sums over it are shuffles, then, if the group has several warps, one exchange
 //    through shared memory per round.  Rounds: two in the forward (the variance is a sum of squares around the mean), one
 //    in the backward, two in the double backward.
 //  - Next to the memory comes the number of instructions: elements are converted once, the arithmetic is on packed pairs, and the
-//    vectors over the columns stay in registers.  (Converted where they are used, with scalar arithmetic, an element of the
-//    forward took 34 instructions, of the double backward 93; now 7 and 20.)
+//    vectors over the columns stay in registers.  (Converted where they are used, with scalar arithmetic, and without
+//    the copies below: 16384 x 2048 bf16 forward 42 us, backward 75, double backward 175; now 26, 43 and 85.)
 //  - What keeps the memory busy is the number of bytes on their way.  Rows come through a ring in shared memory, up to
 //    three rows ahead of the one in work, by asynchronous copies.  On the 16-byte grid a thread copies its own elements
 //    alone: it is the only one to read them, so nothing waits but for its own copies.
@@ -202,14 +202,17 @@ __device__ __forceinline__ void group_sum(float (&x)[N], const P& at, float* exc
   for (int i = 0; i < N; ++i) x[i] = __shfl_sync(kAll, y, i);
 }
 
-// How the three kernels are laid out: blocks of 256, 512 or 1024 threads, 512 threads an SM with 128 registers each (64 in blocks
-// of 1024, which only the longest rows take).
+// How the three kernels are laid out: blocks of 128 to 1024 threads, 512 threads an SM with 128 registers each (64 in blocks
+// of 1024, which only the longest rows take).  768 threads where less is kept of each, 384 where more is (see ln_grid).
 enum { kLnForward, kLnBackward, kLnBwdbwd };
-constexpr int ln_threads(int what, bool wide) { return what == kLnForward && wide ? 768 : 512; }   // of an SM
+constexpr int ln_threads(int what, bool wide, int each) {   // of an SM
+  if (what == kLnForward) return wide && each <= 16 ? 768 : 512;
+  return what == kLnBwdbwd && wide && each == 16 ? 384 : 512;
+}
 template <int WHAT, class T, int V, int NV, int THREADS, bool SUB>
 struct LnCfg {
   static constexpr int kMatrices = WHAT == kLnForward ? 1 : (WHAT == kLnBackward ? 2 : 3);
-  static constexpr int kBlocks = ln_threads(WHAT, kWide<T, V>) > THREADS ? ln_threads(WHAT, kWide<T, V>) / THREADS : 1;   // of an SM
+  static constexpr int kBlocks = ln_threads(WHAT, kWide<T, V>, NV * V) > THREADS ? ln_threads(WHAT, kWide<T, V>, NV * V) / THREADS : 1;   // of an SM
   // Bytes of a row of the ring.  Off the grid a row may start anywhere in a piece of 16 bytes: one more for each group (and a word
   // that the last pair of the last group looks into).
   static constexpr int kRow = THREADS * NV * V * static_cast<int>(sizeof(T)) + (kWide<T, V> ? 0 : 16 * THREADS / (SUB ? 2 : 32));
@@ -217,7 +220,7 @@ struct LnCfg {
   static constexpr int kStages = kFit > 4 ? 4 : kFit;                         // rows of the ring
   static constexpr int kExchange = 2 * LN_MAX_WARPS * 16;                     // bytes in front of it: two areas for the sums over a row
   static constexpr int kSmem = kExchange + kMatrices * kRow * kStages;
-  static constexpr bool kHold = WHAT != kLnBwdbwd || NV * V <= 8;             // vectors over the columns stay in registers
+  static constexpr bool kHold = WHAT != kLnBwdbwd || NV * V <= 8 || THREADS <= 256;   // vectors over the columns stay in registers
   static_assert(kStages >= 1, "a row of the ring");
   static_assert(WHAT == kLnForward || THREADS * NV * V * 4 <= kSmem - kExchange, "room for the sums over rows, see block_columns");
 };
@@ -640,25 +643,31 @@ struct LnGrid {
   int each, lanes, warps, threads, blocks;   // elements of a thread; of a group: lanes and warps; threads and blocks
 };
 constexpr int kSms = 148;
-constexpr int kLnMostBlocks = 2 * kSms;   // that leave sums over rows: of 256 threads or more, 512 threads an SM
+constexpr int kLnMostBlocks = 3 * kSms;   // that leave sums over rows, see ln_threads and ln_grid
 
-LnGrid ln_grid(int what, long long rows, int cols, bool wide) {
+LnGrid ln_grid(int what, long long rows, int cols, bool wide, bool bits16) {
   LnGrid g;
   g.wide = wide;
-  // 16 elements a thread.  8 in the double backward (there are more to keep of each), unless rows are long, and where there are
-  // too few rows to fill the GPU and a row's own time counts.
-  g.each = what == kLnBwdbwd ? (cols <= (wide ? 4096 : 8192) ? 8 : 16) : (rows <= kSms && cols <= 4096 ? 8 : 16);
+  // 16 elements a thread: what is done once a row and thread (exchanges, addresses) is shared by as many.  Where there are
+  // too few rows to fill the GPU a row's own time counts: 8.
+  g.each = rows <= kSms && cols <= 4096 ? 8 : 16;
+  // The forward keeps little of each: 32 (bf16, 2048 columns 27.8 -> 26.3 us, 8192 40 -> 29; fp32 8192 51 -> 50, but 2048 21.6 -> 22.5).
+  if (what == kLnForward && wide && cols >= (bits16 ? 1024 : 4097) && g.each == 16) g.each = 32;
+  // The double backward keeps much: 8.  16 with 384 threads an SM where rows of 16-bit elements are neither short nor long (512
+  // columns 77 -> 63 us, 2048 90 -> 85, 4096 107 -> 99; fp32 2048 61.9 -> 63.6), and for long ones, without the vectors over the columns.
+  if (what == kLnBwdbwd && cols <= (wide ? 4096 : 8192) && !(wide && bits16 && cols > 256 && rows > kSms)) g.each = 8;
   g.lanes = 32;
   while (g.lanes > 2 && g.lanes / 2 * g.each >= cols) g.lanes >>= 1;
   g.warps = 1;
   while (g.warps < LN_MAX_WARPS && g.warps * 32 * g.each < cols) g.warps <<= 1;
   // Larger blocks leave fewer sums over rows to add up (16384 x 2048 bf16, backward 44.2 -> 43.0 us), which in the double backward pays
-  // for rows of few warps only (512 columns 80 -> 77 us, 2048 90 -> 102).
-  const int least = what == kLnForward || g.lanes < 32 || (what == kLnBwdbwd && g.warps > 4) ? 256 : 512;
+  // for rows of few warps only (8 elements a thread, 512 columns 80 -> 77 us, 2048 90 -> 102).
+  const bool held = what == kLnBwdbwd && wide && g.each == 16 && cols <= 4096;
+  const int least = held ? 128 : (what == kLnForward || g.lanes < 32 || (what == kLnBwdbwd && g.warps > 4) ? 256 : 512);
   g.threads = g.warps * 32 > least ? g.warps * 32 : least;
   const int groups = g.threads / (g.warps * g.lanes);
   const long long wanted = (rows + groups - 1) / groups;
-  const int per_sm = ln_threads(what, wide) / g.threads;
+  const int per_sm = ln_threads(what, wide, g.each) / g.threads;
   const long long resident = static_cast<long long>(kSms) * (per_sm > 0 ? per_sm : 1);
   g.blocks = static_cast<int>(wanted < resident ? wanted : resident);
   return g;
@@ -670,29 +679,37 @@ int ln_run(const LnParams& p, const LnGrid& g, cudaStream_t s) {
     constexpr int kThreads = decltype(threads)::value;
     constexpr bool kSub = decltype(sub)::value;
     using C = LnCfg<WHAT, T, V, NV, kThreads, kSub>;
-    constexpr auto kernel = WHAT == kLnForward ? ln_forward_kernel<T, V, NV, kThreads, kSub>
-                                               : (WHAT == kLnBackward ? ln_backward_kernel<T, V, NV, kThreads, kSub> : ln_bwdbwd_kernel<T, V, NV, kThreads, kSub>);
+    constexpr auto kernel = [] {
+      if constexpr (WHAT == kLnForward) return ln_forward_kernel<T, V, NV, kThreads, kSub>;
+      else if constexpr (WHAT == kLnBackward) return ln_backward_kernel<T, V, NV, kThreads, kSub>;
+      else return ln_bwdbwd_kernel<T, V, NV, kThreads, kSub>;
+    }();
     const int st = allow_smem(kernel, C::kSmem);
     if (st != FHOB_OK) return st;
     FHOB_CUDA_OK(launch_pdl(kernel, static_cast<unsigned>(g.blocks), kThreads, C::kSmem, 1, s, p));
     return FHOB_OK;
   };
   // (what ln_grid does not ask for is not built)
-  constexpr bool kFew = NV * V == 8, kSecond = WHAT == kLnBwdbwd;   // 16 elements a thread in the double backward: long rows alone
-  if constexpr (kFew || !kSecond)
+  constexpr int kEach = NV * V;
+  constexpr bool kGrid = kWide<T, V>, kSecond = WHAT == kLnBwdbwd, kHeld = kSecond && kGrid && sizeof(T) == 2 && kEach == 16;
+  if constexpr (kEach == 8 || (kEach == 16 && !kSecond))
     if (g.lanes < 32) return go(std::integral_constant<int, 256>{}, std::true_type{});
-  if constexpr (kSecond ? kFew : WHAT == kLnForward)
+  if constexpr (kHeld)
+    if (g.threads == 128) return go(std::integral_constant<int, 128>{}, std::false_type{});
+  if constexpr (WHAT == kLnForward || kHeld || (kSecond && kEach == 8))
     if (g.threads == 256) return go(std::integral_constant<int, 256>{}, std::false_type{});
-  if constexpr (!kFew || (kSecond && !kWide<T, V>))
-    if (g.threads == 1024) return go(std::integral_constant<int, 1024>{}, std::false_type{});
-  if constexpr (!kSecond || kFew || kWide<T, V>)
+  if constexpr (!(kEach == 16 && ((WHAT == kLnForward && kGrid) || (kSecond && !kGrid))))
     if (g.threads == 512) return go(std::integral_constant<int, 512>{}, std::false_type{});
+  if constexpr (WHAT == kLnForward ? kEach == 16 && !kGrid : (kEach == 16 || (kSecond && !kGrid)))
+    if (g.threads == 1024) return go(std::integral_constant<int, 1024>{}, std::false_type{});
   return FHOB_ERR_SHAPE;
 }
 
 template <int WHAT, class T>
 int ln_pick(const LnParams& p, const LnGrid& g, cudaStream_t s) {
   constexpr int kPiece = 16 / sizeof(T);
+  if constexpr (WHAT == kLnForward)
+    if (g.wide && g.each == 32) return ln_run<WHAT, T, kPiece, 32 / kPiece>(p, g, s);
   if (g.wide) return g.each == 8 ? ln_run<WHAT, T, kPiece, 8 / kPiece>(p, g, s) : ln_run<WHAT, T, kPiece, 16 / kPiece>(p, g, s);
   return g.each == 8 ? ln_run<WHAT, T, 2, 4>(p, g, s) : ln_run<WHAT, T, 2, 8>(p, g, s);
 }
@@ -725,7 +742,7 @@ int ln_call(const FhobLayerNorm* n, LnParams& p, void* dw, void* db, cudaStream_
   p.cols = n->cols;
   p.eps = n->eps;
   p.inv_cols = 1.f / static_cast<float>(n->cols);
-  const LnGrid g = ln_grid(WHAT, n->rows, n->cols, together % 16 == 0);
+  const LnGrid g = ln_grid(WHAT, n->rows, n->cols, together % 16 == 0, es == 2);
   p.warps = g.warps;
   p.lanes = g.lanes;
   if (dw || db) {

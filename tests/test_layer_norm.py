@@ -1,6 +1,6 @@
 """fhob.layer_norm and its derivatives against autograd of the definition in 64 bits.
 
-Error bounds.  A row's sums have at most 16 terms in a thread and ten additions between threads: 2^-24 * 26 of the sum of
+Error bounds.  A row's sums have at most 16 terms one behind the other in a thread and ten additions between threads: 2^-24 * 26 of the sum of
 the terms' sizes.  In the elements of the results these sums come with factors of about their own size, so 64 * 2^-24 of a
 row's scale (times 1 + |mean| rstd where the mean is large against the deviation: the subtraction keeps the
 absolute error of the mean) covers the fp32 arithmetic; storing rounds by at most half a step of the type.
@@ -57,13 +57,16 @@ def columns_close(got, ref, sizes, rows, spread=1.0):
     assert bool(((got.double() - ref).abs() <= bound).all()), float(((got.double() - ref).abs() / bound).max())
 
 
+# rows of every way to cut them up, on both sides of where it changes
+EDGES = [(149, c, d) for d in ("bf16", "fp32") for c in (248, 256, 257, 264, 512, 520, 1016, 1024, 1032, 2049, 2056, 4096, 4097, 4104, 8191, 8192, 8200)]
+EDGES += [(148, c, "fp16") for c in (256, 264, 1024, 2048, 4095, 4096, 4104, 8200)]
 CASES = [(1, 1, "fp32"), (1, 16, "bf16"), (2, 3, "bf16"), (7, 1001, "fp16"), (33, 256, "fp32"), (64, 2048, "bf16"), (300, 1000, "fp16"), (5, 1026, "bf16"),
          (1500, 128, "bf16"), (2000, 2048, "bf16"), (700, 4096, "fp32"), (150, 8192, "bf16"), (150, 8192, "fp32"), (149, 16384, "bf16"), (3, 16384, "fp32"),
          (200, 16383, "bf16"), (40, 12001, "fp32"), (1000, 130, "fp32"), (4099, 514, "fp16"), (170, 6002, "bf16")]
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows,cols,dtype", CASES)
+@pytest.mark.parametrize("rows,cols,dtype", CASES + EDGES)
 def test_all_directions(rows, cols, dtype):
     eps = 1e-5 if cols > 1 else 0.5
     t = make(rows, cols, dtype, seed=cols)
