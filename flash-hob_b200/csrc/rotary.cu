@@ -15,7 +15,8 @@
 // as many as a dozen heads' rows if every thread works out its own.  A block takes a few tokens in all heads of all tensors.
 // Its threads work out the angles of these tokens together, into shared memory; then a thread owns four pairs
 // of one token's rows (a warp covers whole rows) and passes over heads, four in flight, the first of them while
-// the angles are worked out.
+// the angles are worked out.  32 heads N = 8192 D = 128 bf16: 46 us, 5.8 TB/s (55 when every thread worked out its own angles);
+// a token of 8 x 32 heads 3.2 us.
 #include "fhob_common.cuh"
 #include "tc_common.cuh"
 

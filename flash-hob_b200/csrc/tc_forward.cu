@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
   auto m_of = [&](int x) { return (group * p.q_tiles + x) * BM; };
   auto live = [&](int x) { return x < p.q_tiles && m_of(x) < p.n_q; };
   // Steps t of the walk over the key tiles; query tile x takes part in those that are active(x, t).
-  //  Without first keys behind the window (SINKS false): step t is key tile t, query tile x has begin[x] .. end[x] - 1.
+  //  Without first keys behind the window (SINKS false, kernels of their own: sharing one cost them 8 %): step t is key tile t, query tile x has begin[x] .. end[x] - 1.
   //  With them: n_first steps for their tiles (both query tiles take those of the later one), then the window's, key tile
   //  w_begin + t - n_first.
   int begin[2], end[2], n_first = 0;
