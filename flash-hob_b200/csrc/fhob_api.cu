@@ -96,7 +96,9 @@ __global__ void row_stats_kernel(const float* k1, const float* ndd, const float*
   if (b_out) b_out[i] = -(k23[v] + k1[v] * ndd[v]);
 }
 
-// One block a first key of a head: its rows of sums, of the near queries and of the far ones' parts, in that order.
+// One block a first key of a head: adds up its rows of sums, of the near queries and of the far ones' parts.  A thread a column
+// (there are at most 256) and every fourth row, so that all loads are on their way at once; then the four sums, in order.
+constexpr int kFirstCols = 256, kFirstShares = 4;
 template <typename T>
 __global__ void first_keys_kernel(const float* sums, int parts, int sinks, int d, int d_v, int n_k, float scale, T* out0, T* out1) {
   pdl_wait();
@@ -104,10 +106,18 @@ __global__ void first_keys_kernel(const float* sums, int parts, int sinks, int d
   const int head = blockIdx.x / sinks, row = blockIdx.x - head * sinks, cols = d + d_v;
   const size_t slot = static_cast<size_t>(sinks) * cols;
   const float* from = sums + (static_cast<size_t>(head) * (parts + 1) * sinks + row) * cols;
-  for (int c = threadIdx.x; c < cols; c += blockDim.x) {
-    float total = 0.f;
+  const int c = threadIdx.x % kFirstCols, share = threadIdx.x / kFirstCols;
+  __shared__ float shares[kFirstShares][kFirstCols];
+  float total = 0.f;
+  if (c < cols) {
 #pragma unroll 8
-    for (int i = 0; i <= parts; ++i) total += from[i * slot + c];
+    for (int i = share; i <= parts; i += kFirstShares) total += from[i * slot + c];
+  }
+  shares[share][c] = total;
+  __syncthreads();
+  if (share == 0 && c < cols) {
+#pragma unroll
+    for (int i = 1; i < kFirstShares; ++i) total += shares[i][c];
     const size_t at = static_cast<size_t>(head) * n_k + row;
     if (c < d) out0[at * d + c] = static_cast<T>(total * scale);
     else out1[at * d_v + c - d] = static_cast<T>(total);
@@ -261,7 +271,7 @@ int finish_first_keys(const Problem& p, void* out0, void* out1, cudaStream_t s) 
   const int d_v = head_dim_v(p);
   auto go = [&](auto type) {
     using T = decltype(type);
-    return launch_pdl(first_keys_kernel<T>, static_cast<unsigned>(blocks), 128, 0, 1, s, static_cast<const float*>(p.far_sums), p.far_parts, p.sinks, p.d,
+    return launch_pdl(first_keys_kernel<T>, static_cast<unsigned>(blocks), kFirstCols * kFirstShares, 0, 1, s, static_cast<const float*>(p.far_sums), p.far_parts, p.sinks, p.d,
                       d_v, p.n_k, p.scale, static_cast<T*>(out0), static_cast<T*>(out1));
   };
   FHOB_CUDA_OK(p.dtype == FHOB_BF16 ? go(__nv_bfloat16{}) : (p.dtype == FHOB_F16 ? go(__half{}) : go(float{})));

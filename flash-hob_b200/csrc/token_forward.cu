@@ -1,8 +1,8 @@
-// Forward of a few queries (one token a sequence, or a handful) against a window and first keys: O and the logsumexp.
+// Forward of one or two queries (a token that is answered with) against a window and first keys: O and the logsumexp.
 //
 //   s_j = scale q . k_j,  O = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),  L = m + log sum_j exp(s_j - m)
 //
-// What bounds it: every visible key and value is read once for up to eight queries, so the memory: 128 heads of one query,
+// What bounds it: every visible key and value is read once for the one or two queries, so the memory: 128 heads of one query,
 // W = 1024 and 4 first keys, D = 128 read 67 MB.  The tensor-core forward has 128-row query tiles and goes through a head
 // in one CTA, tile after tile: 26 us there.  Here 15.6 us (4.3 TB/s):
 //  - eight lanes read one key's row, one, two or four times 16 bytes a lane: a product takes three shuffles.  Each such group goes
