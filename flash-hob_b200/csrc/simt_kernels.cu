@@ -759,8 +759,8 @@ constexpr SplitCost kSimtCost = {1.f, 0.5f, 1.f / 16};
 
 PairGrid modes_grid(const Problem& p, bool q_side, bool k_side) {
   const int tiles_q = (p.n_q + OM - 1) / OM, tiles_k = (p.n_k + OM - 1) / OM;
-  return pair_grid(q_side ? static_cast<long long>(tiles_q) * p.bh : 0, split_parts(tiles_q, longest(true, p.n_k, ON, OM, p.window, p.sinks), kSimtCost),
-                   k_side ? static_cast<long long>(tiles_k) * p.bh : 0, split_parts(tiles_k, longest(false, p.n_q, ON, OM, p.window, p.sinks), kSimtCost));
+  const Parts parts = item_parts(p, OM, ON, kSimtCost);
+  return pair_grid(q_side ? static_cast<long long>(tiles_q) * p.bh : 0, parts.q, k_side ? static_cast<long long>(tiles_k) * p.bh : 0, parts.k);
 }
 
 template <typename T, int MODE_Q, int MODE_K>

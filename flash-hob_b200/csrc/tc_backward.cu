@@ -549,18 +549,19 @@ int bw_launch(const Problem& p, void* dq, void* dk, void* dv, cudaStream_t s) {
   tp.items_k = tp.tiles_k * p.bh;
   const int st = allow_smem(kernel, kSmem);
   if (st != FHOB_OK) return st;
+  const Parts parts = tc_parts(p);
   auto go = [&](bool q_side, bool k_side) -> int {
-    const PairGrid g = pair_grid(q_side ? tp.items_q : 0, tc_parts(true, p), k_side ? tp.items_k : 0, tc_parts(false, p));
+    const PairGrid g = pair_grid(q_side ? tp.items_q : 0, parts.q, k_side ? tp.items_k : 0, parts.k);
     if (g.blocks > 0x7fffffffLL) return FHOB_ERR_SHAPE;
     tp.split_q = g.split_q; tp.split_k = g.split_k;
     tp.cluster = g.cluster;
     tp.q_blocks = g.q_blocks;
-    tp.far = far_work(p, !k_side || tc_parts(true, p) > 1 || tc_parts(false, p) > 1, BM);
+    tp.far = far_work(p, !k_side || parts.q > 1 || parts.k > 1, BM);
     if (g.blocks + tp.far.blocks > 0x7fffffffLL) return FHOB_ERR_SHAPE;
     FHOB_CUDA_OK(launch_pdl(kernel, static_cast<unsigned>(g.blocks + tp.far.blocks), NTHREADS, kSmem, g.cluster, s, tp));
     return tp.far.sums ? finish_first_keys(p, dk, dv, s) : FHOB_OK;
   };
-  if (!launch_apart(pair_grid(tp.items_q, tc_parts(true, p), tp.items_k, tc_parts(false, p)))) return go(true, true);
+  if (!launch_apart(pair_grid(tp.items_q, parts.q, tp.items_k, parts.k))) return go(true, true);
   const int first = go(true, false);
   return first != FHOB_OK ? first : go(false, true);
 }

@@ -638,7 +638,7 @@ int fw_launch(const Problem& p, void* o_out, float* lse_out, int* status, cudaSt
   const int tiles = (p.n_q + BM - 1) / BM;
   if (static_cast<long long>(tiles) * p.bh > 0x7fffffffLL) return FHOB_ERR_SHAPE;
   // A head of one query tile may split its keys (a second tile would cost the parts more than they save).
-  tp.split = tiles == 1 ? tc_parts(true, p) : 1;
+  tp.split = tiles == 1 ? tc_parts(p).q : 1;
   // Two query tiles a CTA hide each other's latency and share K and V; a tile takes as long alone, so
   // when single tiles fit the GPU at once, a CTA has one.  (The bits are the same.)
   tp.q_tiles = tiles == 1 || static_cast<long long>(tiles) * p.bh <= sm_count() ? 1 : 2;

@@ -1145,7 +1145,7 @@ template <int PASS, int DQK, int DV, int BN, int FUSED, bool F16, bool SPLIT>
 int launch_pass(const Problem& p, TcParams& tp, cudaStream_t s) {
   constexpr auto kernel = tc_pass_kernel<PASS, DQK, DV, BN, FUSED, F16, SPLIT>;
   constexpr int kSmem = Cfg<PASS, DQK, DV, BN>::SMEM_BYTES;
-  if (FUSED) tp.split_q = tp.cluster = tc_parts(true, p);
+  if (FUSED) tp.split_q = tp.cluster = tc_parts(p).q;
   return launch(kernel, tp, static_cast<long long>(tp.items_q) * tp.split_q, kSmem, s);
 }
 
@@ -1155,7 +1155,8 @@ int launch_34(const Problem& p, TcParams& tp, bool pass3, bool pass4, cudaStream
   constexpr auto kernel = tc_pass34_kernel<DQK, DV, F16, SPLIT>;
   constexpr int kSmem3 = Cfg<3, DQK, DV, 64>::SMEM_BYTES, kSmem4 = Cfg<4, DQK, DV, 64>::SMEM_BYTES;
   constexpr int kSmem = kSmem3 > kSmem4 ? kSmem3 : kSmem4;
-  const PairGrid g = pair_grid(pass3 ? tp.items_q : 0, tc_parts(true, p), pass4 ? tp.items_k : 0, tc_parts(false, p));
+  const Parts parts = tc_parts(p);
+  const PairGrid g = pair_grid(pass3 ? tp.items_q : 0, parts.q, pass4 ? tp.items_k : 0, parts.k);
   if (pass3 && pass4 && launch_apart(g)) {
     const int st = launch_34<DQK, DV, F16, SPLIT>(p, tp, true, false, s);
     return st != FHOB_OK ? st : launch_34<DQK, DV, F16, SPLIT>(p, tp, false, true, s);
@@ -1163,7 +1164,7 @@ int launch_34(const Problem& p, TcParams& tp, bool pass3, bool pass4, cudaStream
   tp.split_q = g.split_q; tp.split_k = g.split_k;
   tp.cluster = g.cluster;
   tp.q_blocks = g.q_blocks;
-  tp.far = far_work(p, !pass4 || tc_parts(true, p) > 1 || tc_parts(false, p) > 1, BM);
+  tp.far = far_work(p, !pass4 || parts.q > 1 || parts.k > 1, BM);
   const int st = launch(kernel, tp, g.blocks + tp.far.blocks, kSmem, s);
   return st == FHOB_OK && tp.far.sums ? finish_first_keys(p, p.dk2, p.dv2, s) : st;
 }
@@ -1255,7 +1256,8 @@ int tc_split_inputs(const FhobProblem& p, cudaStream_t s, int which) {
 int tc_grid(const Problem& p, PairGrid* g) {
   if (!tc_items_fit(p)) return FHOB_ERR_SHAPE;
   const int tq = (p.n_q + BM - 1) / BM, tk = (p.n_k + BM - 1) / BM;
-  *g = pair_grid(tq * p.bh, tc_parts(true, p), tk * p.bh, tc_parts(false, p));
+  const Parts parts = tc_parts(p);
+  *g = pair_grid(tq * p.bh, parts.q, tk * p.bh, parts.k);
   return g->blocks > 0x7fffffffLL ? FHOB_ERR_SHAPE : FHOB_OK;
 }
 
