@@ -288,12 +288,13 @@ int rotary_launch(const FhobRotary& r, RoParams& p, cudaStream_t s) {
     constexpr auto kernel = rotary_kernel<T, P, decltype(neighbours)::value>;
     const int pieces = (r.pairs + p.tail) / P, all = p.heads[0] + p.heads[1];
     p.per_row = pieces < RO_THREADS ? pieces : RO_THREADS;
-    // A block works on `copies` heads of its tokens at once: eight or so, four heads in flight each, and more where the tokens
-    // are too few to fill the GPU.
+    // A block works on `copies` heads of its tokens at once, four heads in flight each: up to 16 heads a copy (32 + 1 heads
+    // N = 8192 D = 128 with 8 32.1 us, with 16 26.8), 8 by itself (8 + 8 heads with 16 52.5 us, with 8 48.6), and fewer where the tokens are too
+    // few to fill the GPU.  (The angle of a pair from positions brought into shared memory first: 1 + 1 heads 192 -> 147 us, but 16 + 16 46 -> 48.)
     const int most = RO_THREADS / p.per_row;
     p.block_tokens = most;
     auto blocks = [&] { return (p.tokens + p.block_tokens - 1) / p.block_tokens; };
-    while (p.block_tokens > 1 && (p.block_tokens * r.pairs > RO_ANGLES || (all + most / p.block_tokens - 1) / (most / p.block_tokens) > 8 || blocks() < 4LL * sm_count()) &&
+    while (p.block_tokens > 1 && (p.block_tokens * r.pairs > RO_ANGLES || (all + most / p.block_tokens - 1) / (most / p.block_tokens) > (p.block_tokens == most ? 8 : 16) || blocks() < 4LL * sm_count()) &&
            (p.block_tokens * r.pairs > RO_ANGLES || most / (p.block_tokens / 2) <= all))
       p.block_tokens >>= 1;
     p.copies = most / p.block_tokens;
