@@ -134,7 +134,7 @@ inline SplitBuffers split_buffers(const FhobProblem& p) {
 __host__ __device__ inline bool pair_visible(int qi, int kj, int off, int causal, int window, int sinks) {
   if (!causal) return true;
   const int dist = qi + off - kj;
-  return dist >= 0 && (window <= 0 || dist < window || kj < sinks);
+  return dist >= 0 && (window <= 0 || dist < window || (sinks > 0 && kj < sinks));
 }
 
 // Range [t_begin, t_end) of streamed tiles (tn rows each, n_strm rows in all) that can hold a

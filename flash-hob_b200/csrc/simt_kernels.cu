@@ -205,9 +205,11 @@ __device__ __forceinline__ TileList simt_tiles(bool q_stationary, int m0, int ti
   return list;
 }
 
-// `far`: a key-tiled pass over a part of the queries that see first keys behind their window.
-template <typename T, int MODE>
-__device__ __forceinline__ void simt_body(const SimtParams& p, int block, bool far) {
+// SINKS: with first keys.  (Kernels of their own: sharing one cost those without them 2 %.)  `far`: a key-tiled pass over a
+// part of the queries that see first keys behind their window.
+template <typename T, int MODE, bool SINKS>
+__device__ __forceinline__ void simt_body(const SimtParams& p, int block, bool is_far) {
+  const bool far = SINKS && is_far;
   using C = Tiles<MODE>;
   constexpr bool kQStat = C::kQStat, kFirst = C::kFirst;
   extern __shared__ float smem[];
@@ -270,9 +272,15 @@ __device__ __forceinline__ void simt_body(const SimtParams& p, int block, bool f
 #pragma unroll
     for (int j = 0; j < 4; ++j) out[i][j] = make_float2(0.f, 0.f);
 
-  const int key_sinks = !kQStat && p.far.sums ? 0 : p.sinks;   // first keys whose far queries are among this CTA's
-  TileList list = simt_tiles(kQStat, m0, ON, n_strm, p, key_sinks);
-  int t_begin = 0, t_end = list.count;
+  const int key_sinks = !SINKS || (!kQStat && p.far.sums) ? 0 : p.sinks;   // first keys whose far queries are among this CTA's
+  TileList list = {};
+  int t_begin = 0, t_end;
+  if constexpr (SINKS) {
+    list = simt_tiles(kQStat, m0, ON, n_strm, p, key_sinks);
+    t_end = list.count;
+  } else {
+    visible_tiles(kQStat, m0, OM, ON, n_strm, off, p.causal, p.window, t_begin, t_end);
+  }
   if (split > 1) split_range(begin_part, split, t_begin, t_end);
   if (far) {
     far_tiles(m0, ON, p.n_q, off, p.window, begin_part, p.far.parts, t_begin, t_end);
@@ -282,7 +290,7 @@ __device__ __forceinline__ void simt_body(const SimtParams& p, int block, bool f
   const float sl2 = p.scale * kLog2e;
 
   for (int t = t_begin; t < t_end; ++t) {
-    const int n0 = list.tile(t) * ON;
+    const int n0 = (SINKS ? list.tile(t) : t) * ON;
     __syncthreads();   // the previous step has read its tiles
     load_side(strm, !kQStat, n0, ON);
     if (!kQStat && threadIdx.x < ON) {
@@ -446,7 +454,7 @@ __device__ __forceinline__ void simt_body(const SimtParams& p, int block, bool f
   // Worked out again from the block number: kept in registers through the loop, these cost spills in it.
   uint32_t block_again;
   asm volatile("mov.u32 %0, %%ctaid.x;" : "=r"(block_again));
-  if (!kQStat && p.far.sums && m0 < p.sinks) {
+  if (SINKS && !kQStat && p.far.sums && m0 < p.sinks) {
     // first keys: rows of fp32 sums, added up with the other parts
     const int slot = block_again < static_cast<uint32_t>(p.far.blocks) ? 1 + static_cast<int>(block_again % p.far.parts) : 0;
     const int cols = group == 0 ? d : dv, col = 4 * cx;
@@ -460,7 +468,7 @@ __device__ __forceinline__ void simt_body(const SimtParams& p, int block, bool f
     }
     if (slot > 0) return;   // (no clusters in such a launch)
   }
-  block_again -= p.far.blocks + (kQStat ? 0 : p.q_blocks);
+  block_again -= (SINKS ? p.far.blocks : 0) + (kQStat ? 0 : p.q_blocks);
   const bool live = block_again / split < static_cast<uint32_t>(kQStat ? p.items_q : p.items_k);
   const int part = static_cast<int>(block_again % split);
 
@@ -494,7 +502,7 @@ __device__ __forceinline__ void simt_body(const SimtParams& p, int block, bool f
         continue;
       }
       const int r = m0 + 8 * ry + i;
-      if (!live || r >= n_stat || (!kQStat && p.far.sums && r < p.sinks)) continue;
+      if (!live || r >= n_stat || (SINKS && !kQStat && p.far.sums && r < p.sinks)) continue;
       const size_t at = head + static_cast<size_t>(r) * cols + col;
       if (col < cols) store4<T>(first ? base0 : base1, at, out[i][0], out[i][1], mul);
       if (MODE != 5 && col + 64 < cols) store4<T>(first ? base0 : base1, at + 64, out[i][2], out[i][3], mul);
@@ -523,13 +531,13 @@ __device__ __forceinline__ void simt_body(const SimtParams& p, int block, bool f
 }
 
 // MODE_Q on the first q_blocks CTAs, MODE_K (if not 0) on the others
-template <typename T, int MODE_Q, int MODE_K>
+template <typename T, int MODE_Q, int MODE_K, bool SINKS>
 __global__ void __launch_bounds__(NT, 1) simt_pass_kernel(const __grid_constant__ SimtParams p) {
   pdl_wait();
   if (threadIdx.x == 0) pdl_launch_dependents();
-  const int block = static_cast<int>(blockIdx.x) - p.far.blocks;
-  if (block >= 0 && block < p.q_blocks) simt_body<T, MODE_Q>(p, block, false);
-  else if constexpr (MODE_K != 0) simt_body<T, MODE_K>(p, block < 0 ? blockIdx.x : block - p.q_blocks, block < 0);
+  const int block = static_cast<int>(blockIdx.x) - (SINKS ? p.far.blocks : 0);
+  if ((!SINKS || block >= 0) && block < p.q_blocks) simt_body<T, MODE_Q, SINKS>(p, block, false);
+  else if constexpr (MODE_K != 0) simt_body<T, MODE_K, SINKS>(p, SINKS && block < 0 ? blockIdx.x : block - p.q_blocks, SINKS && block < 0);
 }
 
 // O(N)-memory forward: online softmax.  A CTA owns OM = 64 queries and streams FN = 128 keys; a warp owns eight
@@ -561,7 +569,7 @@ __device__ __forceinline__ void load_rows_any(float* tile, const void* src, size
 __device__ __forceinline__ void loads_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void loads_landed_but_last() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
 
-template <typename T>
+template <typename T, bool SINKS>
 __global__ void __launch_bounds__(NT, 1) simt_forward_kernel(const __grid_constant__ SimtParams p, void* o_out, float* lse_out, int* status, bool vec) {
   pdl_wait();
   if (threadIdx.x == 0) {
@@ -580,8 +588,15 @@ __global__ void __launch_bounds__(NT, 1) simt_forward_kernel(const __grid_consta
   const size_t qoff = static_cast<size_t>(bh) * p.n_q * d, ooff = static_cast<size_t>(bh) * p.n_q * dv;
   const size_t koff = static_cast<size_t>(bh) * p.n_k * d, voff = static_cast<size_t>(bh) * p.n_k * dv;
   const int off = p.n_k - p.n_q;
-  const TileList list = simt_tiles(true, m0, FN, p.n_k, p, p.sinks);
-  int t_begin = 0, t_end = list.count;
+  TileList list = {};
+  int t_begin = 0, t_end;
+  if constexpr (SINKS) {
+    list = simt_tiles(true, m0, FN, p.n_k, p, p.sinks);
+    t_end = list.count;
+  } else {
+    visible_tiles(true, m0, OM, FN, p.n_k, off, p.causal, p.window, t_begin, t_end);
+  }
+  auto key_tile = [&](int t) { return SINKS ? list.tile(t) : t; };
   if (split > 1) split_range(part, split, t_begin, t_end);
   if (!live) t_end = t_begin;
   const float sl2 = p.scale * kLog2e;
@@ -595,11 +610,11 @@ __global__ void __launch_bounds__(NT, 1) simt_forward_kernel(const __grid_consta
     acc[i][0] = acc[i][1] = make_float2(0.f, 0.f);
   }
   load_rows_any<T>(qs, p.q, qoff, m0, OM, p.n_q, d, vec);
-  if (t_begin < t_end) load_rows_any<T>(ks, p.k, koff, list.tile(t_begin) * FN, FN, p.n_k, d, vec);
+  if (t_begin < t_end) load_rows_any<T>(ks, p.k, koff, key_tile(t_begin) * FN, FN, p.n_k, d, vec);
   loads_commit();
 
   for (int t = t_begin; t < t_end; ++t) {
-    const int n0 = list.tile(t) * FN;
+    const int n0 = key_tile(t) * FN;
     if (o_out) load_rows_any<T>(vs, p.v, voff, n0, FN, p.n_k, dv, vec);
     loads_commit();
     loads_landed_but_last();
@@ -624,7 +639,7 @@ __global__ void __launch_bounds__(NT, 1) simt_forward_kernel(const __grid_consta
       }
     }
     __syncthreads();   // K has been read
-    if (t + 1 < t_end) load_rows_any<T>(ks, p.k, koff, list.tile(t + 1) * FN, FN, p.n_k, d, vec);
+    if (t + 1 < t_end) load_rows_any<T>(ks, p.k, koff, key_tile(t + 1) * FN, FN, p.n_k, d, vec);
     loads_commit();
 
     const bool masked = n0 + FN > p.n_k || (p.causal && (n0 + FN - 1 > m0 + off || (p.window > 0 && m0 + OM - 1 + off - n0 >= p.window)));
@@ -635,7 +650,7 @@ __global__ void __launch_bounds__(NT, 1) simt_forward_kernel(const __grid_consta
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int c = n0 + lane + 32 * j;
-        const bool ok = !masked || (c < p.n_k && pair_visible(row0 + i, c, off, p.causal, p.window, p.sinks));
+        const bool ok = !masked || (c < p.n_k && pair_visible(row0 + i, c, off, p.causal, p.window, SINKS ? p.sinks : 0));
         sv[j] = ok ? (s[i][j].x + s[i][j].y) * sl2 : -INFINITY;
         mx = fmaxf(mx, sv[j]);
       }
@@ -765,7 +780,7 @@ PairGrid modes_grid(const Problem& p, bool q_side, bool k_side) {
 
 template <typename T, int MODE_Q, int MODE_K>
 int launch_modes(const Problem& problem, SimtParams& p, bool q_side, bool k_side, cudaStream_t st) {
-  constexpr auto kernel = simt_pass_kernel<T, MODE_Q, MODE_K>;
+  const auto kernel = problem.sinks > 0 ? simt_pass_kernel<T, MODE_Q, MODE_K, true> : simt_pass_kernel<T, MODE_Q, MODE_K, false>;
   constexpr int kQ = Tiles<MODE_Q>::SMEM_BYTES, kK = Tiles<MODE_K ? MODE_K : MODE_Q>::SMEM_BYTES, kSmem = kQ > kK ? kQ : kK;
   const int ok = allow_smem(kernel, kSmem);
   if (ok != FHOB_OK) return ok;
@@ -806,7 +821,7 @@ int launch_backward(const Problem& p, void* dq, void* dk, void* dv, cudaStream_t
 // The forward reads rows element by element if they are not whole, aligned 16-byte pieces.
 template <typename T>
 int launch_forward(const Problem& p, void* o_out, float* lse_out, int* status, cudaStream_t st) {
-  constexpr auto kernel = simt_forward_kernel<T>;
+  const auto kernel = p.sinks > 0 ? simt_forward_kernel<T, true> : simt_forward_kernel<T, false>;
   const int ok = allow_smem(kernel, kForwardSmem);
   if (ok != FHOB_OK) return ok;
   SimtParams s = make_params(p);

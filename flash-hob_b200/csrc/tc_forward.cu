@@ -342,22 +342,30 @@ __global__ void __launch_bounds__(FW_THREADS, 1) fw_kernel(const __grid_constant
         if (it + 1 == steps(x)) umma_commit(&bars->out_full[x]);
         if (x == 1 || !active(1, t)) umma_commit(&bars->kv_free[slot]);
       };
+      // (unrolled over the query tiles with first keys, where telling the steps apart takes longer)
+      auto both = [&](auto&& f) {
+        if constexpr (SINKS) {
+          f(0);
+          f(1);
+        } else {
+          for (int x = 0; ok && x < 2; ++x) f(x);
+        }
+      };
       if (OUT) {
         for (int t = t_begin; ok && t < t_begin + kStages; ++t)
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
+          both([&](int x) {
             if (ok && active(x, t)) scores(x, t);
+          });
         for (int t = t_begin; ok && t < t_end; ++t)
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
+          both([&](int x) {
             if (ok && active(x, t)) output(x, t);
             if (ok && active(x, t + kStages)) scores(x, t + kStages);
-          }
+          });
       } else {
         for (int t = t_begin; ok && t < t_end; ++t)
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
+          both([&](int x) {
             if (ok && active(x, t)) scores(x, t);
+          });
       }
       if (!ok) {
         // abort path: no tcgen05.mma may still be reading shared memory or TMEM at exit
