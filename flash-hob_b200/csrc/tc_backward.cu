@@ -102,10 +102,11 @@ __device__ __forceinline__ void bw_split_pack(float x, float y, uint32_t& hi, ui
   lo = pack_bf16(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xffff0000u));
 }
 
-// One half over one 128-row tile of one head; `block` numbers the (head, tile, part) triples.  `far`: BK over a part of the
+// One half over one 128-row tile of one head; `block` numbers the (head, tile, part) triples.  SINKS: with first keys.  `far`: BK over a part of the
 // queries that see first keys behind their window.
-template <bool KSIDE, int DQK, int DV, bool F16, bool SPLIT>
-__device__ __forceinline__ void bw_body(const BwParams& p, int block, bool far) {
+template <bool KSIDE, int DQK, int DV, bool F16, bool SPLIT, bool SINKS>
+__device__ __forceinline__ void bw_body(const BwParams& p, int block, bool is_far) {
+  const bool far = SINKS && is_far;
   using C = BwCfg<KSIDE, DQK, DV, SPLIT>;
   static_assert(!SPLIT || (DQK == 128 && DV == 128 && !F16), "split fp32 operands are [hi(64) | lo(64)] bf16 rows");
   constexpr int BN = C::BN, CPT = BN / 2;   // CPT: columns of a score tile per elementwise thread
@@ -128,9 +129,18 @@ __device__ __forceinline__ void bw_body(const BwParams& p, int block, bool far) 
   const int m0 = tile * BM;
   const int n_stat = KSIDE ? p.n_k : p.n_q, n_strm = KSIDE ? p.n_q : p.n_k;
   const int off = p.n_k - p.n_q;
-  const int key_sinks = KSIDE && p.far.sums ? 0 : p.sinks;   // first keys whose far queries are among this CTA's
-  TileList list = streamed_tiles(!KSIDE, m0, BM, BN, n_strm, off, p.causal, p.window, key_sinks);
-  int t_begin = 0, t_end = list.count;
+  const int sinks = SINKS ? p.sinks : 0;
+  const bool apart = SINKS && KSIDE && p.far.sums;        // the far queries of first keys are parts of their own
+  const int key_sinks = apart ? 0 : sinks;                // first keys whose far queries are among this CTA's
+  TileList list = {};
+  int t_begin = 0, t_end;
+  if constexpr (SINKS) {
+    list = streamed_tiles(!KSIDE, m0, BM, BN, n_strm, off, p.causal, p.window, key_sinks);
+    t_end = list.count;
+  } else {
+    visible_tiles(!KSIDE, m0, BM, BN, n_strm, off, p.causal, p.window, t_begin, t_end);
+  }
+  auto tile_of = [&](int t) { return SINKS ? list.tile(t) : t; };
   if (split > 1) split_range(part, split, t_begin, t_end);
   if (far) far_tiles(m0, BN, p.n_q, off, p.window, part, p.far.parts, t_begin, t_end), list.begin = 0;
   const int n_iter = live ? t_end - t_begin : 0;
@@ -183,7 +193,7 @@ __device__ __forceinline__ void bw_body(const BwParams& p, int block, bool far) 
       load_tile<BM, DV, BM * 128>(smem + C::STAT0, stat_map(1), &bars->stat_full, m0, head_h, head_b);
       int issued0 = 0, issued1 = 0;
       for (int it = 0; it < n_iter; ++it) {
-        const int n0 = list.tile(t_begin + it) * BN, s1 = it % C::N1, s0 = it % C::N0;
+        const int n0 = tile_of(t_begin + it) * BN, s1 = it % C::N1, s0 = it % C::N0;
         if (!wait_bar(&bars->free1[s1], ((it / C::N1) & 1) ^ 1, bars, status)) break;
         mbar_arrive_expect_tx(&bars->full1[s1], C::TILE1);
         load_tile<BN, DV, BN * 128>(ring1 + s1 * C::SLOT1, strm_map(1), &bars->full1[s1], n0, head_h, head_b);
@@ -319,13 +329,13 @@ __device__ __forceinline__ void bw_body(const BwParams& p, int block, bool far) 
       hi = p.n_k - 1;
       if (p.causal && g_row + off < hi) hi = g_row + off;
       if (p.window > 0 && g_row + off - p.window + 1 > 0) lo = g_row + off - p.window + 1;
-      if (lo < p.sinks) lo = p.sinks;
+      if (SINKS && lo < sinks) lo = sinks;
     } else {
       lo = p.causal ? g_row - off : 0;
       if (lo < 0) lo = 0;
       hi = p.n_q - 1;
       if (far) lo = max(lo, g_row - off + p.window);   // (rows that are no first key are not stored)
-      else if (p.window > 0 && g_row >= key_sinks && g_row - off + p.window - 1 < hi) hi = g_row - off + p.window - 1;
+      else if (p.window > 0 && (!SINKS || g_row >= key_sinks) && g_row - off + p.window - 1 < hi) hi = g_row - off + p.window - 1;
     }
     bool ok = true;
     constexpr int NC = CPT / 32;
@@ -412,19 +422,19 @@ __device__ __forceinline__ void bw_body(const BwParams& p, int block, bool far) 
     };
 
     for (int it = 0; it < n_iter; ++it) {
-      const int n0 = list.tile(t_begin + it) * BN;
-      const bool first = !KSIDE && t_begin + it < list.first;   // a tile of the first keys: [0, sinks) of it
+      const int n0 = tile_of(t_begin + it) * BN;
+      const bool first = SINKS && !KSIDE && t_begin + it < list.first;   // a tile of the first keys: [0, sinks) of it
       bool masked = n0 + BN > n_strm;
       if (p.causal) {
         if (!KSIDE) masked = masked || (n0 + BN - 1 > m0 + off);
         else masked = masked || (n0 + off < m0 + BM - 1);
         if (p.window > 0) {
-          if (!KSIDE) masked = masked || (first ? n0 + BN > p.sinks : m0 + BM - 1 + off - n0 >= p.window || n0 < p.sinks);
-          else if (far) masked = masked || n0 < min(p.sinks, m0 + BM) - 1 - off + p.window;
+          if (!KSIDE) masked = masked || (first ? n0 + BN > sinks : m0 + BM - 1 + off - n0 >= p.window || (SINKS && n0 < sinks));
+          else if (far) masked = masked || n0 < min(sinks, m0 + BM) - 1 - off + p.window;
           else masked = masked || (n0 + BN - 1 + off - m0 >= p.window);
         }
       }
-      const int lo_t = first ? 0 : lo, hi_t = first && p.sinks <= hi ? p.sinks - 1 : hi;
+      const int lo_t = first ? 0 : lo, hi_t = first && sinks <= hi ? sinks - 1 : hi;
       if (masked) step(std::true_type{}, it, n0 + half * CPT, lo_t, hi_t);
       else step(std::false_type{}, it, n0 + half * CPT, lo_t, hi_t);
       if (!ok) break;
@@ -438,9 +448,9 @@ __device__ __forceinline__ void bw_body(const BwParams& p, int block, bool far) 
       stage_row<C::W0 / 2, SPLIT>(dst + half * (C::W0 / 2), lane_base + half * (C::W0 / 2), n_iter > 0);
       if constexpr (KSIDE) stage_row<C::W1 / 2, SPLIT>(dst + C::W0 + half * (C::W1 / 2), lane_base + C::OUT0 + half * (C::W1 / 2), n_iter > 0);
     } else if (ok && live) {
-      const bool sums = KSIDE && p.far.sums && g_row < p.sinks;   // a first key: added up with the other parts
-      if (KSIDE && p.far.sums && m0 < p.sinks) {
-        float* dst = far_row(p.far, head, far ? 1 + part : 0, sums ? g_row : 0, p.sinks, p.d + p.d_v);
+      const bool sums = apart && g_row < sinks;   // a first key: added up with the other parts
+      if (apart && m0 < sinks) {
+        float* dst = far_row(p.far, head, far ? 1 + part : 0, sums ? g_row : 0, sinks, p.d + p.d_v);
         store_sums<C::W0 / 2, SPLIT>(dst, lane_base + half * (C::W0 / 2), half * (C::W0 / 2), p.d, n_iter > 0, sums);
         if constexpr (KSIDE)
           store_sums<C::W1 / 2, SPLIT>(dst + p.d, lane_base + C::OUT0 + half * (C::W1 / 2), half * (C::W1 / 2), p.d_v, n_iter > 0, sums);
@@ -502,17 +512,17 @@ __device__ __forceinline__ void bw_body(const BwParams& p, int block, bool far) 
   if (threadIdx.x == 0 && fault) atomicOr(status, fault);
 }
 
-template <int DQK, int DV, bool F16, bool SPLIT>
+template <int DQK, int DV, bool F16, bool SPLIT, bool SINKS>
 __global__ void __launch_bounds__(NTHREADS, 1) bw_kernel(const __grid_constant__ BwParams p) {
-  const int block = static_cast<int>(blockIdx.x) - p.far.blocks;
-  if (block >= 0 && block < p.q_blocks) bw_body<false, DQK, DV, F16, SPLIT>(p, block, false);
-  else bw_body<true, DQK, DV, F16, SPLIT>(p, block < 0 ? blockIdx.x : block - p.q_blocks, block < 0);
+  const int block = static_cast<int>(blockIdx.x) - (SINKS ? p.far.blocks : 0);
+  if ((!SINKS || block >= 0) && block < p.q_blocks) bw_body<false, DQK, DV, F16, SPLIT, SINKS>(p, block, false);
+  else bw_body<true, DQK, DV, F16, SPLIT, SINKS>(p, SINKS && block < 0 ? blockIdx.x : block - p.q_blocks, SINKS && block < 0);
 }
 
 // ------------------------------------------------------------------ host side
 template <int DQK, int DV, bool F16, bool SPLIT = false>
 int bw_launch(const Problem& p, void* dq, void* dk, void* dv, cudaStream_t s) {
-  constexpr auto kernel = bw_kernel<DQK, DV, F16, SPLIT>;
+  const auto kernel = p.sinks > 0 ? bw_kernel<DQK, DV, F16, SPLIT, true> : bw_kernel<DQK, DV, F16, SPLIT, false>;
   using CQ = BwCfg<false, DQK, DV, SPLIT>;
   using CK = BwCfg<true, DQK, DV, SPLIT>;
   constexpr int kSmem = CQ::SMEM_BYTES > CK::SMEM_BYTES ? CQ::SMEM_BYTES : CK::SMEM_BYTES;

@@ -423,9 +423,11 @@ __device__ __forceinline__ float row_dot(const void* o, const void* d_o, int c0,
 
 // One pass over one 128-row tile of one head; `block` numbers the (head, tile, part) triples of the pass.
 // With few tiles a head the streamed axis is split over the CTAs of a cluster (see split_parts); each computes its
-// part's sums and the cluster adds them up.  `far`: pass 4 over a part of the queries that see first keys behind their window.
-template <int PASS, int DQK, int DV, int BN, int FUSED, bool F16, bool SPLIT>
-__device__ __forceinline__ void tc_pass_body(const TcParams& p, int block, bool far = false) {
+// part's sums and the cluster adds them up.  SINKS: with first keys.  (Kernels of their own: sharing one cost small calls without
+// them 2 %, 64 heads N = 2048 D = 64 1 %.)  `far`: pass 4 over a part of the queries that see first keys behind their window.
+template <int PASS, int DQK, int DV, int BN, int FUSED, bool F16, bool SPLIT, bool SINKS>
+__device__ __forceinline__ void tc_pass_body(const TcParams& p, int block, bool is_far = false) {
+  const bool far = SINKS && is_far;
   static_assert(FUSED == 0 || PASS == 2, "only pass 2 has a fused form");
   static_assert(!SPLIT || (DQK == 128 && DV == 128 && !F16), "split fp32 operands are [hi(64) | lo(64)] bf16 rows");
   using C = Cfg<PASS, DQK, DV, BN>;
@@ -455,9 +457,18 @@ __device__ __forceinline__ void tc_pass_body(const TcParams& p, int block, bool 
   const int n_strm = kQStat ? p.n_k : p.n_q;
   const int off = p.n_k - p.n_q;
 
-  const int key_sinks = !kQStat && p.far.sums ? 0 : p.sinks;   // first keys whose far queries are among this CTA's
-  TileList list = streamed_tiles(kQStat, m0, BM, BN, n_strm, off, p.causal, p.window, key_sinks);
-  int t_begin = 0, t_end = list.count;
+  const int sinks = SINKS ? p.sinks : 0;
+  const bool apart = SINKS && !kQStat && p.far.sums;      // the far queries of first keys are parts of their own
+  const int key_sinks = apart ? 0 : sinks;                // first keys whose far queries are among this CTA's
+  TileList list = {};
+  int t_begin = 0, t_end;
+  if constexpr (SINKS) {
+    list = streamed_tiles(kQStat, m0, BM, BN, n_strm, off, p.causal, p.window, key_sinks);
+    t_end = list.count;
+  } else {
+    visible_tiles(kQStat, m0, BM, BN, n_strm, off, p.causal, p.window, t_begin, t_end);
+  }
+  auto tile_of = [&](int t) { return SINKS ? list.tile(t) : t; };
   if (split > 1) split_range(part, split, t_begin, t_end);
   if (far) {
     far_tiles(m0, BN, p.n_q, off, p.window, part, p.far.parts, t_begin, t_end);
@@ -533,7 +544,7 @@ __device__ __forceinline__ void tc_pass_body(const TcParams& p, int block, bool 
         if (!wait_bar(&bars->strm_free[slot], ((it / C::NSLOT) & 1) ^ 1, bars, p.status)) break;
         mbar_arrive_expect_tx(&bars->strm_full[slot], C::SLOT_BYTES);
         uint8_t* dst = strm_tiles + slot * C::SLOT_BYTES;
-        const int n0 = list.tile(t_begin + it) * BN;
+        const int n0 = tile_of(t_begin + it) * BN;
 #pragma unroll
         for (int i = 0; i < C::NSTRM; ++i) {
           uint8_t* at = dst + C::strm_base(i);
@@ -761,13 +772,13 @@ __device__ __forceinline__ void tc_pass_body(const TcParams& p, int block, bool 
       c.hi = p.n_k - 1;
       if (p.causal && g_row + off < c.hi) c.hi = g_row + off;
       if (p.window > 0 && g_row + off - p.window + 1 > 0) c.lo = g_row + off - p.window + 1;
-      if (c.lo < p.sinks) c.lo = p.sinks;
+      if (SINKS && c.lo < sinks) c.lo = sinks;
     } else {
       c.lo = p.causal ? g_row - off : 0;
       if (c.lo < 0) c.lo = 0;
       c.hi = p.n_q - 1;
       if (far) c.lo = max(c.lo, g_row - off + p.window);   // (rows that are no first key are not stored)
-      else if (p.window > 0 && g_row >= key_sinks && g_row - off + p.window - 1 < c.hi) c.hi = g_row - off + p.window - 1;
+      else if (p.window > 0 && (!SINKS || g_row >= key_sinks) && g_row - off + p.window - 1 < c.hi) c.hi = g_row - off + p.window - 1;
     }
     [[maybe_unused]] const int row_lo = c.lo, row_hi = c.hi;
     float2 racc[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -775,11 +786,11 @@ __device__ __forceinline__ void tc_pass_body(const TcParams& p, int block, bool 
     bool ok = true;
 
     for (int it = 0; it < n_iter; ++it) {
-      const int n0 = list.tile(t_begin + it) * BN;
-      const bool first = kQStat && t_begin + it < list.first;   // a tile of the first keys: [0, sinks) of it
-      if (kQStat && list.first > 0) {
+      const int n0 = tile_of(t_begin + it) * BN;
+      const bool first = SINKS && kQStat && t_begin + it < list.first;   // a tile of the first keys: [0, sinks) of it
+      if (SINKS && kQStat && list.first > 0) {
         c.lo = first ? 0 : row_lo;
-        c.hi = first && p.sinks <= row_hi ? p.sinks - 1 : row_hi;
+        c.hi = first && sinks <= row_hi ? sinks - 1 : row_hi;
       }
       // does any element of this tile need masking?  (CTA-uniform: depends on tile coordinates only)
       bool masked = n0 + BN > n_strm;
@@ -788,8 +799,8 @@ __device__ __forceinline__ void tc_pass_body(const TcParams& p, int block, bool 
         else masked = masked || (n0 + off < m0 + BM - 1);
         if (p.window > 0) {
           // the pair of the tile that is furthest apart: last query row against first key row
-          if (kQStat) masked = masked || (first ? n0 + BN > p.sinks : m0 + BM - 1 + off - n0 >= p.window || n0 < p.sinks);
-          else if (far) masked = masked || n0 < min(p.sinks, m0 + BM) - 1 - off + p.window;
+          if (kQStat) masked = masked || (first ? n0 + BN > sinks : m0 + BM - 1 + off - n0 >= p.window || (SINKS && n0 < sinks));
+          else if (far) masked = masked || n0 < min(sinks, m0 + BM) - 1 - off + p.window;
           else masked = masked || (n0 + BN - 1 + off - m0 >= p.window);
         }
       }
@@ -914,10 +925,10 @@ __device__ __forceinline__ void tc_pass_body(const TcParams& p, int block, bool 
           stage_row<DV / 2>(dst + DQK + half * (DV / 2), acc + C::OUT0_COLS + half * (DV / 2), n_iter > 0);
         }
       } else if (ok && live) {   // a CTA that only fills up a cluster has no tile to store
-        const bool sums = !kQStat && p.far.sums && g_row < p.sinks;   // a first key: added up with the other parts
-        if (!kQStat && p.far.sums && m0 < p.sinks) {
+        const bool sums = apart && g_row < sinks;   // a first key: added up with the other parts
+        if (apart && m0 < sinks) {
           constexpr int W0 = SPLIT ? 64 : DQK, W1 = SPLIT ? 64 : DV;
-          float* dst = far_row(p.far, head, far ? 1 + part : 0, sums ? g_row : 0, p.sinks, p.d + p.d_v);
+          float* dst = far_row(p.far, head, far ? 1 + part : 0, sums ? g_row : 0, sinks, p.d + p.d_v);
           const uint32_t acc = tmem_base + lane_base;
           store_sums<W0 / 2, SPLIT>(dst, acc + half * (W0 / 2), half * (W0 / 2), p.d, n_iter > 0, sums);
           store_sums<W1 / 2, SPLIT>(dst + p.d, acc + C::OUT0_COLS + half * (W1 / 2), half * (W1 / 2), p.d_v, n_iter > 0, sums);
@@ -1031,18 +1042,18 @@ __device__ __forceinline__ void tc_pass_body(const TcParams& p, int block, bool 
   if (threadIdx.x == 0 && fault) atomicOr(p.status, fault);
 }
 
-template <int PASS, int DQK, int DV, int BN, int FUSED, bool F16, bool SPLIT>
+template <int PASS, int DQK, int DV, int BN, int FUSED, bool F16, bool SPLIT, bool SINKS>
 __global__ void __launch_bounds__(NTHREADS, 1) tc_pass_kernel(const __grid_constant__ TcParams p) {
-  tc_pass_body<PASS, DQK, DV, BN, FUSED, F16, SPLIT>(p, blockIdx.x);
+  tc_pass_body<PASS, DQK, DV, BN, FUSED, F16, SPLIT, SINKS>(p, blockIdx.x);
 }
 
 // Passes 3 and 4 in one launch: they only need the sweep, not each other, so pass 4's CTAs fill the
 // SMs that run out of pass-3 work (and a small problem runs both side by side).
-template <int DQK, int DV, bool F16, bool SPLIT>
+template <int DQK, int DV, bool F16, bool SPLIT, bool SINKS>
 __global__ void __launch_bounds__(NTHREADS, 1) tc_pass34_kernel(const __grid_constant__ TcParams p) {
-  const int block = static_cast<int>(blockIdx.x) - p.far.blocks;
-  if (block >= 0 && block < p.q_blocks) tc_pass_body<3, DQK, DV, 64, 0, F16, SPLIT>(p, block);
-  else tc_pass_body<4, DQK, DV, 64, 0, F16, SPLIT>(p, block < 0 ? blockIdx.x : block - p.q_blocks, block < 0);
+  const int block = static_cast<int>(blockIdx.x) - (SINKS ? p.far.blocks : 0);
+  if ((!SINKS || block >= 0) && block < p.q_blocks) tc_pass_body<3, DQK, DV, 64, 0, F16, SPLIT, SINKS>(p, block);
+  else tc_pass_body<4, DQK, DV, 64, 0, F16, SPLIT, SINKS>(p, SINKS && block < 0 ? blockIdx.x : block - p.q_blocks, SINKS && block < 0);
 }
 
 // ------------------------------------------------------------------ host side
@@ -1143,7 +1154,9 @@ int launch(K kernel, const TcParams& tp, long long blocks, int smem, cudaStream_
 
 template <int PASS, int DQK, int DV, int BN, int FUSED, bool F16, bool SPLIT>
 int launch_pass(const Problem& p, TcParams& tp, cudaStream_t s) {
-  constexpr auto kernel = tc_pass_kernel<PASS, DQK, DV, BN, FUSED, F16, SPLIT>;
+  auto kernel = tc_pass_kernel<PASS, DQK, DV, BN, FUSED, F16, SPLIT, false>;
+  if constexpr (FUSED != 0)   // (single passes take no first keys)
+    if (p.sinks > 0) kernel = tc_pass_kernel<PASS, DQK, DV, BN, FUSED, F16, SPLIT, true>;
   constexpr int kSmem = Cfg<PASS, DQK, DV, BN>::SMEM_BYTES;
   if (FUSED) tp.split_q = tp.cluster = tc_parts(p).q;
   return launch(kernel, tp, static_cast<long long>(tp.items_q) * tp.split_q, kSmem, s);
@@ -1152,7 +1165,7 @@ int launch_pass(const Problem& p, TcParams& tp, cudaStream_t s) {
 // Passes 3 and 4, or one of them.
 template <int DQK, int DV, bool F16, bool SPLIT>
 int launch_34(const Problem& p, TcParams& tp, bool pass3, bool pass4, cudaStream_t s) {
-  constexpr auto kernel = tc_pass34_kernel<DQK, DV, F16, SPLIT>;
+  const auto kernel = p.sinks > 0 ? tc_pass34_kernel<DQK, DV, F16, SPLIT, true> : tc_pass34_kernel<DQK, DV, F16, SPLIT, false>;
   constexpr int kSmem3 = Cfg<3, DQK, DV, 64>::SMEM_BYTES, kSmem4 = Cfg<4, DQK, DV, 64>::SMEM_BYTES;
   constexpr int kSmem = kSmem3 > kSmem4 ? kSmem3 : kSmem4;
   const Parts parts = tc_parts(p);
