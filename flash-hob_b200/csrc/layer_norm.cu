@@ -11,7 +11,7 @@
 //   terms do not cancel when v or g have a large common part.
 //
 // What bounds it: each matrix is read once and written once, so the memory.
-//  - A row belongs to a group: 2 to 32 lanes of a warp or 2 to 32 warps, 8 to 32 elements a lane.  It is in registers, in fp32,
+//  - A row belongs to a group: 2 to 32 lanes of a warp or up to 32 warps, 8 to 32 elements a lane.  It is in registers, in fp32,
 //    from its only load to its results; sums over it are shuffles, then, if the group has several warps, one exchange
 //    through shared memory per round.  Rounds: two in the forward (the variance is a sum of squares around the mean), one
 //    in the backward, two in the double backward.
@@ -202,8 +202,8 @@ __device__ __forceinline__ void group_sum(float (&x)[N], const P& at, float* exc
   for (int i = 0; i < N; ++i) x[i] = __shfl_sync(kAll, y, i);
 }
 
-// How the three kernels are laid out: blocks of 128 to 1024 threads, 512 threads an SM with 128 registers each (64 in blocks
-// of 1024, which only the longest rows take).  768 threads where less is kept of each, 384 where more is (see ln_grid).
+// How the three kernels are laid out: blocks with room for 128 to 1024 threads, 512 threads an SM with 128 registers each (80 in
+// blocks of 768 and 64 in those of 1024, which only long rows take).  768 threads where less is kept of each, 384 where more is (see ln_grid).
 enum { kLnForward, kLnBackward, kLnBwdbwd };
 constexpr int ln_threads(int what, bool wide, int each) {   // of an SM
   if (what == kLnForward) return wide && each <= 16 ? 768 : 512;
@@ -220,7 +220,7 @@ struct LnCfg {
   static constexpr int kStages = kFit > 4 ? 4 : kFit;                         // rows of the ring
   static constexpr int kExchange = 2 * LN_MAX_WARPS * 16;                     // bytes in front of it: two areas for the sums over a row
   static constexpr int kSmem = kExchange + kMatrices * kRow * kStages;
-  static constexpr bool kHold = WHAT != kLnBwdbwd || NV * V <= 8 || THREADS <= 256;   // vectors over the columns stay in registers
+  static constexpr bool kHold = WHAT != kLnBwdbwd || NV * V <= 8 || THREADS <= 384;   // vectors over the columns stay in registers
   static_assert(kStages >= 1, "a row of the ring");
   static_assert(WHAT == kLnForward || THREADS * NV * V * 4 <= kSmem - kExchange, "room for the sums over rows, see block_columns");
 };
@@ -640,7 +640,8 @@ __global__ void __launch_bounds__(1024) ln_columns_kernel(const float* partial, 
 // How a call is cut up.
 struct LnGrid {
   bool wide;
-  int each, lanes, warps, threads, blocks;   // elements of a thread; of a group: lanes and warps; threads and blocks
+  int each, lanes, warps;      // elements of a thread; of a group: lanes and warps
+  int room, threads, blocks;   // threads that a block has room for, and that it has (whole groups of several warps); blocks
 };
 constexpr int kSms = 148;
 constexpr int kLnMostBlocks = 3 * kSms;   // that leave sums over rows, see ln_threads and ln_grid
@@ -658,17 +659,28 @@ LnGrid ln_grid(int what, long long rows, int cols, bool wide, bool bits16) {
   if (what == kLnBwdbwd && cols <= (wide ? 4096 : 8192) && !(wide && bits16 && cols > 256 && rows > kSms)) g.each = 8;
   g.lanes = 32;
   while (g.lanes > 2 && g.lanes / 2 * g.each >= cols) g.lanes >>= 1;
-  g.warps = 1;
-  while (g.warps < LN_MAX_WARPS && g.warps * 32 * g.each < cols) g.warps <<= 1;
+  // As many warps as a row needs; what follows takes the next power of two of them.
+  g.warps = (cols + 32 * g.each - 1) / (32 * g.each);
+  int room = 1;
+  while (room < g.warps) room <<= 1;
   // Larger blocks leave fewer sums over rows to add up (16384 x 2048 bf16, backward 44.2 -> 43.0 us), which in the double backward pays
   // for rows of few warps only (8 elements a thread, 512 columns 80 -> 77 us, 2048 90 -> 102).
   const bool held = what == kLnBwdbwd && wide && g.each == 16 && cols <= 4096;
-  const int least = held ? 128 : (what == kLnForward || g.lanes < 32 || (what == kLnBwdbwd && g.warps > 4) ? 256 : 512);
-  g.threads = g.warps * 32 > least ? g.warps * 32 : least;
+  const int least = held ? 128 : (what == kLnForward || g.lanes < 32 || (what == kLnBwdbwd && room > 4) ? 256 : 512);
+  auto blocks_of_sm = [&](int threads) {
+    const int n = ln_threads(what, wide, g.each) / threads;
+    return n > 0 ? n : 1;
+  };
+  g.room = room * 32 > least ? room * 32 : least;
+  // Another size of block where that has more rows at once in work, or fits closer (backward, 2560 columns bf16 72 -> 54 us, 2501 123 -> 86).
+  auto rows_at_once = [&](int threads) { return blocks_of_sm(threads) * (threads / (32 * g.warps)); };
+  const int other = held ? 384 : 512;
+  if (g.lanes == 32 && g.room <= other && rows_at_once(other) > rows_at_once(g.room)) g.room = other;
+  if (g.room == 1024 && g.warps <= 24 && g.each == 16) g.room = 768;
+  g.threads = g.lanes < 32 ? g.room : g.room / (32 * g.warps) * 32 * g.warps;
   const int groups = g.threads / (g.warps * g.lanes);
   const long long wanted = (rows + groups - 1) / groups;
-  const int per_sm = ln_threads(what, wide, g.each) / g.threads;
-  const long long resident = static_cast<long long>(kSms) * (per_sm > 0 ? per_sm : 1);
+  const long long resident = static_cast<long long>(kSms) * blocks_of_sm(g.room);
   g.blocks = static_cast<int>(wanted < resident ? wanted : resident);
   return g;
 }
@@ -686,7 +698,7 @@ int ln_run(const LnParams& p, const LnGrid& g, cudaStream_t s) {
     }();
     const int st = allow_smem(kernel, C::kSmem);
     if (st != FHOB_OK) return st;
-    FHOB_CUDA_OK(launch_pdl(kernel, static_cast<unsigned>(g.blocks), kThreads, C::kSmem, 1, s, p));
+    FHOB_CUDA_OK(launch_pdl(kernel, static_cast<unsigned>(g.blocks), static_cast<unsigned>(g.threads), C::kSmem, 1, s, p));
     return FHOB_OK;
   };
   // (what ln_grid does not ask for is not built)
@@ -694,14 +706,20 @@ int ln_run(const LnParams& p, const LnGrid& g, cudaStream_t s) {
   constexpr bool kGrid = kWide<T, V>, kSecond = WHAT == kLnBwdbwd, kHeld = kSecond && kGrid && sizeof(T) == 2 && kEach == 16;
   if constexpr (kEach == 8 || (kEach == 16 && !kSecond))
     if (g.lanes < 32) return go(std::integral_constant<int, 256>{}, std::true_type{});
-  if constexpr (kHeld)
-    if (g.threads == 128) return go(std::integral_constant<int, 128>{}, std::false_type{});
+  if constexpr (kHeld) {
+    if (g.room == 128) return go(std::integral_constant<int, 128>{}, std::false_type{});
+    if (g.room == 384) return go(std::integral_constant<int, 384>{}, std::false_type{});
+  }
   if constexpr (WHAT == kLnForward || kHeld || (kSecond && kEach == 8))
-    if (g.threads == 256) return go(std::integral_constant<int, 256>{}, std::false_type{});
+    if (g.room == 256) return go(std::integral_constant<int, 256>{}, std::false_type{});
   if constexpr (!(kEach == 16 && ((WHAT == kLnForward && kGrid) || (kSecond && !kGrid))))
-    if (g.threads == 512) return go(std::integral_constant<int, 512>{}, std::false_type{});
-  if constexpr (WHAT == kLnForward ? kEach == 16 && !kGrid : (kEach == 16 || (kSecond && !kGrid)))
-    if (g.threads == 1024) return go(std::integral_constant<int, 1024>{}, std::false_type{});
+    if (g.room == 512) return go(std::integral_constant<int, 512>{}, std::false_type{});
+  if constexpr (kEach == 16 && !(WHAT == kLnForward && kGrid)) {
+    if (g.room == 768) return go(std::integral_constant<int, 768>{}, std::false_type{});
+    if (g.room == 1024) return go(std::integral_constant<int, 1024>{}, std::false_type{});
+  }
+  if constexpr (kEach == 8 && kSecond && !kGrid)
+    if (g.room == 1024) return go(std::integral_constant<int, 1024>{}, std::false_type{});
   return FHOB_ERR_SHAPE;
 }
 
