@@ -216,13 +216,16 @@ struct LnCfg {
   // Bytes of a row of the ring.  Off the grid a row may start anywhere in a piece of 16 bytes: one more for each group (and a word
   // that the last pair of the last group looks into).
   static constexpr int kRow = THREADS * NV * V * static_cast<int>(sizeof(T)) + (kWide<T, V> ? 0 : 16 * THREADS / (SUB ? 2 : 32));
-  static constexpr int kFit = 200 * 1024 / kBlocks / (kMatrices * kRow);
+  static constexpr bool kHold = WHAT != kLnBwdbwd || NV * V <= 8 || THREADS <= 384;   // vectors over the columns stay in registers,
+  static constexpr bool kShare = !kHold && THREADS == 512;                            // or in shared memory, a thread's own (or in L1)
+  static constexpr int kVectors = kShare ? 3 * THREADS * NV * V * 4 : 0;              // bytes behind the ring
+  static constexpr int kFit = (200 * 1024 - kVectors) / kBlocks / (kMatrices * kRow);
   static constexpr int kStages = kFit > 4 ? 4 : kFit;                         // rows of the ring
   static constexpr int kExchange = 2 * LN_MAX_WARPS * 16;                     // bytes in front of it: two areas for the sums over a row
-  static constexpr int kSmem = kExchange + kMatrices * kRow * kStages;
-  static constexpr bool kHold = WHAT != kLnBwdbwd || NV * V <= 8 || THREADS <= 384;   // vectors over the columns stay in registers
+  static constexpr int kRing = kMatrices * kRow * kStages;
+  static constexpr int kSmem = kExchange + kRing + kVectors;
   static_assert(kStages >= 1, "a row of the ring");
-  static_assert(WHAT == kLnForward || THREADS * NV * V * 4 <= kSmem - kExchange, "room for the sums over rows, see block_columns");
+  static_assert(WHAT == kLnForward || THREADS * NV * V * 4 <= kRing, "room for the sums over rows, see block_columns");
 };
 
 // The ring.  On the grid it is a thread's own: piece i of (stage, matrix) is THREADS * 16 bytes on from piece i - 1.  Off the
@@ -523,17 +526,33 @@ __global__ void __launch_bounds__(THREADS, LnCfg<kLnBwdbwd, T, V, NV, THREADS, S
 #pragma unroll
   for (int i = 0; i < C::kStages - 1; ++i) fetch(i, row + i * step);
   float2 w[NV][H], vw[NV][H], vb[NV][H], dw2[NV][H];
-  // what of them is not kept in registers is read (from L1) where it is needed
-  auto w_again = [&](int i) { if (!C::kHold) at.vector(w[i], p.w, p.w_f32, i, p.cols, 1.f); };
-  auto vw_again = [&](int i) { if (!C::kHold) at.vector(vw[i], p.vw, p.w_f32, i, p.cols, 0.f); };
-  auto vb_again = [&](int i) { if (!C::kHold) at.vector(vb[i], p.vb, p.w_f32, i, p.cols, 0.f); };
+  // what of them is not kept in registers is read where it is needed
+  float2* const shared = reinterpret_cast<float2*>(in_ring + C::kRing) + threadIdx.x;
+  auto again = [&](float2 (&to)[H], int which, const void* from, int i, float otherwise) {
+    if constexpr (C::kShare) {
+#pragma unroll
+      for (int j = 0; j < H; ++j) to[j] = shared[((which * NV + i) * H + j) * THREADS];
+    } else if constexpr (!C::kHold) {
+      at.vector(to, from, p.w_f32, i, p.cols, otherwise);
+    }
+  };
+  auto w_again = [&](int i) { again(w[i], 0, p.w, i, 1.f); };
+  auto vw_again = [&](int i) { again(vw[i], 1, p.vw, i, 0.f); };
+  auto vb_again = [&](int i) { again(vb[i], 2, p.vb, i, 0.f); };
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    if (C::kHold) {
+    if (C::kHold || C::kShare) {
       at.vector(w[i], p.w, p.w_f32, i, p.cols, 1.f);
       at.vector(vw[i], p.vw, p.w_f32, i, p.cols, 0.f);
       at.vector(vb[i], p.vb, p.w_f32, i, p.cols, 0.f);
     }
+    if (C::kShare)
+#pragma unroll
+      for (int j = 0; j < H; ++j) {
+        shared[((0 * NV + i) * H + j) * THREADS] = w[i][j];
+        shared[((1 * NV + i) * H + j) * THREADS] = vw[i][j];
+        shared[((2 * NV + i) * H + j) * THREADS] = vb[i][j];
+      }
 #pragma unroll
     for (int j = 0; j < H; ++j) dw2[i][j] = both(0.f);
   }
@@ -665,13 +684,14 @@ LnGrid ln_grid(int what, long long rows, int cols, bool wide, bool bits16) {
   while (room < g.warps) room <<= 1;
   // Larger blocks leave fewer sums over rows to add up (16384 x 2048 bf16, backward 44.2 -> 43.0 us), which in the double backward pays
   // for rows of few warps only (8 elements a thread, 512 columns 80 -> 77 us, 2048 90 -> 102).
-  const bool held = what == kLnBwdbwd && wide && g.each == 16 && cols <= 4096;
+  const bool held = what == kLnBwdbwd && wide && g.each == 16 && cols <= 384 * 16;
   const int least = held ? 128 : (what == kLnForward || g.lanes < 32 || (what == kLnBwdbwd && room > 4) ? 256 : 512);
   auto blocks_of_sm = [&](int threads) {
     const int n = ln_threads(what, wide, g.each) / threads;
     return n > 0 ? n : 1;
   };
   g.room = room * 32 > least ? room * 32 : least;
+  if (held && g.room > 384) g.room = 384;
   // Another size of block where that has more rows at once in work, or fits closer (backward, 2560 columns bf16 72 -> 54 us, 2501 123 -> 86).
   auto rows_at_once = [&](int threads) { return blocks_of_sm(threads) * (threads / (32 * g.warps)); };
   const int other = held ? 384 : 512;
@@ -703,7 +723,7 @@ int ln_run(const LnParams& p, const LnGrid& g, cudaStream_t s) {
   };
   // (what ln_grid does not ask for is not built)
   constexpr int kEach = NV * V;
-  constexpr bool kGrid = kWide<T, V>, kSecond = WHAT == kLnBwdbwd, kHeld = kSecond && kGrid && sizeof(T) == 2 && kEach == 16;
+  constexpr bool kGrid = kWide<T, V>, kSecond = WHAT == kLnBwdbwd, kHeld = kSecond && kGrid && kEach == 16;
   if constexpr (kEach == 8 || (kEach == 16 && !kSecond))
     if (g.lanes < 32) return go(std::integral_constant<int, 256>{}, std::true_type{});
   if constexpr (kHeld) {
