@@ -202,13 +202,10 @@ __device__ __forceinline__ void group_sum(float (&x)[N], const P& at, float* exc
   for (int i = 0; i < N; ++i) x[i] = __shfl_sync(kAll, y, i);
 }
 
-// How the three kernels are laid out: blocks with room for 128 to 1024 threads, 512 threads an SM with 128 registers each (80 in
-// blocks of 768 and 64 in those of 1024, which only long rows take).  768 threads where less is kept of each, 384 where more is (see ln_grid).
+// How the three kernels are laid out: blocks with room for 256 to 1024 threads, 512 threads an SM with 128 registers each (168 in
+// blocks of 384, 80 in those of 768 and 64 in those of 1024, which only long rows take), 768 where less is kept of each.
 enum { kLnForward, kLnBackward, kLnBwdbwd };
-constexpr int ln_threads(int what, bool wide, int each) {   // of an SM
-  if (what == kLnForward) return wide && each <= 16 ? 768 : 512;
-  return what == kLnBwdbwd && wide && each == 16 ? 384 : 512;
-}
+constexpr int ln_threads(int what, bool wide, int each) { return what == kLnForward && each <= 16 ? 768 : 512; }   // of an SM
 template <int WHAT, class T, int V, int NV, int THREADS, bool SUB>
 struct LnCfg {
   static constexpr int kMatrices = WHAT == kLnForward ? 1 : (WHAT == kLnBackward ? 2 : 3);
@@ -216,7 +213,7 @@ struct LnCfg {
   // Bytes of a row of the ring.  Off the grid a row may start anywhere in a piece of 16 bytes: one more for each group (and a word
   // that the last pair of the last group looks into).
   static constexpr int kRow = THREADS * NV * V * static_cast<int>(sizeof(T)) + (kWide<T, V> ? 0 : 16 * THREADS / (SUB ? 2 : 32));
-  static constexpr bool kHold = WHAT != kLnBwdbwd || NV * V <= 8 || THREADS <= 384;   // vectors over the columns stay in registers,
+  static constexpr bool kHold = WHAT != kLnBwdbwd || NV * V <= 8 || THREADS == 384;   // vectors over the columns stay in registers,
   static constexpr bool kShare = !kHold && THREADS == 512;                            // or in shared memory, a thread's own (or in L1)
   static constexpr int kVectors = kShare ? 3 * THREADS * NV * V * 4 : 0;              // bytes behind the ring
   static constexpr int kFit = (200 * 1024 - kVectors) / kBlocks / (kMatrices * kRow);
@@ -663,7 +660,7 @@ struct LnGrid {
   int room, threads, blocks;   // threads that a block has room for, and that it has (whole groups of several warps); blocks
 };
 constexpr int kSms = 148;
-constexpr int kLnMostBlocks = 3 * kSms;   // that leave sums over rows, see ln_threads and ln_grid
+constexpr int kLnMostBlocks = 2 * kSms;   // that leave sums over rows, see ln_threads and ln_grid
 
 LnGrid ln_grid(int what, long long rows, int cols, bool wide, bool bits16) {
   LnGrid g;
@@ -673,9 +670,10 @@ LnGrid ln_grid(int what, long long rows, int cols, bool wide, bool bits16) {
   g.each = rows <= kSms && cols <= 4096 ? 8 : 16;
   // The forward keeps little of each: 32 (bf16, 2048 columns 27.8 -> 26.3 us, 8192 40 -> 29; fp32 8192 51 -> 50, but 2048 21.6 -> 22.5).
   if (what == kLnForward && wide && cols >= (bits16 ? 1024 : 4097) && g.each == 16) g.each = 32;
-  // The double backward keeps much: 8.  16 with 384 threads an SM where rows of 16-bit elements are neither short nor long (512
-  // columns 77 -> 63 us, 2048 90 -> 85, 4096 107 -> 99; fp32 2048 61.9 -> 63.6), and for long ones, without the vectors over the columns.
-  if (what == kLnBwdbwd && cols <= (wide ? 4096 : 8192) && !(wide && bits16 && cols > 256 && rows > kSms)) g.each = 8;
+  // The double backward keeps much: 8.  16, with the vectors over the columns in shared memory, for 16-bit elements unless rows are short
+  // (512 columns 77 -> 60 us, 2048 90 -> 74, 4096 107 -> 86, 2001 154 -> 122; fp32 2048 62 -> 65, 2001 84 -> 94), and for long rows (8001 fp32
+  // 378 -> 225).
+  if (what == kLnBwdbwd && cols <= 4096 && !(bits16 && cols > 256 && rows > kSms)) g.each = 8;
   g.lanes = 32;
   while (g.lanes > 2 && g.lanes / 2 * g.each >= cols) g.lanes >>= 1;
   // As many warps as a row needs; what follows takes the next power of two of them.
@@ -684,19 +682,21 @@ LnGrid ln_grid(int what, long long rows, int cols, bool wide, bool bits16) {
   while (room < g.warps) room <<= 1;
   // Larger blocks leave fewer sums over rows to add up (16384 x 2048 bf16, backward 44.2 -> 43.0 us), which in the double backward pays
   // for rows of few warps only (8 elements a thread, 512 columns 80 -> 77 us, 2048 90 -> 102).
-  const bool held = what == kLnBwdbwd && wide && g.each == 16 && cols <= 384 * 16;
-  const int least = held ? 128 : (what == kLnForward || g.lanes < 32 || (what == kLnBwdbwd && room > 4) ? 256 : 512);
+  const bool several = what == kLnBwdbwd && g.each == 8 && room > 4;
+  const int least = what == kLnForward || g.lanes < 32 || several ? 256 : 512;
   auto blocks_of_sm = [&](int threads) {
     const int n = ln_threads(what, wide, g.each) / threads;
     return n > 0 ? n : 1;
   };
   g.room = room * 32 > least ? room * 32 : least;
-  if (held && g.room > 384) g.room = 384;
-  // Another size of block where that has more rows at once in work, or fits closer (backward, 2560 columns bf16 72 -> 54 us, 2501 123 -> 86).
+  // Larger blocks also where these have more rows at once in work (forward, 2501 columns bf16 101 -> 75 us, 5001 108 -> 81).
   auto rows_at_once = [&](int threads) { return blocks_of_sm(threads) * (threads / (32 * g.warps)); };
-  const int other = held ? 384 : 512;
-  if (g.lanes == 32 && g.room <= other && rows_at_once(other) > rows_at_once(g.room)) g.room = other;
+  if (g.lanes == 32 && g.room < 512 && rows_at_once(512) > rows_at_once(g.room)) g.room = 512;
+  if (what == kLnForward && !wide && g.each == 16 && g.room == 512 && rows_at_once(768) > rows_at_once(g.room)) g.room = 768;
+  // What fits closer has more registers a thread: long rows of up to 24 warps (double backward, 12288 columns bf16 480 -> 280 us), and in the
+  // double backward those of fp32 with up to 12, which then keep the vectors (6144 columns 127 -> 107).
   if (g.room == 1024 && g.warps <= 24 && g.each == 16) g.room = 768;
+  if (what == kLnBwdbwd && wide && !bits16 && g.each == 16 && g.warps <= 12) g.room = 384;
   g.threads = g.lanes < 32 ? g.room : g.room / (32 * g.warps) * 32 * g.warps;
   const int groups = g.threads / (g.warps * g.lanes);
   const long long wanted = (rows + groups - 1) / groups;
@@ -723,23 +723,19 @@ int ln_run(const LnParams& p, const LnGrid& g, cudaStream_t s) {
   };
   // (what ln_grid does not ask for is not built)
   constexpr int kEach = NV * V;
-  constexpr bool kGrid = kWide<T, V>, kSecond = WHAT == kLnBwdbwd, kHeld = kSecond && kGrid && kEach == 16;
+  constexpr bool kGrid = kWide<T, V>, kSecond = WHAT == kLnBwdbwd, kHeld = kSecond && kGrid && sizeof(T) == 4 && kEach == 16;
   if constexpr (kEach == 8 || (kEach == 16 && !kSecond))
     if (g.lanes < 32) return go(std::integral_constant<int, 256>{}, std::true_type{});
-  if constexpr (kHeld) {
-    if (g.room == 128) return go(std::integral_constant<int, 128>{}, std::false_type{});
+  if constexpr (kHeld)
     if (g.room == 384) return go(std::integral_constant<int, 384>{}, std::false_type{});
-  }
-  if constexpr (WHAT == kLnForward || kHeld || (kSecond && kEach == 8))
+  if constexpr (WHAT == kLnForward || (kSecond && kEach == 8))
     if (g.room == 256) return go(std::integral_constant<int, 256>{}, std::false_type{});
-  if constexpr (!(kEach == 16 && ((WHAT == kLnForward && kGrid) || (kSecond && !kGrid))))
+  if constexpr (!(kEach == 16 && WHAT == kLnForward && kGrid))
     if (g.room == 512) return go(std::integral_constant<int, 512>{}, std::false_type{});
   if constexpr (kEach == 16 && !(WHAT == kLnForward && kGrid)) {
     if (g.room == 768) return go(std::integral_constant<int, 768>{}, std::false_type{});
     if (g.room == 1024) return go(std::integral_constant<int, 1024>{}, std::false_type{});
   }
-  if constexpr (kEach == 8 && kSecond && !kGrid)
-    if (g.room == 1024) return go(std::integral_constant<int, 1024>{}, std::false_type{});
   return FHOB_ERR_SHAPE;
 }
 
