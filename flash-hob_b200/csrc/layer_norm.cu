@@ -16,8 +16,9 @@
 //    through shared memory per round.  Rounds: two in the forward (the variance is a sum of squares around the mean), one
 //    in the backward, two in the double backward.
 //  - Next to the memory comes the number of instructions: elements are converted once, the arithmetic is on packed pairs, and the
-//    vectors over the columns stay in registers.  (Converted where they are used, with scalar arithmetic, and without
-//    the copies below: 16384 x 2048 bf16 forward 42 us, backward 75, double backward 175; now 26, 43 and 85.)
+//    vectors over the columns stay in registers or (double backward) in a thread's own shared memory.  (Converted where they are
+//    used, with scalar arithmetic, and without the copies below: 16384 x 2048 bf16 forward 42 us, backward 75, double backward 175;
+//    now 26 (5.1 TB/s), 43 (4.7) and 74 (4.5).)
 //  - What keeps the memory busy is the number of bytes on their way.  Rows come through a ring in shared memory, up to
 //    three rows ahead of the one in work, by asynchronous copies.  On the 16-byte grid a thread copies its own elements
 //    alone: it is the only one to read them, so nothing waits but for its own copies.
