@@ -216,7 +216,9 @@ struct LnCfg {
   static constexpr int kRow = THREADS * NV * V * static_cast<int>(sizeof(T)) + (kWide<T, V> ? 0 : 16 * THREADS / (SUB ? 2 : 32));
   static constexpr bool kHold = WHAT != kLnBwdbwd || NV * V <= 8 || THREADS == 384;   // vectors over the columns stay in registers,
   static constexpr bool kShare = !kHold && THREADS == 512;                            // or in shared memory, a thread's own (or in L1)
-  static constexpr int kVectors = kShare ? 3 * THREADS * NV * V * 4 : 0;              // bytes behind the ring
+  // Of the backward: the weight, for long rows (12288 columns, 4096 rows bf16 149 -> 117 us; off the grid 9001 84 -> 92).
+  static constexpr bool kShareW = WHAT == kLnBackward && kWide<T, V> && THREADS >= 768;
+  static constexpr int kVectors = (kShare ? 3 : kShareW ? 1 : 0) * THREADS * NV * V * 4;   // bytes behind the ring
   static constexpr int kFit = (200 * 1024 - kVectors) / kBlocks / (kMatrices * kRow);
   static constexpr int kStages = kFit > 4 ? 4 : kFit;                         // rows of the ring
   static constexpr int kExchange = 2 * LN_MAX_WARPS * 16;                     // bytes in front of it: two areas for the sums over a row
@@ -446,9 +448,13 @@ __global__ void __launch_bounds__(THREADS, LnCfg<kLnBackward, T, V, NV, THREADS,
 #pragma unroll
   for (int i = 0; i < C::kStages - 1; ++i) fetch(i, row + i * step);
   float2 w[NV][H], dw[NV][H], db[NV][H];
+  float2* const shared = reinterpret_cast<float2*>(in_ring + C::kRing) + threadIdx.x;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     at.vector(w[i], p.w, p.w_f32, i, p.cols, 1.f);
+    if (C::kShareW)
+#pragma unroll
+      for (int j = 0; j < H; ++j) shared[(i * H + j) * THREADS] = w[i][j];
 #pragma unroll
     for (int j = 0; j < H; ++j) dw[i][j] = db[i][j] = both(0.f);
   }
@@ -476,7 +482,7 @@ __global__ void __launch_bounds__(THREADS, LnCfg<kLnBackward, T, V, NV, THREADS,
         h[i][j] = __fmul2_rn(__fadd2_rn(h[i][j], minus), both(r));
         dw[i][j] = __ffma2_rn(g[i][j], h[i][j], dw[i][j]);
         db[i][j] = __fadd2_rn(db[i][j], g[i][j]);
-        g[i][j] = __fmul2_rn(g[i][j], w[i][j]);
+        g[i][j] = __fmul2_rn(g[i][j], C::kShareW ? shared[(i * H + j) * THREADS] : w[i][j]);
         s0 = __fadd2_rn(s0, g[i][j]);
         s1 = __ffma2_rn(g[i][j], h[i][j], s1);
       }
