@@ -360,6 +360,7 @@ int fhob_static_scratch_status(void* stream);
  * takes up to two tensors of the same tokens (queries and keys, with heads of
  * their own).  Positions may be any integers of their type; the angle is
  * exact to position * frequency * 2^-52 radians.  Frequencies are finite.
+ * Positions and frequencies are aligned to their elements, else FHOB_ERR_ALIGN.
  * in: rows contiguous, other strides in elements, any alignment of whole
  * elements.  out: contiguous (batch, heads, n, d), not overlapping in.
  */
@@ -405,6 +406,8 @@ int fhob_rotary(const FhobRotary* r, void* stream);
  *                           NULL) dw2 of dy, x, w; mean and rstd are
  *                           regarded as functions of x.
  *
+ * Every pointer is aligned to its elements, else FHOB_ERR_ALIGN; rows and vectors
+ * on 16 bytes are faster.
  * The sums over rows need a workspace of fhob_layer_norm_workspace_bytes(cols)
  * bytes, 256-byte aligned; they are added up in a fixed order.
  */
