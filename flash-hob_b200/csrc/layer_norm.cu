@@ -214,8 +214,10 @@ struct LnCfg {
   // Bytes of a row of the ring.  Off the grid a row may start anywhere in a piece of 16 bytes: one more for each group (and a word
   // that the last pair of the last group looks into).
   static constexpr int kRow = THREADS * NV * V * static_cast<int>(sizeof(T)) + (kWide<T, V> ? 0 : 16 * THREADS / (SUB ? 2 : 32));
-  static constexpr bool kHold = WHAT != kLnBwdbwd || NV * V <= 8 || THREADS == 384;   // vectors over the columns stay in registers,
-  static constexpr bool kShare = !kHold && THREADS == 512;                            // or in shared memory, a thread's own (or in L1)
+  // Where the vectors over the columns are kept through the rows: in registers, or (kShare) in shared memory, a thread's own, or neither:
+  // read again for every row.
+  static constexpr bool kHold = WHAT != kLnBwdbwd || NV * V <= 8 || THREADS == 384;
+  static constexpr bool kShare = !kHold && THREADS == 512;
   // Of the backward: the weight, for long rows (12288 columns, 4096 rows bf16 149 -> 117 us; off the grid 9001 84 -> 92).
   static constexpr bool kShareW = WHAT == kLnBackward && kWide<T, V> && THREADS >= 768;
   static constexpr int kVectors = (kShare ? 3 : kShareW ? 1 : 0) * THREADS * NV * V * 4;   // bytes behind the ring
