@@ -206,11 +206,11 @@ __device__ __forceinline__ void group_sum(float (&x)[N], const P& at, float* exc
 // How the three kernels are laid out: blocks with room for 256 to 1024 threads, 512 threads an SM with 128 registers each (168 in
 // blocks of 384, 80 in those of 768 and 64 in those of 1024, which only long rows take), 768 where less is kept of each.
 enum { kLnForward, kLnBackward, kLnBwdbwd };
-constexpr int ln_threads(int what, bool wide, int each) { return what == kLnForward && each <= 16 ? 768 : 512; }   // of an SM
+constexpr int ln_threads(int what, int each) { return what == kLnForward && each <= 16 ? 768 : 512; }   // of an SM
 template <int WHAT, class T, int V, int NV, int THREADS, bool SUB>
 struct LnCfg {
   static constexpr int kMatrices = WHAT == kLnForward ? 1 : (WHAT == kLnBackward ? 2 : 3);
-  static constexpr int kBlocks = ln_threads(WHAT, kWide<T, V>, NV * V) > THREADS ? ln_threads(WHAT, kWide<T, V>, NV * V) / THREADS : 1;   // of an SM
+  static constexpr int kBlocks = ln_threads(WHAT, NV * V) > THREADS ? ln_threads(WHAT, NV * V) / THREADS : 1;   // of an SM
   // Bytes of a row of the ring.  Off the grid a row may start anywhere in a piece of 16 bytes: one more for each group (and a word
   // that the last pair of the last group looks into).
   static constexpr int kRow = THREADS * NV * V * static_cast<int>(sizeof(T)) + (kWide<T, V> ? 0 : 16 * THREADS / (SUB ? 2 : 32));
@@ -694,7 +694,7 @@ LnGrid ln_grid(int what, long long rows, int cols, bool wide, bool bits16) {
   const bool several = what == kLnBwdbwd && g.each == 8 && room > 4;
   const int least = what == kLnForward || g.lanes < 32 || several ? 256 : 512;
   auto blocks_of_sm = [&](int threads) {
-    const int n = ln_threads(what, wide, g.each) / threads;
+    const int n = ln_threads(what, g.each) / threads;
     return n > 0 ? n : 1;
   };
   g.room = room * 32 > least ? room * 32 : least;
