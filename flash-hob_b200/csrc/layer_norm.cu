@@ -6,9 +6,11 @@
 //   cotangents v of dx, vw of dw, vb of db; a = mean v, c = mean(v h), m = mean g, q = mean(g h):
 //     p = v - a - h c:   ddy = r w p + vw h + vb              dw2 = sum dy r p
 //     e = vw dy - r (g c + v q):
-//       dx2 = r (e - mean e - h mean(e h)) - r^2 h mean(p (g - m - h q))
-//   (sums over rows for dw, db, dw2; means over a row).  mean(p (g - m - h q)) equals mean(v g) - a m - c q, but its
-//   terms do not cancel when v or g have a large common part.
+//       dx2 = r (e - mean e - h mean(e h)) - r^2 h mean(p (g - m))
+//   (sums over rows for dw, db, dw2; means over a row).  The last mean stands for mean(v g) - a m - c q, which it equals for every eps:
+//   mean(p (g - m)) = mean(v g) - m a - a mean(g - m) - c mean(h g) + c m mean h, where mean(g - m) = mean h = 0.  Both of its factors are
+//   centred, so nothing cancels when v or g have a large common part.  (Not p (g - m - h q): that adds c q (mean(h^2) - 1), and
+//   mean(h^2) = var / (var + eps) is one only for eps = 0.)
 //
 // What bounds it: each matrix is read once and written once, so the memory.
 //  - A row belongs to a group: 2 to 32 lanes of a warp or up to 32 warps, 8 to 32 elements a lane.  It is in registers, in fp32,
@@ -596,7 +598,7 @@ __global__ void __launch_bounds__(THREADS, LnCfg<kLnBwdbwd, T, V, NV, THREADS, S
     float s[4] = {s0.x + s0.y, s1.x + s1.y, s2.x + s2.y, s3.x + s3.y};
     group_sum<4>(s, at, exchange);
     const float a = s[0] * p.inv_cols, c = s[1] * p.inv_cols, m = s[2] * p.inv_cols, q = s[3] * p.inv_cols;
-    s0 = s1 = s2 = both(0.f);   // sums of p (g - m - h q), e, e h
+    s0 = s1 = s2 = both(0.f);   // sums of p (g - m), e, e h
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const float2 minus = at.inside(-a, i, p.cols);
@@ -608,7 +610,7 @@ __global__ void __launch_bounds__(THREADS, LnCfg<kLnBwdbwd, T, V, NV, THREADS, S
         const float2 e = __ffma2_rn(vw[i][j], d[i][j], __ffma2_rn(g, both(-r * c), __fmul2_rn(u[i][j], both(-r * q))));
         const float2 pp = __ffma2_rn(h[i][j], both(-c), __fadd2_rn(u[i][j], minus));
         dw2[i][j] = __ffma2_rn(__fmul2_rn(d[i][j], both(r)), pp, dw2[i][j]);
-        s0 = __ffma2_rn(pp, __ffma2_rn(h[i][j], both(-q), __fadd2_rn(g, both(-m))), s0);
+        s0 = __ffma2_rn(pp, __fadd2_rn(g, both(-m)), s0);
         s1 = __fadd2_rn(s1, e);
         s2 = __ffma2_rn(e, h[i][j], s2);
         u[i][j] = pp;
