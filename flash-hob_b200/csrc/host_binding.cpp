@@ -235,6 +235,7 @@ struct AttentionBackward : torch::autograd::Function<AttentionBackward> {
     const auto s = ctx->get_saved_variables();
     const double scale = ctx->saved_data["scale"].toDouble();
     const Mask m{ctx->saved_data["causal"].toBool(), ctx->saved_data["window"].toInt(), ctx->saved_data["sinks"].toInt()};
+    TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent({&g[0], &g[1], &g[2]}), "fhob.attention has no forward-mode derivative of its double backward");
     py::gil_scoped_acquire gil;
     Tensor r[4];
     if (!run_bwdbwd(s[0], s[1], s[2], &s[3], s[5], g[0], g[1], g[2], s[4], scale, m, FHOB_IMPL_AUTO, r)) {

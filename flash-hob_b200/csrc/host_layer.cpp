@@ -120,7 +120,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
     Tensor d[2];
     const bool has0 = g[0].defined(), has1 = ctx->saved_data["both"].toBool() && g[1].defined();
     if (!has0 && !has1) return variable_list(7);
-    if (!at::GradMode::is_enabled()) {   // no graph is asked for
+    if (!at::GradMode::is_enabled() && !has_tangent({&g[0], has1 ? &g[1] : &g[0]})) {   // no derivative of this is asked for
       const auto r = rotate(has0 ? g[0] : g[1], has0 && has1 ? g[1] : Tensor(), s[0], s[1], axes, interleaved, inverse);
       d[has0 ? 0 : 1] = r[0];
       if (has0 && has1) d[1] = r[1];
@@ -155,7 +155,7 @@ void check_rotary(const Tensor* const* x, int count, const Tensor& positions, co
   TORCH_CHECK_TYPE(frequencies.scalar_type() == at::kFloat || frequencies.scalar_type() == at::kDouble, "frequencies must be float32 or float64, got ",
                    frequencies.scalar_type());
   TORCH_CHECK_VALUE(frequencies.device() == q.device(), "frequencies are on ", frequencies.device(), ", the tensors on ", q.device());
-  TORCH_CHECK_VALUE(!frequencies.requires_grad(), "frequencies are constants: no gradient flows into them (pass frequencies.detach())");
+  TORCH_CHECK_VALUE(!frequencies.requires_grad() && !has_tangent({&frequencies}), "frequencies are constants: no gradient flows into them (pass frequencies.detach())");
   TORCH_CHECK_VALUE(frequencies.dim() == 1 && frequencies.size(0) >= 1 && 2 * frequencies.size(0) <= q.size(-1),
                     "frequencies: expected one for each of at most D / 2 = ", q.size(-1) / 2, " pairs, got ", frequencies.sizes());
   TORCH_CHECK_VALUE(q.size(-1) <= FHOB_ROTARY_MAX_DIM, "rows of at most ", FHOB_ROTARY_MAX_DIM, " elements, got ", q.size(-1));
@@ -316,7 +316,7 @@ struct LayerNormBackward : torch::autograd::Function<LayerNormBackward> {
     const Tensor ddw = has_dw ? g[1] : Tensor(), ddb = has_db ? g[1 + has_dw] : Tensor();
     Tensor ddy, dx2, dw2;
     norm_bwdbwd(g[0], ddw, ddb, s[0], s[1], s[2], s[3], s[4], ddy, dx2, dw2);
-    if (at::GradMode::is_enabled()) {
+    if (at::GradMode::is_enabled() || has_tangent({&g[0], &ddw, &ddb})) {
       const auto r = NoThirdDerivative::apply(ddy, dx2, maybe(dw2), s[0], s[1], maybe(s[2]), maybe(g[0]), maybe(ddw), maybe(ddb));
       ddy = r[0];
       dx2 = r[1];
@@ -340,7 +340,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const auto s = ctx->get_saved_variables();
     const bool has_w = s[1].defined();   // (inputs are counted without those that are missing)
     const bool want_dw = has_w && ctx->needs_input_grad(1), want_db = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(1 + has_w);
-    if (!at::GradMode::is_enabled()) {   // no graph is asked for
+    if (!at::GradMode::is_enabled() && !has_tangent({&g[0]})) {   // no derivative of this is asked for
       Tensor dx, dw, db;
       norm_backward(g[0], s[0], s[1], s[2], s[3], want_dw, want_db, static_cast<at::ScalarType>(ctx->saved_data["type"].toInt()), dx, dw, db);
       return {dx, dw, db, Tensor()};
@@ -385,7 +385,9 @@ const Tensor& tensor_arg(PyObject* o, const char* name) {
 }
 Tensor optional_arg(PyObject* o, const char* name) { return o == Py_None ? Tensor() : tensor_arg(o, name); }
 
+// Does the call go through its autograd function?
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
+  if (has_tangent(ts)) return true;
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : ts)
     if (t->defined() && t->requires_grad()) return true;
