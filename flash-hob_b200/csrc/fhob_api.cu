@@ -222,10 +222,11 @@ bool use_tc(const FhobProblem& p) {
 // Where the sums of the first keys' far queries go: behind everything else in the workspace.
 size_t far_offset(const FhobProblem& p, bool split) { return align256(split ? split_workspace_bytes(p) : fhob_workspace_bytes(p.bh, p.n_q)); }
 
-// The problem of a call with first tokens that stay visible: FHOB_ERR_ARG for sinks without a window.  Where that
-// leaves no key in front of a diagonal hidden, the mask is the window's (it hides none) or plainly causal.
+// The problem of a call with first tokens that stay visible: FHOB_ERR_ARG for sinks without a causal mask and a window (checked
+// here, since the mask is rewritten).  Where that leaves no key in front of a diagonal hidden, the mask is the window's (it hides
+// none) or plainly causal.
 int attention_problem(const FhobProblem* p, int32_t sink_tokens, Problem* q) {
-  if (!p || sink_tokens < 0 || (sink_tokens > 0 && p->window <= 0)) return FHOB_ERR_ARG;
+  if (!p || sink_tokens < 0 || (sink_tokens > 0 && (p->window <= 0 || p->causal != 1))) return FHOB_ERR_ARG;
   static_cast<FhobProblem&>(*q) = *p;
   q->sinks = 0;
   if (sink_tokens == 0 || p->window >= p->n_k) return FHOB_OK;

@@ -290,8 +290,9 @@ int fhob_backward(const FhobProblem* p, void* dq, void* dk, void* dv, void* stre
  * > 0) and a few first tokens that stay visible behind it: key j is visible to
  * query i iff i + n_k - n_q >= j and (i + n_k - n_q - j < window or
  * j < sink_tokens).  sink_tokens = 0 is the call without it; sink_tokens < 0, or
- * > 0 without a window, FHOB_ERR_ARG.  A forward's L and O go with a backward of
- * the same window and sink_tokens.  The reference has no counterpart.
+ * > 0 without a causal mask and a window, FHOB_ERR_ARG.  A forward's L and O go
+ * with a backward of the same window and sink_tokens.  The reference has no
+ * counterpart.
  *
  * With a workspace of fhob_workspace_bytes_sinks() bytes the backward calls cut
  * the queries that see the first keys behind their window into parts that run
