@@ -509,8 +509,9 @@ int fhob_forward_sinks(const FhobProblem* given, int32_t sink_tokens, void* o_ou
     if (tc) return FHOB_ERR_WORKSPACE;
     status = nullptr;   // the CUDA-core kernel only clears the word: it does without one
   }
+  // every kernel clears the status word, which another call's may just have set; fp32 on the tensor cores: the hi/lo copies
+  std::lock_guard<std::mutex> together(workspace_lock(p->workspace));
   if (p->impl == FHOB_IMPL_AUTO && token_supported(*p, o_out)) return token_forward(*p, o_out, lse_out, status, s);
-  std::lock_guard<std::mutex> together(workspace_lock(p->workspace));   // fp32 on the tensor cores: the hi/lo copies
   return tc ? tc_forward(*p, o_out, lse_out, status, s) : simt_forward(*p, o_out, lse_out, status, s);
 }
 
