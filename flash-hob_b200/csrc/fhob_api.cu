@@ -222,13 +222,22 @@ bool use_tc(const FhobProblem& p) {
 // Where the sums of the first keys' far queries go: behind everything else in the workspace.
 size_t far_offset(const FhobProblem& p, bool split) { return align256(split ? split_workspace_bytes(p) : fhob_workspace_bytes(p.bh, p.n_q)); }
 
+// The caller's problem as the kernels take it.  A window beyond both lengths hides what one of their size hides, nothing, and leaves
+// sums of rows and window below 2^31 (with 2^31 - 1 the last visible query of a key came out negative: no gradient of keys and values).
+Problem plain_problem(const FhobProblem& p) {
+  Problem q;
+  static_cast<FhobProblem&>(q) = p;
+  const int most = p.n_q > p.n_k ? p.n_q : p.n_k;
+  if (q.window > most) q.window = most;
+  return q;
+}
+
 // The problem of a call with first tokens that stay visible: FHOB_ERR_ARG for sinks without a causal mask and a window (checked
 // here, since the mask is rewritten).  Where that leaves no key in front of a diagonal hidden, the mask is the window's (it hides
 // none) or plainly causal.
 int attention_problem(const FhobProblem* p, int32_t sink_tokens, Problem* q) {
   if (!p || sink_tokens < 0 || (sink_tokens > 0 && (p->window <= 0 || p->causal != 1))) return FHOB_ERR_ARG;
-  static_cast<FhobProblem&>(*q) = *p;
-  q->sinks = 0;
+  *q = plain_problem(*p);
   if (sink_tokens == 0 || p->window >= p->n_k) return FHOB_OK;
   if (static_cast<long long>(sink_tokens) + p->window >= p->n_k) q->window = 0;
   else q->sinks = sink_tokens;
@@ -245,11 +254,6 @@ int backward_problem(const FhobProblem* p, int32_t sink_tokens, Problem* q) {
     q->far_sums = reinterpret_cast<float*>(static_cast<char*>(q->workspace) + at);
   }
   return FHOB_OK;
-}
-Problem plain_problem(const FhobProblem& p) {
-  Problem q;
-  static_cast<FhobProblem&>(q) = p;
-  return q;
 }
 
 // Backwards with first keys in fp32: the CUDA cores, unless the caller asks for the tensor cores.  Split operands
