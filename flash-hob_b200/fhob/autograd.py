@@ -38,7 +38,8 @@ def attention_backward(Q, K, V, O, dO, L, scale, *, is_causal: bool = False, sli
         if got is not None:
             return got
     if Q.numel() == 0 or K.numel() == 0 or V.numel() == 0:
-        _sinks(_window(is_causal, sliding_window), sink_tokens)
+        if sink_tokens:
+            _sinks(_window(is_causal, sliding_window), sink_tokens)
         return tuple(torch.zeros_like(t) for t in (Q, K, V))   # no queries or no keys: nothing to launch
     # the problem struct wants three cotangent tensors of the right shapes; they are not read
     prob = _Problem(Q, K, V, O, dO, Q, K, V, L, scale, is_causal, impl, need_outputs=False, window=sliding_window,

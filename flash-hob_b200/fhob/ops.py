@@ -499,7 +499,7 @@ def attention_forward(Q, K, V, scale=None, *, is_causal: bool = False, sliding_w
         raise ValueError("attention_forward needs CUDA bfloat16/float16/float32 tensors")
     if impl not in _lib.IMPL:
         raise ValueError(f"impl must be one of {sorted(_lib.IMPL)}, got {impl!r}")
-    sinks = _sinks(_window(is_causal, sliding_window), sink_tokens)
+    sinks = _sinks(_window(is_causal, sliding_window), sink_tokens) if sink_tokens else 0
     # views are read in place when the tensor-core kernels run (see _Problem); else folded copies
     strides = None
     if (all(t.dim() in (3, 4) for t in (Q, K, V)) and impl != "simt" and _tc_capable(Q.dtype, Q.shape[-1], V.shape[-1])
