@@ -256,10 +256,12 @@ int backward_problem(const FhobProblem* p, int32_t sink_tokens, Problem* q) {
   return FHOB_OK;
 }
 
-// Backwards with first keys in fp32: the CUDA cores, unless the caller asks for the tensor cores.  Split operands
-// leave 2-norm errors of 0.8e-5 to 3e-5 (the longer the window, the larger), the CUDA cores 6e-7 (8 heads N = 2048 D = 64 W = 512, double
-// backward: 122 us against 916).  Problems without first keys keep the kernels they had.
-bool use_tc_backward(const Problem& p) { return use_tc(p) && !(p.sinks > 0 && p.dtype == FHOB_F32 && p.impl == FHOB_IMPL_AUTO); }
+// fp32 with first keys: the CUDA cores in all directions, unless the caller asks for the tensor cores.  Split operands leave 2-norm errors
+// of 0.8e-5 to 3e-5 in the backwards (the longer the window, the larger) and 3e-6 to 7e-6 in O and L, which the backwards start from; the CUDA
+// cores 6e-7 (8 heads N = 2048 D = 64 W = 512: double backward 122 us against 916, forward 33 against 161).  Problems without first keys
+// keep the kernels they had.
+bool keeps_fp32(const Problem& p) { return p.sinks > 0 && p.dtype == FHOB_F32 && p.impl == FHOB_IMPL_AUTO; }
+bool use_tc_backward(const Problem& p) { return use_tc(p) && !keeps_fp32(p); }
 
 int run_pass(int pass, const FhobProblem* p, void* stream) {
   int st = validate(p, pass >= 3);
@@ -504,7 +506,7 @@ int fhob_forward_sinks(const FhobProblem* given, int32_t sink_tokens, void* o_ou
     if (!layout_ok(l, mats, 3, p->dtype == FHOB_F32 ? 4 : 2)) return FHOB_ERR_ALIGN;
   }
   if (p->impl == FHOB_IMPL_TCGEN05 && !tc_ok) return FHOB_ERR_SHAPE;
-  const bool tc = p->impl != FHOB_IMPL_SIMT && tc_ok;
+  const bool tc = p->impl != FHOB_IMPL_SIMT && tc_ok && !keeps_fp32(*p);
   int* status = static_cast<int*>(p->workspace);
   if (!status) {
     int st = own_status_word(&status);
@@ -516,6 +518,7 @@ int fhob_forward_sinks(const FhobProblem* given, int32_t sink_tokens, void* o_ou
   // every kernel clears the status word, which another call's may just have set; fp32 on the tensor cores: the hi/lo copies
   std::lock_guard<std::mutex> together(workspace_lock(p->workspace));
   if (p->impl == FHOB_IMPL_AUTO && token_supported(*p, o_out)) return token_forward(*p, o_out, lse_out, status, s);
+  if (p->layout && !tc) return FHOB_ERR_SHAPE;   // (the CUDA cores read no views)
   return tc ? tc_forward(*p, o_out, lse_out, status, s) : simt_forward(*p, o_out, lse_out, status, s);
 }
 

@@ -93,8 +93,8 @@ bool fill(Call& c, const Tensor* const (&t)[kTensors], double scale, const Mask&
     // views are read in place through the tensor maps of the tensor-core kernels, if every stride
     // stays on the 16-byte grid
     if (impl == FHOB_IMPL_SIMT || !is_tc_capable(dtype, d, dv)) return false;
-    // backwards with first keys in fp32 run on the CUDA cores, which read no views
-    if (t[kDO] && m.sinks > 0 && dtype == at::kFloat && impl == FHOB_IMPL_AUTO) return false;
+    // fp32 with first keys runs on the CUDA cores, which read no views (the forward of one or two queries does)
+    if ((t[kDO] || n_q > 2) && m.sinks > 0 && dtype == at::kFloat && impl == FHOB_IMPL_AUTO) return false;
     memset(&c.lay, 0, sizeof(c.lay));
     c.lay.heads = static_cast<int32_t>(heads);
     for (int i = 0; i < kTensors; ++i) {

@@ -486,7 +486,9 @@ def attention_forward(Q, K, V, scale=None, *, is_causal: bool = False, sliding_w
     ``need_o=False`` skips the ``P V`` product and returns ``(None, L)``.
     ``check`` synchronises and raises if a bounded device wait ran out.
     Queries that see no key (causal with N_K < N_Q) get ``O = 0``, ``L = -inf``.
-    ``sliding_window`` and ``sink_tokens`` as in ``flash_bwdbwd``.
+    ``sliding_window`` and ``sink_tokens`` as in ``flash_bwdbwd`` (float32 with
+    first keys: fp32 throughout, several times slower than ``impl="tcgen05"``,
+    whose operands in two bf16 parts leave errors of 3e-6 to 7e-6).
     """
     if Q.is_cuda:
         got = _native().forward(Q, K, V, scale, is_causal, sliding_window, impl, need_o, sink_tokens)
@@ -502,8 +504,9 @@ def attention_forward(Q, K, V, scale=None, *, is_causal: bool = False, sliding_w
     sinks = _sinks(_window(is_causal, sliding_window), sink_tokens) if sink_tokens else 0
     # views are read in place when the tensor-core kernels run (see _Problem); else folded copies
     strides = None
-    if (all(t.dim() in (3, 4) for t in (Q, K, V)) and impl != "simt" and _tc_capable(Q.dtype, Q.shape[-1], V.shape[-1])
-            and not all(t.is_contiguous() for t in (Q, K, V))):
+    fp32_throughout = impl == "auto" and sinks and Q.dtype == torch.float32   # on the CUDA cores, but for one or two queries
+    if (all(t.dim() in (3, 4) for t in (Q, K, V)) and impl != "simt" and not (fp32_throughout and Q.shape[-2] > 2)
+            and _tc_capable(Q.dtype, Q.shape[-1], V.shape[-1]) and not all(t.is_contiguous() for t in (Q, K, V))):
         batches, heads = (Q.shape[0], Q.shape[1]) if Q.dim() == 4 else (1, Q.shape[0])
         strides = [_strides_of(t, batches, heads) for t in (Q, K, V)]
         if any(st is None for st in strides):

@@ -294,6 +294,11 @@ int fhob_backward(const FhobProblem* p, void* dq, void* dk, void* dv, void* stre
  * with a backward of the same window and sink_tokens.  The reference has no
  * counterpart.
  *
+ * fp32 with FHOB_IMPL_AUTO runs on the CUDA cores in all directions where first
+ * keys count (2-norm errors of 6e-7).  They read no views: FHOB_ERR_SHAPE with a
+ * layout, but for the forward of one or two queries.  FHOB_IMPL_TCGEN05 asks for
+ * the tensor cores (2 to 10 times faster, errors of 3e-6 to 3e-5).
+ *
  * With a workspace of fhob_workspace_bytes_sinks() bytes the backward calls cut
  * the queries that see the first keys behind their window into parts that run
  * side by side, with fhob_workspace_bytes_problem() bytes one CTA goes through
