@@ -17,10 +17,12 @@
 //    from its only load to its results; sums over it are shuffles, then, if the group has several warps, one exchange
 //    through shared memory per round.  Rounds: two in the forward (the variance is a sum of squares around the mean), one
 //    in the backward, two in the double backward.
-//  - Next to the memory comes the number of instructions: elements are converted once, the arithmetic is on packed pairs, and the
-//    vectors over the columns stay in registers or (double backward) in a thread's own shared memory.  (Converted where they are
-//    used, with scalar arithmetic, and without the copies below: 16384 x 2048 bf16 forward 42 us, backward 75, double backward 175;
-//    now 26 (5.1 TB/s), 43 (4.7) and 74 (4.5).)
+//  - What is left next to the memory is latency: a row's conversion, sums, exchange and stores follow one another, and the 16 to 24 warps
+//    an SM that the registers allow (24 to 25 % of the most) issue in 50 to 57 % of the cycles.  So that these are short, elements are
+//    converted once, the arithmetic is on packed pairs, and the vectors over the columns stay in registers or (double backward) in a thread's
+//    own shared memory.  (Converted where they are used, with scalar arithmetic, and without the copies below: 16384 x 2048 bf16 forward
+//    42 us, backward 75, double backward 175; now 26 (5.1 TB/s), 43 (4.7, of which the second launch takes 6) and 72 (4.6).  fp32 50 (5.4), 69 (5.9)
+//    and 112 (6.0).)
 //  - What keeps the memory busy is the number of bytes on their way.  Rows come through a ring in shared memory, up to
 //    three rows ahead of the one in work, by asynchronous copies.  On the 16-byte grid a thread copies its own elements
 //    alone: it is the only one to read them, so nothing waits but for its own copies.

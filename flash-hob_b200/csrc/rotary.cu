@@ -16,7 +16,7 @@
 // Its threads work out the angles of these tokens together, into shared memory; then a thread owns four pairs
 // of one token's rows (a warp covers whole rows) and passes over heads, four in flight, the first of them while
 // the angles are worked out.  32 heads N = 8192 D = 128 bf16: 46 us, 5.8 TB/s (55 when every thread worked out its own angles);
-// a token of 8 x 32 heads 3.2 us.
+// a token of 8 x 32 heads 3.2 us.  fp32, 32 + 32 heads N = 8192 D = 128: 89 us, 6.0 TB/s.
 #include "fhob_common.cuh"
 #include "tc_common.cuh"
 

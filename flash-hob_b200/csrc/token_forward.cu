@@ -4,7 +4,7 @@
 //
 // What bounds it: every visible key and value is read once for the one or two queries, so the memory: 128 heads of one query,
 // W = 1024 and 4 first keys, D = 128 read 67 MB.  The tensor-core forward has 128-row query tiles and goes through a head
-// in one CTA, tile after tile: 26 us there.  Here 15.6 us (4.3 TB/s):
+// in one CTA, tile after tile: 26 us there.  Here 15.5 us (4.3 TB/s; 4000 keys 5.3, 8000 6.1, fp32 5.0, 6.2 and 6.6):
 //  - eight lanes read one key's row, one, two or four times 16 bytes a lane: a product takes three shuffles.  Each such group goes
 //    through keys of its own with a running maximum and sum of its own: groups, warps and CTAs meet at the end;
 //  - a group takes four keys at a time: their rows of K and V are all on their way before the first is used.  What counts besides is
@@ -304,8 +304,9 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS > 4 ? 1 : (R > 1 ? 3 : 4)) t
 template <class T>
 int token_launch(const TkParams& p, int heads, cudaStream_t s) {
   const int pieces = ((p.d > p.d_v ? p.d : p.d_v) * static_cast<int>(sizeof(T)) + 15) / 16;
-  // Up to five rounds of 64 keys a CTA of 4 warps (128 heads W = 1024: 15.6 us; with four 21.8, with six 16.3; 16 heads 6.4, 5.7 and 6.8).
-  // What 8 such CTAs would take long for, CTAs of 16 warps share.
+  // Up to five rounds of 64 keys a CTA of 4 warps (128 heads W = 1024: 15.6 us; with four 21.8, with six 16.3; 16 heads 6.4, 5.7 and 6.8: at other
+  // lengths the three have not been compared).  What 8 such CTAs would take long for, CTAs of 16 warps share.  64 heads of 500, 1000, 2000, 4000,
+  // 8000 and 16000 keys, bf16: 10, 11, 16, 27, 45 and 106 us (1.7, 2.9, 4.1, 4.9, 5.8 and 5.0 TB/s).
   constexpr int kRound = 4 * TK_GROUPS * TK_BATCH;
   int parts = (p.count + 5 * kRound - 1) / (5 * kRound);
   parts = parts > kMaxParts ? kMaxParts : parts;

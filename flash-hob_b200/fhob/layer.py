@@ -29,8 +29,9 @@ def rotary(x, positions, frequencies, axis_of_pair=None, *, interleaved: bool = 
     ``interleaved``, ``(2j, 2j + 1)``; pair ``j`` turns by ``positions[axis_of_pair[j]] * frequencies[j]`` radians
     (``inverse``: by the negative of that), the other elements are copied.
 
-    ``positions`` are int32 or int64 on the same device, ``(axes, N)`` or ``(axes, B, N)``: any integers, the angle is
-    exact however far they are (see include/fhob.h).  ``frequencies`` is a float32 or float64 vector on the
+    ``positions`` are int32 or int64 on the same device, ``(axes, N)`` or ``(axes, B, N)``: any integers.  The angle is good to
+    ``position * frequency * 2^-52`` radians, a millionth where that product is 2^32 (near 2^52 it says nothing; an fp32 product is off
+    by a radian at 2^24).  ``frequencies`` is a float32 or float64 vector on the
     device, regarded as constant.  ``axis_of_pair`` is a sequence with the axis of every pair; it may be left out
     when there is one axis.
     """

@@ -281,7 +281,7 @@ def flash_bwdbwd(Q, K, V, O, dO, ddQ, ddK, ddV, L, scale, *, is_causal: bool = F
     Same positional signature and return order as the reference
     (fhog/triton_bwdbwd.py:558, :648).  Tensors are ``(BH, N, D)`` like the
     reference or ``(B, H, N, D)``; bfloat16 or float16 (tensor-core kernels,
-    fp32 accumulation) or float32 (tensor cores with every operand split into
+    fp32 accumulation; P and its derivatives are rounded to the type as operands) or float32 (tensor cores with every operand split into
     a bf16 hi + lo pair when D = 64, CUDA-core kernels otherwise).  ``V``, ``O``, ``dO``
     and ``ddV`` may have a head dim of their own (the reference operator has a
     single D, :577; its maths does not need that, jax_refs/flash_impl.py:381-389):
