@@ -32,7 +32,7 @@ def rotary(x, positions, frequencies, axis_of_pair=None, *, interleaved: bool = 
     ``positions`` are int32 or int64 on the same device, ``(axes, N)`` or ``(axes, B, N)``: any integers.  The angle is good to
     ``position * frequency * 2^-52`` radians, a millionth where that product is 2^32 (near 2^52 it says nothing; an fp32 product is off
     by a radian at 2^24).  ``frequencies`` is a float32 or float64 vector on the
-    device, regarded as constant.  ``axis_of_pair`` is a sequence with the axis of every pair; it may be left out
+    device, finite and regarded as constant.  ``axis_of_pair`` is a sequence with the axis of every pair; it may be left out
     when there is one axis.
     """
     several = isinstance(x, (tuple, list))
